@@ -335,6 +335,100 @@ VMOE_API int vmoe_ffn_workspace_size(const vmoe_handle* h, int64_t tokens, size_
 VMOE_API int vmoe_ffn_forward(vmoe_handle* h, const void* x, int64_t tokens, void* out,
                               void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- Dense training operators ----------------------------------------------------------
+ * Operators over weights that stay in the caller's own buffers, in nn.Linear's [out, in]
+ * layout: nothing is packed or kept between calls, so a training loop that changes its
+ * weights every step calls them as they are.  They run on a vmoe_ops context: one per device
+ * and calling thread (calls on one context must not overlap; two contexts may run at once,
+ * each call with its own workspace).  bf16 needs an sm_100 GPU; every product accumulates in
+ * fp32.  Each function returns a status code, enqueues its work on `stream` and allocates
+ * nothing; vmoe_ops_last_error has the text of the last failure. */
+typedef struct vmoe_ops vmoe_ops;
+VMOE_API int vmoe_ops_create(int device, vmoe_ops** out);
+VMOE_API int vmoe_ops_destroy(vmoe_ops* ops);
+VMOE_API const char* vmoe_ops_last_error(const vmoe_ops* ops);
+/* As vmoe_device_status: reads and clears the status word, synchronises `stream`. */
+VMOE_API int vmoe_ops_device_status(vmoe_ops* ops, int32_t* code, void* stream);
+
+/* Activations.  gelu_tanh is GELU's tanh form; ERA = gelu_tanh + gamma * softplus
+ * (python/vesper/model.py:69-76, softplus linear above 20). */
+enum {
+  VMOE_ACT_NONE = 0,
+  VMOE_ACT_RELU = 1,
+  VMOE_ACT_SILU = 2,
+  VMOE_ACT_GELU_TANH = 3,
+  VMOE_ACT_ERA = 4
+};
+
+/* Fused linear:  y = residual + act(x W^T + b), rounded once.  The Linear of the reference's
+ * projections (python/vesper/model.py:83-126, :173-242) with what follows it in a pre-norm
+ * block.  A null bias or residual is left out. */
+typedef struct vmoe_linear {
+  int64_t tokens;       /* T >= 0                                                        */
+  int64_t in_features;  /* K >= 1                                                        */
+  int64_t out_features; /* N >= 1                                                        */
+  int64_t ldx, ldw;     /* row pitches of x [T, K] and W [N, K] in elements, >= K        */
+  int64_t ldr;          /* row pitch of residual [T, N], >= N (ignored without one)      */
+  int32_t dtype;        /* of x, W, bias, residual, y                                    */
+  int32_t activation;   /* VMOE_ACT_*                                                    */
+  float gamma;          /* of VMOE_ACT_ERA                                               */
+  int32_t grad_dtype;   /* of dW and db: the config dtype, or VMOE_F32                   */
+} vmoe_linear;
+
+/* Bytes of workspace of a forward (backward = 0) or a backward (1); 256-byte aligned. */
+VMOE_API int vmoe_linear_workspace_size(vmoe_ops* ops, const vmoe_linear* d, int backward,
+                                        size_t* bytes);
+/* y [T, N] contiguous.  z [T, N] contiguous, optional: the pre-activations x W^T + b, which
+ * the backward of an activation other than VMOE_ACT_NONE reads.  bf16 x and W whose pitch is
+ * a multiple of 8 must start on a 16-byte boundary (other pitches may start anywhere). */
+VMOE_API int vmoe_linear_forward(vmoe_ops* ops, const vmoe_linear* d, const void* x,
+                                 const void* weight, const void* bias, const void* residual,
+                                 void* y, void* z, void* workspace, size_t workspace_bytes,
+                                 void* stream);
+/* dz = dy act'(z);  dx = dz W;  dW = dz^T x;  db = column sums of dz (fp32 sums, fixed order:
+ * two runs give the same bits).  Each output may be null; they are overwritten.  The
+ * residual's gradient is dy itself.  dy [T, N] has row pitch lddy: N, or for bf16 any larger
+ * multiple of 8 (fp32: any), and x's alignment. */
+VMOE_API int vmoe_linear_backward(vmoe_ops* ops, const vmoe_linear* d, const void* x,
+                                  const void* weight, const void* z, const void* dy, int64_t lddy,
+                                  void* dx, void* dweight, void* dbias, void* workspace,
+                                  size_t workspace_bytes, void* stream);
+
+/* Gated feed-forward block (python/vesper/model.py:249-270, :295-298):
+ *   g = x Wg^T + bg;  u = x Wu^T + bu;  h = act(g) * u;  y = residual + h Wd^T + bd
+ * with both projections, the activation and the product in one kernel.  Wg, Wu [I, H],
+ * Wd [H, I]; the weights' rows are contiguous. */
+typedef struct vmoe_gated_ffn {
+  int64_t tokens, hidden, inter; /* T >= 0, H >= 1, I >= 1 */
+  int64_t ldx, ldr;              /* row pitches of x and residual [T, H] */
+  int32_t dtype, activation;     /* any activation but VMOE_ACT_NONE */
+  float gamma;
+  int32_t grad_dtype;
+} vmoe_gated_ffn;
+typedef struct vmoe_ffn_weights {
+  const void *gate_w, *up_w, *down_w; /* required; as x, 16-byte aligned where H (I) % 8 == 0 */
+  const void *gate_b, *up_b, *down_b; /* optional */
+} vmoe_ffn_weights;
+typedef struct vmoe_ffn_grads {       /* each may be null */
+  void *gate_w, *up_w, *down_w, *gate_b, *up_b, *down_b;
+} vmoe_ffn_grads;
+/* workspace of a forward or a backward, and what a training forward keeps (g, u and h) */
+VMOE_API int vmoe_gated_ffn_workspace_size(vmoe_ops* ops, const vmoe_gated_ffn* d, int backward,
+                                           size_t* bytes, size_t* saved_bytes);
+/* `saved` (256-byte aligned): null for inference, else vmoe_gated_ffn_workspace_size's
+ * saved_bytes, untouched until the backward. */
+VMOE_API int vmoe_gated_ffn_forward(vmoe_ops* ops, const vmoe_gated_ffn* d, const void* x,
+                                    const vmoe_ffn_weights* w, const void* residual, void* y,
+                                    void* saved, size_t saved_bytes, void* workspace,
+                                    size_t workspace_bytes, void* stream);
+/*   dh = dy Wd;  dg = dh * u * act'(g);  du = dh * act(g);  dx = dg Wg + du Wu;
+ *   dWg = dg^T x;  dWu = du^T x;  dWd = dy^T h;  the biases' gradients are column sums */
+VMOE_API int vmoe_gated_ffn_backward(vmoe_ops* ops, const vmoe_gated_ffn* d, const void* x,
+                                     const vmoe_ffn_weights* w, const void* dy, int64_t lddy,
+                                     void* dx, const vmoe_ffn_grads* grads, const void* saved,
+                                     size_t saved_bytes, void* workspace, size_t workspace_bytes,
+                                     void* stream);
+
 /* Read (and clear) the device status word the kernels write when a bounded wait gives
  * up or an index check fails.  Synchronises `stream`.  *code = 0 when all is well. */
 VMOE_API int vmoe_device_status(vmoe_handle* h, int32_t* code, void* stream);

@@ -1,0 +1,461 @@
+"""GPU: linear and gated_ffn against 64-bit forms of the same formulas, forward and backward."""
+import pytest
+import torch
+
+from tests import dense_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+GAMMA = 0.1
+ACTS = ["none", "relu", "silu", "gelu_tanh", "era"]
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+def rand(gen, *shape, std=1.0, dtype=BF16):
+    return (torch.randn(*shape, generator=gen, dtype=torch.float32) * std).to(dtype)
+
+
+def d64(t):
+    return None if t is None else t.detach().double().cpu()
+
+
+def leaf(t):
+    return None if t is None else t.cuda().requires_grad_()
+
+
+def run_linear(T, K, N, act="none", dtype=BF16, bias=True, residual=True, seed=0, wdtype=None,
+               train=True):
+    import velvetoptimizer_b200 as vb
+    gen = torch.Generator().manual_seed(seed)
+    wd = wdtype or dtype
+    x, w = rand(gen, T, K, dtype=dtype), rand(gen, N, K, std=K ** -0.5, dtype=wd)
+    b = rand(gen, N, std=0.1, dtype=wd) if bias else None
+    r = rand(gen, T, N, dtype=dtype) if residual else None
+    dy = rand(gen, T, N, dtype=dtype)
+    leaves = [leaf(t) for t in (x, w, b, r)]
+    with torch.set_grad_enabled(train):
+        y = vb.linear(leaves[0], leaves[1], leaves[2], residual=leaves[3], activation=act, gamma=GAMMA)
+    # fp32 parameters of a bf16 call are cast to bf16
+    want = ref.linear(d64(x), d64(w.to(dtype)), d64(None if b is None else b.to(dtype)), d64(r),
+                      d64(dy) if train else None, act, GAMMA, dtype, wd)
+    assert y.dtype == dtype
+    ref.check("y", y, *want["y"], 1, dtype)
+    if not train:
+        assert not y.requires_grad
+        return
+    have = [t for t in leaves if t is not None]
+    grads = torch.autograd.grad(y, have, dy.cuda())
+    names = [n for n, t in zip(("dx", "dw", "db", "dr"), leaves) if t is not None]
+    for n, g, t in zip(names, grads, have):
+        assert g.dtype == t.dtype
+        if n == "dr":
+            assert torch.equal(g.cpu(), dy)
+        else:
+            ref.check(n, g, *want[n], 3, BF16 if BF16 in (dtype, g.dtype) else F32)
+
+
+# one token, the small-batch form's edges (8, 9, 16 | 17), tiles and their edges (256, 257)
+@pytest.mark.parametrize("T", [1, 2, 8, 9, 16, 17, 63, 256, 257])
+@pytest.mark.parametrize("K,N", [(64, 64), (40, 24), (136, 264)])
+def test_linear_sizes(T, K, N):
+    run_linear(T, K, N, act="silu", seed=T + K)
+
+
+# widths that no 16-byte load divides, single columns
+@pytest.mark.parametrize("T,K,N", [(1, 1, 1), (5, 33, 7), (16, 65, 1), (17, 1, 3), (33, 257, 129),
+                                   (300, 31, 513), (129, 7, 255)])
+@pytest.mark.parametrize("act", ["none", "era"])
+def test_linear_odd(T, K, N, act):
+    run_linear(T, K, N, act=act, seed=T)
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("T", [3, 70])
+@pytest.mark.parametrize("bias,residual", [(True, True), (True, False), (False, True), (False, False)])
+def test_linear_forms(act, T, bias, residual):
+    run_linear(T, 72, 48, act=act, bias=bias, residual=residual, seed=T)
+
+
+@pytest.mark.parametrize("T,K,N", [(1, 40, 24), (7, 33, 5), (130, 96, 200), (64, 1000, 16),
+                                   (1000, 24, 40)])
+@pytest.mark.parametrize("act", ["none", "gelu_tanh"])
+def test_linear_f32(T, K, N, act):
+    run_linear(T, K, N, act=act, dtype=F32, seed=T)
+
+
+@pytest.mark.parametrize("T", [5, 90])
+@pytest.mark.parametrize("dtype,wdtype", [(BF16, F32), (F32, BF16)])
+def test_linear_parameters_of_another_type(T, dtype, wdtype):
+    run_linear(T, 48, 40, act="era", dtype=dtype, wdtype=wdtype, seed=3)
+
+
+# k divided over SMs (few tiles, long sums) and many tiles
+@pytest.mark.parametrize("T,K,N", [(64, 4096, 256), (40, 2048, 520), (2100, 72, 136),
+                                   (3000, 256, 2304), (513, 512, 4096)])
+def test_linear_splits(T, K, N):
+    run_linear(T, K, N, act="gelu_tanh", seed=1)
+
+
+@pytest.mark.parametrize("T", [1, 12, 40, 300])
+@pytest.mark.parametrize("act", ["none", "era"])
+def test_linear_inference(T, act):
+    run_linear(T, 264, 104, act=act, seed=2, train=False)
+
+
+def test_linear_empty_batch():
+    import velvetoptimizer_b200 as vb
+    for dtype in (BF16, F32):
+        x = torch.zeros(0, 40, device="cuda", dtype=dtype, requires_grad=True)
+        w = torch.randn(24, 40, device="cuda").to(dtype).requires_grad_()
+        b = torch.zeros(24, device="cuda", dtype=dtype, requires_grad=True)
+        y = vb.linear(x, w, b, activation="era")
+        assert y.shape == (0, 24)
+        dx, dw, db = torch.autograd.grad(y, (x, w, b), torch.zeros_like(y))
+        assert dx.shape == x.shape and not dw.any() and not db.any()
+
+
+def views(gen, T, K, dtype=BF16):
+    """The same kinds of x that a program holds: slices, transposes, expansions, odd starts."""
+    base = rand(gen, T + 2, 2 * K + 16, dtype=dtype).cuda()
+    yield base[1:T + 1, 8:8 + K]                       # aligned column slice, long pitch
+    yield base[1:T + 1, 3:3 + K]                       # starts between 16-byte boundaries
+    yield rand(gen, K, T, dtype=dtype).cuda().t()      # columns contiguous
+    yield rand(gen, 1, K, dtype=dtype).cuda().expand(T, K)
+    yield rand(gen, T, 2 * K, dtype=dtype).cuda()[:, ::2]
+    yield rand(gen, 2 * T, K, dtype=dtype).cuda()[::2]
+    flat = rand(gen, T * (K + 1) + 1, dtype=dtype).cuda()
+    yield flat[1:1 + T * (K + 1)].view(T, K + 1)[:, :K]  # an odd pitch
+
+
+@pytest.mark.parametrize("T", [6, 130])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_linear_strides(T, dtype):
+    import velvetoptimizer_b200 as vb
+    K, N = 64, 56
+    gen = torch.Generator().manual_seed(0)
+    w0 = rand(gen, N, K, std=0.1, dtype=dtype).cuda()
+    dys = list(views(gen, T, N, dtype))
+    for i, x in enumerate(views(gen, T, K, dtype)):
+        wide = rand(gen, N, K + 24, std=0.1, dtype=dtype).cuda()
+        for w in (w0, wide[:, 8:8 + K], wide[:, 5:5 + K], w0.t().contiguous().t()):
+            dy, r = dys[i], dys[(i + 1) % len(dys)]
+            lx, lw = x.detach().requires_grad_(), w.detach().requires_grad_()
+            y = vb.linear(lx, lw, residual=r, activation="silu")
+            dx, dw = torch.autograd.grad(y, (lx, lw), dy)
+            want = ref.linear(d64(x), d64(w), None, d64(r), d64(dy), "silu", GAMMA, dtype)
+            for n, g in (("y", y), ("dx", dx), ("dw", dw)):
+                ref.check(f"{n} of view {i}", g, *want[n], 3, dtype)
+
+
+def test_linear_batched_and_1d():
+    import velvetoptimizer_b200 as vb
+    gen = torch.Generator().manual_seed(0)
+    x, w = rand(gen, 2, 3, 5, 40).cuda(), rand(gen, 24, 40).cuda()
+    y = vb.linear(x, w)
+    assert y.shape == (2, 3, 5, 24)
+    assert torch.equal(y.reshape(30, 24), vb.linear(x.reshape(30, 40), w))
+    assert torch.equal(vb.linear(x[0, 0, 0], w), vb.linear(x[0, 0, :1], w)[0])
+
+
+@pytest.mark.parametrize("T", [4, 200])
+def test_linear_partial_gradients(T):
+    """Only what is asked for is computed, with the same bits."""
+    import velvetoptimizer_b200 as vb
+    gen = torch.Generator().manual_seed(0)
+    base = [rand(gen, T, 72).cuda(), rand(gen, 88, 72, std=0.1).cuda(), rand(gen, 88).cuda(),
+            rand(gen, T, 88).cuda()]
+    dy = rand(gen, T, 88).cuda()
+
+    def grads(mask):
+        p = [t.clone().requires_grad_(bool(m)) for t, m in zip(base, mask)]
+        y = vb.linear(p[0], p[1], p[2], residual=p[3], activation="era")
+        return torch.autograd.grad(y, [t for t in p if t.requires_grad], dy)
+
+    full = grads((1, 1, 1, 1))
+    for mask in [(1, 0, 0, 0), (0, 1, 0, 0), (0, 0, 1, 0), (0, 0, 0, 1), (1, 0, 1, 0), (0, 1, 1, 1)]:
+        want = [g for g, m in zip(full, mask) if m]
+        assert all(torch.equal(a, b) for a, b in zip(grads(mask), want)), mask
+
+
+def run_ffn(T, H, I, act="era", dtype=BF16, bias=True, residual=True, seed=0, wdtype=None, train=True):
+    import velvetoptimizer_b200 as vb
+    gen = torch.Generator().manual_seed(seed)
+    wd = wdtype or dtype
+    x = rand(gen, T, H, dtype=dtype)
+    ws = [rand(gen, I, H, std=H ** -0.5, dtype=wd), rand(gen, I, H, std=H ** -0.5, dtype=wd),
+          rand(gen, H, I, std=I ** -0.5, dtype=wd)]
+    bs = [rand(gen, n, std=0.1, dtype=wd) if bias else None for n in (I, I, H)]
+    r = rand(gen, T, H, dtype=dtype) if residual else None
+    dy = rand(gen, T, H, dtype=dtype)
+    leaves = [leaf(t) for t in (x, *ws, *bs, r)]
+    with torch.set_grad_enabled(train):
+        y = vb.gated_ffn(*leaves[:7], residual=leaves[7], activation=act, gamma=GAMMA)
+    to = lambda t: None if t is None else d64(t.to(dtype))  # noqa: E731
+    want = ref.gated_ffn(d64(x), *map(to, ws), *map(to, bs), d64(r), d64(dy) if train else None,
+                         act, GAMMA, dtype, wd)
+    # h and y rounded
+    ref.check("y", y, *want["y"], 2, dtype)
+    if not train:
+        return
+    have = [t for t in leaves if t is not None]
+    grads = torch.autograd.grad(y, have, dy.cuda())
+    names = [n for n, t in zip(("dx", "dwg", "dwu", "dwd", "dbg", "dbu", "dbd", "dr"), leaves)
+             if t is not None]
+    for n, g, t in zip(names, grads, have):
+        assert g.dtype == t.dtype
+        if n == "dr":
+            assert torch.equal(g.cpu(), dy)
+        else:  # g, u, then dg or du (or h), then the gradient rounded
+            ref.check(n, g, *want[n], 4, dtype)
+
+
+@pytest.mark.parametrize("T", [1, 8, 9, 16, 17, 100, 256, 300])
+@pytest.mark.parametrize("H,I", [(64, 128), (40, 72), (136, 264)])
+def test_gated_ffn_sizes(T, H, I):
+    run_ffn(T, H, I, seed=T)
+
+
+@pytest.mark.parametrize("T,H,I", [(1, 1, 1), (3, 33, 17), (16, 7, 129), (17, 31, 1), (70, 129, 65),
+                                   (260, 65, 257)])
+def test_gated_ffn_odd(T, H, I):
+    run_ffn(T, H, I, seed=T)
+
+
+@pytest.mark.parametrize("act", ACTS[1:])
+@pytest.mark.parametrize("T", [3, 70])
+@pytest.mark.parametrize("bias,residual", [(True, False), (False, True)])
+def test_gated_ffn_forms(act, T, bias, residual):
+    run_ffn(T, 72, 104, act=act, bias=bias, residual=residual, seed=T)
+
+
+@pytest.mark.parametrize("T,H,I", [(1, 40, 24), (9, 33, 21), (140, 72, 200), (70, 520, 48)])
+def test_gated_ffn_f32(T, H, I):
+    run_ffn(T, H, I, dtype=F32, seed=T)
+
+
+@pytest.mark.parametrize("T", [5, 90])
+def test_gated_ffn_f32_parameters(T):
+    run_ffn(T, 48, 72, wdtype=F32, seed=3)
+
+
+@pytest.mark.parametrize("T,H,I", [(40, 1024, 2048), (1500, 256, 640), (700, 520, 1304)])
+def test_gated_ffn_splits(T, H, I):
+    run_ffn(T, H, I, seed=1)
+
+
+@pytest.mark.parametrize("T", [1, 12, 40, 300])
+def test_gated_ffn_inference(T):
+    run_ffn(T, 264, 520, seed=2, train=False)
+
+
+def test_gated_ffn_empty_batch():
+    import velvetoptimizer_b200 as vb
+    for dtype in (BF16, F32):
+        x = torch.zeros(0, 40, device="cuda", dtype=dtype, requires_grad=True)
+        ws = [torch.randn(s, device="cuda").to(dtype).requires_grad_() for s in ((24, 40), (24, 40), (40, 24))]
+        y = vb.gated_ffn(x, *ws)
+        got = torch.autograd.grad(y, (x, *ws), torch.zeros_like(y))
+        assert y.shape == (0, 40) and not any(g.any() for g in got)
+
+
+def test_gated_ffn_partial_gradients():
+    import velvetoptimizer_b200 as vb
+    gen = torch.Generator().manual_seed(0)
+    T, H, I = 150, 72, 104
+    base = [rand(gen, T, H), rand(gen, I, H, std=0.1), rand(gen, I, H, std=0.1), rand(gen, H, I, std=0.1),
+            rand(gen, I), rand(gen, I), rand(gen, H), rand(gen, T, H)]
+    base = [t.cuda() for t in base]
+    dy = rand(gen, T, H).cuda()
+
+    def grads(mask):
+        p = [t.clone().requires_grad_(bool(m)) for t, m in zip(base, mask)]
+        y = vb.gated_ffn(*p[:7], residual=p[7])
+        return torch.autograd.grad(y, [t for t in p if t.requires_grad], dy)
+
+    full = grads([1] * 8)
+    for i in range(8):
+        one = grads([j == i for j in range(8)])
+        # one weight's gradient alone may be divided over k differently: within two roundings
+        assert torch.allclose(one[0].float(), full[i].float(), rtol=2 ** -7, atol=1e-3), i
+
+
+def test_far_values_stay_finite():
+    """Pre-activations far out in the tails: the derivative's polynomial must not overflow."""
+    import velvetoptimizer_b200 as vb
+    for dtype in (BF16, F32):
+        for T in (4, 40):
+            x = torch.ones(T, 8, device="cuda", dtype=dtype)
+            x[1::2] = -1
+            w = torch.full((16, 8), 1e18, device="cuda", dtype=dtype)
+            for act in ACTS:
+                lx, lw = x.clone().requires_grad_(), w.clone().requires_grad_()
+                y = vb.linear(lx, lw, activation=act)
+                assert torch.isfinite(y).all(), act
+                dx, dw = torch.autograd.grad(y, (lx, lw), torch.ones_like(y))
+                assert torch.isfinite(dx).all() and torch.isfinite(dw).all(), act
+
+
+def test_nan_and_inf_pass_through():
+    import velvetoptimizer_b200 as vb
+    for dtype in (BF16, F32):
+        for T in (4, 40):
+            x = torch.zeros(T, 16, device="cuda", dtype=dtype)
+            x[1, 3], x[2, 5] = float("nan"), float("inf")
+            w = torch.ones(24, 16, device="cuda", dtype=dtype)
+            for act in ACTS:
+                y = vb.linear(x, w, activation=act)
+                assert torch.isnan(y[1]).all() and torch.isinf(y[2]).all(), (act, dtype, T)
+                assert torch.isfinite(y[0]).all() and torch.isfinite(y[3:]).all()
+
+
+@pytest.mark.parametrize("T", [5, 100])
+def test_gradients_against_differences(T):
+    """fp32: <gradient, v> against the difference of the operators' own values along v.
+
+    With f = <dy, op(p)> the central difference has a truncation error of eps^2 / 6 |f'''| and a
+    rounding error of about |f| 2^-23 sqrt(n) / eps; at eps = 2^-6 both are below 1e-3 of the
+    norms used here, the allowance is 5e-3 of |gradient| |v|.
+    """
+    import velvetoptimizer_b200 as vb
+    gen = torch.Generator().manual_seed(5)
+    H, I = 24, 40
+    p = [rand(gen, T, H, dtype=F32), rand(gen, I, H, std=0.2, dtype=F32),
+         rand(gen, I, H, std=0.2, dtype=F32), rand(gen, H, I, std=0.2, dtype=F32),
+         rand(gen, I, dtype=F32), rand(gen, I, dtype=F32), rand(gen, H, dtype=F32)]
+    p = [t.cuda() for t in p]
+    dy, dz = rand(gen, T, H, dtype=F32).cuda(), rand(gen, T, I, dtype=F32).cuda()
+
+    def ffn(q):
+        return vb.gated_ffn(*q)
+
+    def lin(q):
+        return vb.linear(q[0], q[1], q[4], activation="era")
+
+    for fn, cot, used in ((ffn, dy, range(7)), (lin, dz, (0, 1, 4))):
+        leaves = [t.clone().requires_grad_() for t in p]
+        grads = torch.autograd.grad(fn(leaves), [leaves[i] for i in used], cot)
+        for i, g in zip(used, grads):
+            v = torch.randn(p[i].shape, generator=gen).cuda()
+            eps = 2.0 ** -6 / float(v.abs().max())
+            with torch.no_grad():
+                at = [[(t + s * eps * v) if j == i else t for j, t in enumerate(p)] for s in (1, -1)]
+                diff = (cot.double() * (fn(at[0]).double() - fn(at[1]).double())).sum() / (2 * eps)
+            dot = (g.double() * v.double()).sum()
+            assert abs(float(dot - diff)) <= 5e-3 * float(g.norm() * v.norm()), i
+
+
+def test_same_bits_every_run():
+    import velvetoptimizer_b200 as vb
+    gen = torch.Generator().manual_seed(0)
+    for T, H, I in ((12, 264, 520), (64, 1024, 2048), (700, 256, 640)):
+        p = [rand(gen, T, H), rand(gen, I, H, std=0.05), rand(gen, I, H, std=0.05),
+             rand(gen, H, I, std=0.05), rand(gen, I), rand(gen, I), rand(gen, H)]
+        p = [t.cuda().requires_grad_() for t in p]
+        dy = rand(gen, T, H).cuda()
+        first = None
+        for _ in range(4):
+            y = vb.gated_ffn(*p)
+            got = [y, *torch.autograd.grad(y, p, dy)]
+            first = first or got
+            assert all(torch.equal(a, b) for a, b in zip(first, got))
+
+
+def test_captured_and_replayed():
+    """Forward and backward in a CUDA graph, replayed on new inputs."""
+    import velvetoptimizer_b200 as vb
+    gen = torch.Generator().manual_seed(0)
+    for T in (8, 150):
+        H, I = 72, 136
+        shapes = ((T, H), (I, H), (I, H), (H, I), (I,), (I,), (H,))
+        p = [rand(gen, *s, std=0.1).cuda().requires_grad_() for s in shapes]
+        dy = rand(gen, T, H).cuda()
+
+        def step():
+            y = vb.linear(vb.gated_ffn(*p, residual=p[0]), p[1], p[4], activation="silu")
+            return [y, *torch.autograd.grad(y.float().square().sum(), p)]
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            for _ in range(2):
+                step()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+        for k in range(2):
+            with torch.no_grad():
+                p[0].copy_(rand(gen, T, H, std=0.1 * (k + 1)))
+            graph.replay()
+            torch.cuda.synchronize()
+            captured = [t.detach().clone() for t in out]
+            assert all(torch.equal(a, b) for a, b in zip(captured, step()))
+        del graph, out, dy
+
+
+def test_two_streams_and_two_threads():
+    """Calls at the same time, each with its own workspace and context, give the same bits."""
+    import threading
+
+    import velvetoptimizer_b200 as vb
+    gen = torch.Generator().manual_seed(0)
+    T, H, I = 64, 1024, 2048
+    sets = []
+    for _ in range(2):
+        p = [rand(gen, T, H), rand(gen, I, H, std=0.05), rand(gen, I, H, std=0.05),
+             rand(gen, H, I, std=0.05)]
+        sets.append([t.cuda() for t in p])
+    alone = [vb.gated_ffn(*p) for p in sets]
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def work(k):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(20):
+                got[k].append(vb.gated_ffn(*sets[k]))
+        s.synchronize()
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for k in range(2):
+        assert len(got[k]) == 20 and all(torch.equal(g, alone[k]) for g in got[k])
+
+
+def test_refusals():
+    import velvetoptimizer_b200 as vb
+    x = torch.zeros(4, 16, device="cuda", dtype=BF16)
+    w = torch.zeros(24, 16, device="cuda", dtype=BF16)
+    with pytest.raises(TypeError):
+        vb.linear(x.half(), w)
+    with pytest.raises(TypeError):
+        vb.linear(x, w.half())
+    with pytest.raises(ValueError):
+        vb.linear(x, w[:, :8])
+    with pytest.raises(ValueError):
+        vb.linear(x, w, torch.zeros(23, device="cuda", dtype=BF16))
+    with pytest.raises(ValueError):
+        vb.linear(x, w.cpu())
+    with pytest.raises(ValueError):
+        vb.linear(x, w, activation="tanh")
+    with pytest.raises(ValueError):
+        vb.linear(x, w, residual=torch.zeros(4, 16, device="cuda", dtype=BF16))
+    with pytest.raises(TypeError):
+        vb.linear(x, w, residual=torch.zeros(4, 24, device="cuda"))
+    with pytest.raises(ValueError):
+        vb.linear(x, torch.zeros(0, 16, device="cuda", dtype=BF16))
+    with pytest.raises(ValueError):
+        vb.gated_ffn(x, w, w, w.t(), activation="none")
+    with pytest.raises(ValueError):
+        vb.gated_ffn(x, w, w, w)
+    with pytest.raises(ValueError):
+        vb.gated_ffn(x, w, w[:8], w.t())
+
+
+def test_device_status_clean():
+    from velvetoptimizer_b200.dense import ops_for
+    torch.cuda.synchronize()
+    assert ops_for(torch.device("cuda")).device_status(torch.cuda.current_stream().cuda_stream) == 0

@@ -42,6 +42,9 @@ EXPORTED = (
     "vmoe_set_norm", "vmoe_forward_residual", "vmoe_set_training", "vmoe_train_workspace_size",
     "vmoe_forward_train", "vmoe_backward", "vmoe_backward_stage_times",
     "vmoe_backward_stage_name",
+    "vmoe_ops_create", "vmoe_ops_destroy", "vmoe_ops_last_error", "vmoe_ops_device_status",
+    "vmoe_linear_workspace_size", "vmoe_linear_forward", "vmoe_linear_backward",
+    "vmoe_gated_ffn_workspace_size", "vmoe_gated_ffn_forward", "vmoe_gated_ffn_backward",
 )
 
 
@@ -77,6 +80,26 @@ class VmoeWsLayout(ctypes.Structure):
     _fields_ = [("slot_of", c_size_t), ("expert_offsets", c_size_t), ("num_tiles", c_size_t),
                 ("x_perm", c_size_t), ("h", c_size_t), ("y", c_size_t), ("max_rows", c_int64),
                 ("h_ld", c_int64), ("y_ld", c_int64), ("total", c_size_t)]
+
+
+class VmoeLinear(ctypes.Structure):
+    _fields_ = [("tokens", c_int64), ("in_features", c_int64), ("out_features", c_int64),
+                ("ldx", c_int64), ("ldw", c_int64), ("ldr", c_int64), ("dtype", c_int32),
+                ("activation", c_int32), ("gamma", c_float), ("grad_dtype", c_int32)]
+
+
+class VmoeGatedFfn(ctypes.Structure):
+    _fields_ = [("tokens", c_int64), ("hidden", c_int64), ("inter", c_int64), ("ldx", c_int64),
+                ("ldr", c_int64), ("dtype", c_int32), ("activation", c_int32), ("gamma", c_float),
+                ("grad_dtype", c_int32)]
+
+
+class VmoeFfnWeights(ctypes.Structure):
+    _fields_ = [(n, c_void_p) for n in ("gate_w", "up_w", "down_w", "gate_b", "up_b", "down_b")]
+
+
+class VmoeFfnGrads(ctypes.Structure):
+    _fields_ = [(n, c_void_p) for n in ("gate_w", "up_w", "down_w", "gate_b", "up_b", "down_b")]
 
 
 class VmoeError(RuntimeError):
@@ -190,6 +213,35 @@ def load() -> ctypes.CDLL:
     lib.vmoe_last_error.restype = c_char_p
     lib.vmoe_status_string.argtypes = [c_int]
     lib.vmoe_status_string.restype = c_char_p
+    lib.vmoe_ops_create.argtypes = [c_int, POINTER(H)]
+    lib.vmoe_ops_create.restype = c_int
+    lib.vmoe_ops_destroy.argtypes = [H]
+    lib.vmoe_ops_destroy.restype = c_int
+    lib.vmoe_ops_last_error.argtypes = [H]
+    lib.vmoe_ops_last_error.restype = c_char_p
+    lib.vmoe_ops_device_status.argtypes = [H, POINTER(c_int32), c_void_p]
+    lib.vmoe_ops_device_status.restype = c_int
+    lib.vmoe_linear_workspace_size.argtypes = [H, POINTER(VmoeLinear), c_int, POINTER(c_size_t)]
+    lib.vmoe_linear_workspace_size.restype = c_int
+    lib.vmoe_linear_forward.argtypes = [H, POINTER(VmoeLinear), c_void_p, c_void_p, c_void_p,
+                                        c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]
+    lib.vmoe_linear_forward.restype = c_int
+    lib.vmoe_linear_backward.argtypes = [H, POINTER(VmoeLinear), c_void_p, c_void_p, c_void_p,
+                                         c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,
+                                         c_size_t, c_void_p]
+    lib.vmoe_linear_backward.restype = c_int
+    lib.vmoe_gated_ffn_workspace_size.argtypes = [H, POINTER(VmoeGatedFfn), c_int,
+                                                  POINTER(c_size_t), POINTER(c_size_t)]
+    lib.vmoe_gated_ffn_workspace_size.restype = c_int
+    lib.vmoe_gated_ffn_forward.argtypes = [H, POINTER(VmoeGatedFfn), c_void_p,
+                                           POINTER(VmoeFfnWeights), c_void_p, c_void_p, c_void_p,
+                                           c_size_t, c_void_p, c_size_t, c_void_p]
+    lib.vmoe_gated_ffn_forward.restype = c_int
+    lib.vmoe_gated_ffn_backward.argtypes = [H, POINTER(VmoeGatedFfn), c_void_p,
+                                            POINTER(VmoeFfnWeights), c_void_p, c_int64, c_void_p,
+                                            POINTER(VmoeFfnGrads), c_void_p, c_size_t, c_void_p,
+                                            c_size_t, c_void_p]
+    lib.vmoe_gated_ffn_backward.restype = c_int
     lib.vmoe_abi_version.argtypes = []
     lib.vmoe_abi_version.restype = c_int
     _lib = lib
@@ -324,3 +376,37 @@ class Handle:
 
     def last_launch_count(self) -> int:
         return int(self.lib.vmoe_last_launch_count(self.ptr))
+
+
+class Ops:
+    """Owns one ``vmoe_ops`` context: the dense operators' calls of one thread on one device."""
+
+    def __init__(self, device: int):
+        self.lib = load()
+        self.device = device
+        self.ptr = c_void_p()
+        check(self.lib.vmoe_ops_create(device, ctypes.byref(self.ptr)), None, "vmoe_ops_create")
+
+    def close(self) -> None:
+        if self.ptr:
+            self.lib.vmoe_ops_destroy(self.ptr)
+            self.ptr = c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def check(self, rc: int, what: str) -> None:
+        if rc == VMOE_OK:
+            return
+        detail = (self.lib.vmoe_ops_last_error(self.ptr) or b"").decode()
+        status = (self.lib.vmoe_status_string(rc) or b"").decode()
+        raise VmoeError(rc, f"{what} failed: {status}" + (f" ({detail})" if detail else ""))
+
+    def device_status(self, stream: int) -> int:
+        code = c_int32()
+        self.check(self.lib.vmoe_ops_device_status(self.ptr, ctypes.byref(code), c_void_p(stream)),
+                   "vmoe_ops_device_status")
+        return code.value

@@ -1,0 +1,118 @@
+// Kernel launchers of the dense training operators (fused linear, gated feed-forward,
+// gradient norm): the interface between their kernels and the C-ABI host side in dense.cu
+// and grad_norm.cu.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace vmoe {
+
+// activations, the values of VMOE_ACT_*
+enum Act : int { kActNone = 0, kActRelu = 1, kActSilu = 2, kActGeluTanh = 3, kActEra = 4 };
+
+// What happens to an accumulated product on its way to memory.
+//   kEpiLinear  z = acc + bias; [z kept]; out = res + act(z)
+//   kEpiGated   g = acc_g + bias, u = acc_u + bias2; [g, u kept]; out = act(g) * u
+//   kEpiGluBwd  acc = dh, g and u read: out = dh * u * act'(g), out2 = dh * act(g)
+enum EpiKind : int { kEpiLinear = 0, kEpiGated = 1, kEpiGluBwd = 2 };
+
+// `vec` bits: the buffer's base and row pitch allow 16-byte accesses
+enum : int { kVecOut = 1, kVecRes = 2, kVecZ = 4 };
+
+struct DenseEpi {
+  int act = kActNone;
+  float gamma = 0.f;
+  const void* bias = nullptr;   // [N], the operands' type
+  const void* bias2 = nullptr;  // kEpiGated: the up projection's
+  const void* res = nullptr;
+  int64_t ldr = 0;
+  void* out = nullptr;
+  void* out2 = nullptr;  // kEpiGluBwd: du; second group of a grouped launch: its output
+  int64_t ldo = 0;
+  void* z = nullptr;   // kept pre-activations (linear: z, gated: g; glu backward reads g)
+  void* z2 = nullptr;  // u
+  int64_t ldz = 0;
+  int out_f32 = 0;  // out is fp32 (gradients of fp32 parameters)
+  int vec = 0;
+};
+
+// One product C[M, N] = sum over k of A(m, k) B(n, k) on CTA pairs (gemm_dense.cu).
+struct DenseGemm {
+  int64_t M = 0, N = 0;  // valid rows and columns (kEpiGated: N = features)
+  int m_tiles = 0, n_tiles = 0;
+  int groups = 1;        // independent products sharing B: A map g, output out / out2
+  int kb0 = 0, kb1 = 0;  // 64-wide k blocks of the first and second operand pair
+  int splits = 1, kb_per_split = 0;
+  int band = 0;          // n tiles per band of the tile order
+  float* partial = nullptr;  // splits > 1: [splits][groups][M][ldp]
+  int64_t ldp = 0;
+  DenseEpi epi;
+  int* status = nullptr;
+};
+
+struct DenseMaps {
+  CUtensorMap a0, a1, b0, b1;
+};
+
+// a_mn / b_mn: the operand is stored [k rows, M (or N) columns] and read MN-major;
+// otherwise [M (or N) rows, k columns].  Built combinations: K-K (forward), K-MN (input
+// gradients), MN-MN (weight gradients).
+cudaError_t launch_gemm_dense(bool a_mn, bool b_mn, int epi, const DenseMaps& maps,
+                              const DenseGemm& g, int num_sms, cudaStream_t s);
+
+// Sum of a split product's partials in split order, then its epilogue (dense_finish.cu).
+cudaError_t launch_dense_finish(int dtype, int epi, const DenseGemm& g, cudaStream_t s);
+
+// fp32 products on the CUDA cores, partials only (dense_simt.cu): element (m, k) of A at
+// a[m * am + k * ak], (n, k) of B at b[n * bn + k * bk].
+struct SimtGemm {
+  const float *a, *b;
+  int64_t am, ak, bn, bk;
+  int64_t M, N, K;
+  int splits;
+  int64_t k_per_split;
+  float* partial;  // [splits][.][ldp]; split s at partial + s * split_stride
+  int64_t ldp, split_stride;
+  int gated_cols;  // 0 plain; 1 / 2: gate / up columns of the 128-feature interleave
+};
+cudaError_t launch_dense_simt(const SimtGemm& g, cudaStream_t s);
+
+// Few rows (at most kSmallTokens): weights streamed once through registers (dense_small.cu).
+constexpr int kSmallTokens = 16;
+struct SmallGemm {
+  const void* x;
+  const void* w;   // [N, K]; kEpiGated: gate weight
+  const void* w2;  // kEpiGated: up weight
+  int64_t ldx, ldw, ldw2;
+  int64_t T, N, K;
+  DenseEpi epi;
+  int vec_in;  // x and the weights allow 16-byte loads
+};
+cudaError_t launch_dense_small(int epi, const SmallGemm& g, cudaStream_t s);
+
+// Elementwise and column work (dense_finish.cu).
+// dz = dy * act'(z) into dz [T, ld_dz] (null: not written), and the column sums of dz.
+struct DzArgs {
+  const void* dy;
+  int64_t lddy;
+  const void* z;
+  int64_t ldz;
+  void* dz;
+  int64_t lddz;
+  int64_t T, N;
+  int act;
+  float gamma;
+  float* colsum;  // [row_blocks][N] partials, or null
+  int row_blocks;
+  int64_t rows_per_block;
+};
+cudaError_t launch_dense_dz(int dtype, const DzArgs& a, cudaStream_t s);
+cudaError_t launch_colsum_finish(const float* partial, int row_blocks, int64_t N, void* out,
+                                 bool out_f32, cudaStream_t s);
+// rows of bf16 to a buffer whose pitch is a multiple of 8
+cudaError_t launch_pad_copy(const void* src, int64_t lds, int64_t rows, int64_t cols, void* dst,
+                            int64_t ldd, cudaStream_t s);
+
+}  // namespace vmoe

@@ -1,0 +1,232 @@
+// The elementwise and column kernels around the dense products.
+//
+//   finish   sums a split product's fp32 partials in split order and runs the epilogue
+//   dz       dz = dy act'(z) with the column sums of dz (the bias gradient) in the same pass;
+//            also the plain column sums, and the copy of dy to a pitch the TMA can read
+//   colsum   adds the row blocks' column sums in block order
+// All are bound by the bytes they move: 16-byte accesses where the buffers allow them.
+#include "common.cuh"
+#include "dense.h"
+#include "dense_act.cuh"
+
+namespace vmoe {
+namespace {
+
+constexpr int V = 8;  // columns per thread of the finish kernel
+
+template <typename T, int EPI>
+__global__ void __launch_bounds__(256)
+dense_finish_kernel(const DenseGemm g) {
+  constexpr bool kFast = sizeof(T) == 2;
+  const DenseEpi& ep = g.epi;
+  const int64_t per_row = (g.N + V - 1) / V;
+  const int64_t total = g.M * per_row;
+  const int grp = blockIdx.y;
+  const int64_t split_stride = static_cast<int64_t>(g.groups) * g.M * g.ldp;
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
+    const int64_t row = i / per_row, col = (i - row * per_row) * V;
+    const int64_t valid = g.N - col;
+    const int64_t pcol = EPI == kEpiGated ? (col / 128) * 256 + (col & 127) : col;
+    const float* p = g.partial + (static_cast<int64_t>(grp) * g.M + row) * g.ldp + pcol;
+    float v[V] = {}, u[V] = {};
+    for (int s = 0; s < g.splits; ++s, p += split_stride) {
+      float t[V];
+      load_row<V, float>(p, t, V, true);
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] += t[j];
+      if constexpr (EPI == kEpiGated) {
+        load_row<V, float>(p + 128, t, V, true);
+#pragma unroll
+        for (int j = 0; j < V; ++j) u[j] += t[j];
+      }
+    }
+    if constexpr (EPI == kEpiGluBwd) {
+      float gg[V];
+      load_row<V>(static_cast<const T*>(ep.z) + row * ep.ldz + col, gg, valid, ep.vec & kVecZ);
+      load_row<V>(static_cast<const T*>(ep.z2) + row * ep.ldz + col, u, valid, ep.vec & kVecZ);
+      act_switch(ep.act, [&](auto A) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          float a, d;
+          act_grad<kFast, decltype(A)::value>(gg[j], ep.gamma, a, d);
+          gg[j] = v[j] * u[j] * d;
+          u[j] = v[j] * a;
+        }
+      });
+      store_row<V>(static_cast<T*>(ep.out) + row * ep.ldo + col, gg, valid, ep.vec & kVecOut);
+      store_row<V>(static_cast<T*>(ep.out2) + row * ep.ldo + col, u, valid, ep.vec & kVecOut);
+      continue;
+    }
+    if (ep.bias) {
+      float b[V];
+      load_row<V>(static_cast<const T*>(ep.bias) + col, b, valid, false);
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] += b[j];
+    }
+    if constexpr (EPI == kEpiGated) {
+      if (ep.bias2) {
+        float b[V];
+        load_row<V>(static_cast<const T*>(ep.bias2) + col, b, valid, false);
+#pragma unroll
+        for (int j = 0; j < V; ++j) u[j] += b[j];
+      }
+      if (ep.z) {
+        store_row<V>(static_cast<T*>(ep.z) + row * ep.ldz + col, v, valid, ep.vec & kVecZ);
+        store_row<V>(static_cast<T*>(ep.z2) + row * ep.ldz + col, u, valid, ep.vec & kVecZ);
+      }
+      act_switch(ep.act, [&](auto A) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = act_value<kFast, decltype(A)::value>(v[j], ep.gamma) * u[j];
+      });
+    } else {
+      if (ep.z) store_row<V>(static_cast<T*>(ep.z) + row * ep.ldz + col, v, valid, ep.vec & kVecZ);
+      act_switch(ep.act, [&](auto A) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = act_value<kFast, decltype(A)::value>(v[j], ep.gamma);
+      });
+      if (ep.res) {
+        float r[V];
+        load_row<V>(static_cast<const T*>(ep.res) + row * ep.ldr + col, r, valid, ep.vec & kVecRes);
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] += r[j];
+      }
+    }
+    void* out = grp ? ep.out2 : ep.out;
+    if (ep.out_f32)
+      store_row<V>(static_cast<float*>(out) + row * ep.ldo + col, v, valid, ep.vec & kVecOut);
+    else
+      store_row<V>(static_cast<T*>(out) + row * ep.ldo + col, v, valid, ep.vec & kVecOut);
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256)
+dense_dz_kernel(const DzArgs a, bool vec_dy, bool vec_z, bool vec_dz) {
+  constexpr int W = Vec16<T>::N;
+  constexpr bool kFast = sizeof(T) == 2;
+  __shared__ float red[8][32 * W];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int64_t col = (static_cast<int64_t>(blockIdx.x) * 32 + tx) * W;
+  const int64_t valid = a.N - col;
+  const int64_t r0 = blockIdx.y * a.rows_per_block;
+  const int64_t r1 = min(a.T, r0 + a.rows_per_block);
+  float sum[W] = {};
+  if (valid > 0) {
+    for (int64_t r = r0 + ty; r < r1; r += 8) {
+      float v[W];
+      load_row<W>(static_cast<const T*>(a.dy) + r * a.lddy + col, v, valid, vec_dy);
+      if (a.act != kActNone) {
+        float z[W];
+        load_row<W>(static_cast<const T*>(a.z) + r * a.ldz + col, z, valid, vec_z);
+        act_switch(a.act, [&](auto A) {
+#pragma unroll
+          for (int j = 0; j < W; ++j) {
+            float y, d;
+            act_grad<kFast, decltype(A)::value>(z[j], a.gamma, y, d);
+            v[j] *= d;
+          }
+        });
+      }
+      if (a.dz)
+        store_row<W>(static_cast<T*>(a.dz) + r * a.lddz + col, v, valid, vec_dz);
+#pragma unroll
+      for (int j = 0; j < W; ++j) sum[j] += v[j];
+    }
+  }
+  if (!a.colsum) return;
+#pragma unroll
+  for (int j = 0; j < W; ++j) red[ty][tx * W + j] = sum[j];
+  __syncthreads();
+  for (int c = threadIdx.x; c < 32 * W; c += 256) {
+    const int64_t n = static_cast<int64_t>(blockIdx.x) * 32 * W + c;
+    if (n >= a.N) continue;
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s += red[k][c];
+    a.colsum[blockIdx.y * a.N + n] = s;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256)
+colsum_finish_kernel(const float* partial, int row_blocks, int64_t N, T* out) {
+  const int64_t n = blockIdx.x * 256ll + threadIdx.x;
+  if (n >= N) return;
+  float s = 0.f;
+#pragma unroll 8
+  for (int b = 0; b < row_blocks; ++b) s += partial[b * N + n];
+  out[n] = Elt<T>::from_f(s);
+}
+
+__global__ void __launch_bounds__(256)
+pad_copy_kernel(const unsigned short* src, int64_t lds, int64_t rows, int64_t cols,
+                unsigned short* dst, int64_t ldd) {
+  const int64_t total = rows * ldd;
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
+    const int64_t r = i / ldd, c = i - r * ldd;
+    dst[i] = c < cols ? src[r * lds + c] : 0;
+  }
+}
+
+unsigned blocks_for(int64_t threads) {
+  const int64_t b = (threads + 255) / 256;
+  return static_cast<unsigned>(b < 148 * 16 ? (b > 0 ? b : 1) : 148 * 16);
+}
+
+template <typename T>
+bool vec_ok(const void* p, int64_t ld) {
+  return ((reinterpret_cast<uintptr_t>(p) | static_cast<uintptr_t>(ld * sizeof(T))) & 15u) == 0;
+}
+
+}  // namespace
+
+cudaError_t launch_dense_finish(int dtype, int epi, const DenseGemm& g, cudaStream_t s) {
+  const dim3 grid(blocks_for(g.M * ((g.N + V - 1) / V)), static_cast<unsigned>(g.groups));
+  if (dtype == kF32) {
+    if (epi == kEpiGated) dense_finish_kernel<float, kEpiGated><<<grid, 256, 0, s>>>(g);
+    else if (epi == kEpiGluBwd) dense_finish_kernel<float, kEpiGluBwd><<<grid, 256, 0, s>>>(g);
+    else dense_finish_kernel<float, kEpiLinear><<<grid, 256, 0, s>>>(g);
+  } else {
+    using B = __nv_bfloat16;
+    if (epi == kEpiGated) dense_finish_kernel<B, kEpiGated><<<grid, 256, 0, s>>>(g);
+    else if (epi == kEpiGluBwd) dense_finish_kernel<B, kEpiGluBwd><<<grid, 256, 0, s>>>(g);
+    else dense_finish_kernel<B, kEpiLinear><<<grid, 256, 0, s>>>(g);
+  }
+  return cudaGetLastError();
+}
+
+cudaError_t launch_dense_dz(int dtype, const DzArgs& a, cudaStream_t s) {
+  const int width = 32 * (dtype == kF32 ? 4 : 8);
+  const dim3 grid(static_cast<unsigned>((a.N + width - 1) / width),
+                  static_cast<unsigned>(a.row_blocks));
+  if (dtype == kF32)
+    dense_dz_kernel<float><<<grid, 256, 0, s>>>(a, vec_ok<float>(a.dy, a.lddy),
+                                                vec_ok<float>(a.z, a.ldz),
+                                                vec_ok<float>(a.dz, a.lddz));
+  else
+    dense_dz_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(a, vec_ok<__nv_bfloat16>(a.dy, a.lddy),
+                                                        vec_ok<__nv_bfloat16>(a.z, a.ldz),
+                                                        vec_ok<__nv_bfloat16>(a.dz, a.lddz));
+  return cudaGetLastError();
+}
+
+cudaError_t launch_colsum_finish(const float* partial, int row_blocks, int64_t N, void* out,
+                                 bool out_f32, cudaStream_t s) {
+  const unsigned grid = static_cast<unsigned>((N + 255) / 256);
+  if (out_f32)
+    colsum_finish_kernel<float><<<grid, 256, 0, s>>>(partial, row_blocks, N, static_cast<float*>(out));
+  else
+    colsum_finish_kernel<__nv_bfloat16>
+        <<<grid, 256, 0, s>>>(partial, row_blocks, N, static_cast<__nv_bfloat16*>(out));
+  return cudaGetLastError();
+}
+
+cudaError_t launch_pad_copy(const void* src, int64_t lds, int64_t rows, int64_t cols, void* dst,
+                            int64_t ldd, cudaStream_t s) {
+  pad_copy_kernel<<<blocks_for(rows * ldd), 256, 0, s>>>(static_cast<const unsigned short*>(src), lds,
+                                                         rows, cols,
+                                                         static_cast<unsigned short*>(dst), ldd);
+  return cudaGetLastError();
+}
+
+}  // namespace vmoe

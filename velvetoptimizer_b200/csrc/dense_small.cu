@@ -1,0 +1,157 @@
+// Fused linear and gated projection for few rows (T <= 16): the weights are the work.
+//
+//   out[t, n] = epilogue(sum_k w[n, k] x[t, k])
+//
+// Bound: each weight is read once and used T times, so the kernel is as fast as the weights
+// stream in.  mma.sync m16n8k16 takes 16 weight rows as its M operand and 8 tokens as N; the
+// products cost nothing next to the loads, and both operands come straight from global memory
+// in fragment order with 16-byte loads: k is only summed over, so within 32 consecutive k
+// lane t of a row takes k = 8t..8t+7 and hands them to two MMAs as their (2t, 2t+1, 2t+8,
+// 2t+9) pairs, the same permutation for weights and tokens.  No shared memory or barrier
+// stands between a load and its use; four 32-wide chunks of two weight rows per lane are in
+// flight.  A block owns 16 weight rows, its 8 warps take every eighth chunk and add their
+// sums through shared memory in warp order.  The gated form takes 8 gate rows and 8 up rows
+// of the same features as the 16, so one thread ends up with both.
+#include "common.cuh"
+#include "dense.h"
+#include "dense_act.cuh"
+
+namespace vmoe {
+namespace {
+
+constexpr int WARPS = 8;
+constexpr int UNROLL = 4;
+
+__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                         uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// 8 elements of a row from k on, 0 past K or without a row
+template <bool VEC>
+__device__ __forceinline__ uint4 load8(const __nv_bfloat16* row, int64_t k, int64_t K) {
+  uint4 v = make_uint4(0, 0, 0, 0);
+  if (!row) return v;
+  if constexpr (VEC) {  // K % 8 == 0 and 16-byte aligned rows
+    if (k < K) v = __ldg(reinterpret_cast<const uint4*>(row + k));
+  } else {
+    const auto* p = reinterpret_cast<const unsigned short*>(row);
+    uint32_t e[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) e[j] = k + j < K ? __ldg(p + k + j) : 0u;
+    v = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+  }
+  return v;
+}
+
+template <int EPI, bool VEC, int NT>
+__global__ void __launch_bounds__(32 * WARPS)
+dense_small_kernel(const SmallGemm g) {
+  constexpr bool kGate = EPI == kEpiGated;
+  constexpr int ROWS = kGate ? 8 : 16;  // output features per block
+  __shared__ float red[WARPS][NT][32][4];
+  __shared__ float sum[NT][16][8];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int gid = lane >> 2, tig = lane & 3;
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * ROWS;
+  pdl_wait_and_trigger();
+
+  const auto* w = static_cast<const __nv_bfloat16*>(g.w);
+  const auto* w2 = static_cast<const __nv_bfloat16*>(g.w2);
+  const auto* x = static_cast<const __nv_bfloat16*>(g.x);
+  const __nv_bfloat16* r0 = n0 + gid < g.N ? w + (n0 + gid) * g.ldw : nullptr;
+  const __nv_bfloat16* r1;
+  if constexpr (kGate) {
+    r1 = n0 + gid < g.N ? w2 + (n0 + gid) * g.ldw2 : nullptr;
+  } else {
+    r1 = n0 + gid + 8 < g.N ? w + (n0 + gid + 8) * g.ldw : nullptr;
+  }
+  const __nv_bfloat16* xr[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) xr[n] = n * 8 + gid < g.T ? x + (n * 8 + gid) * g.ldx : nullptr;
+
+  float acc[NT][4] = {};
+  const int64_t chunks = (g.K + 31) / 32;
+  for (int64_t c = warp; c < chunks; c += WARPS * UNROLL) {
+    uint4 a[UNROLL], b[UNROLL], v[UNROLL][NT];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const int64_t k = (c + u * WARPS) * 32 + tig * 8;  // past K: zeros
+      a[u] = load8<VEC>(r0, k, g.K);
+      b[u] = load8<VEC>(r1, k, g.K);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) v[u][n] = load8<VEC>(xr[n], k, g.K);
+    }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        mma_bf16(acc[n], a[u].x, b[u].x, a[u].y, b[u].y, v[u][n].x, v[u][n].y);
+        mma_bf16(acc[n], a[u].z, b[u].z, a[u].w, b[u].w, v[u][n].z, v[u][n].w);
+      }
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) red[warp][n][lane][i] = acc[n][i];
+  __syncthreads();
+  if (threadIdx.x < NT * 128) {
+    const int n = threadIdx.x >> 7, l = (threadIdx.x >> 2) & 31, i = threadIdx.x & 3;
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < WARPS; ++k) s += red[k][n][l][i];
+    sum[n][(l >> 2) + 8 * (i >> 1)][(l & 3) * 2 + (i & 1)] = s;
+  }
+  __syncthreads();
+  const int f = threadIdx.x % ROWS, t = threadIdx.x / ROWS;
+  const int64_t col = n0 + f;
+  if (t >= g.T || t >= NT * 8 || col >= g.N) return;
+  const DenseEpi& ep = g.epi;
+  auto bias = [&](const void* p) {
+    return p ? __bfloat162float(static_cast<const __nv_bfloat16*>(p)[col]) : 0.f;
+  };
+  float z = sum[t >> 3][f][t & 7] + bias(ep.bias);
+  auto* zp = static_cast<__nv_bfloat16*>(ep.z);
+  auto* out = static_cast<__nv_bfloat16*>(ep.out);
+  if constexpr (kGate) {
+    const float up = sum[t >> 3][f + 8][t & 7] + bias(ep.bias2);
+    if (zp) {
+      zp[t * ep.ldz + col] = __float2bfloat16_rn(z);
+      static_cast<__nv_bfloat16*>(ep.z2)[t * ep.ldz + col] = __float2bfloat16_rn(up);
+    }
+    act_switch(ep.act, [&](auto A) { z = act_value<true, decltype(A)::value>(z, ep.gamma) * up; });
+  } else {
+    if (zp) zp[t * ep.ldz + col] = __float2bfloat16_rn(z);
+    act_switch(ep.act, [&](auto A) { z = act_value<true, decltype(A)::value>(z, ep.gamma); });
+    if (ep.res) z += __bfloat162float(static_cast<const __nv_bfloat16*>(ep.res)[t * ep.ldr + col]);
+  }
+  out[t * ep.ldo + col] = __float2bfloat16_rn(z);
+}
+
+template <int EPI, bool VEC>
+cudaError_t launch_nt(const SmallGemm& g, unsigned blocks, cudaStream_t s) {
+  if (g.T <= 8)
+    return launch_kernel(dense_small_kernel<EPI, VEC, 1>, dim3(blocks), dim3(32 * WARPS), 0, s, g);
+  return launch_kernel(dense_small_kernel<EPI, VEC, 2>, dim3(blocks), dim3(32 * WARPS), 0, s, g);
+}
+
+}  // namespace
+
+cudaError_t launch_dense_small(int epi, const SmallGemm& g, cudaStream_t s) {
+  if (g.T < 1 || g.T > kSmallTokens || g.epi.out_f32) return cudaErrorInvalidValue;
+  const int rows = epi == kEpiGated ? 8 : 16;
+  const unsigned blocks = static_cast<unsigned>((g.N + rows - 1) / rows);
+  cudaError_t e;
+  if (epi == kEpiGated)
+    e = g.vec_in ? launch_nt<kEpiGated, true>(g, blocks, s) : launch_nt<kEpiGated, false>(g, blocks, s);
+  else
+    e = g.vec_in ? launch_nt<kEpiLinear, true>(g, blocks, s) : launch_nt<kEpiLinear, false>(g, blocks, s);
+  return e != cudaSuccess ? e : cudaGetLastError();
+}
+
+}  // namespace vmoe

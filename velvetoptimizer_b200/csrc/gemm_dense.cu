@@ -1,0 +1,477 @@
+// Dense bf16 products on CTA pairs (tcgen05.mma.cta_group::2) for the fused linear and the
+// gated feed-forward block, reading every operand in the layout the user holds it in.
+//
+//   forward           C[T, N] = x[T, K] w[N, K]^T       both operands K-major
+//   input gradient    C[T, K] = dz[T, N] w[N, K]        B stored [k, n]: read MN-major
+//   weight gradient   C[N, K] = dz[T, N]^T x[T, K]      both stored [k, mn]: read MN-major
+//
+// so no transposed or repacked copy of a weight or an activation is written.  A pair of CTAs
+// computes a 256 x 256 tile: each loads its own 128 rows of A and its own half of B per
+// 64-wide k block (32 KB a stage, 6 stages), the leader issues M256 N256 K16, each CTA's TMEM
+// holds its 128 rows, two accumulators deep, and eight epilogue warps per CTA drain one while
+// the other fills.  A K-major stage is one box of 64 k x 128 rows, an MN-major one two boxes
+// of 64 columns x 64 k rows (128-byte swizzle; descriptor leading offset 8 KB between the
+// 64-column chunks, stride offset 1 KB between 8-row groups).
+//
+// Extra forms of the k loop and of B:
+//   * two operand pairs (kb1 > 0): dx = dg Wg + du Wu runs as one product whose k blocks come
+//     from (dg, Wg) and then from (du, Wu), in one accumulator;
+//   * kEpiGated: the leader's half of B is 128 gate rows and the follower's 128 up rows of the
+//     same features, so a row's gate and up values meet in the epilogue;
+//   * groups: two A operands against one B (the gate's and the up's weight gradients);
+//   * splits: when the tiles are too few for the SMs the k blocks are divided, every split
+//     writes fp32 partials, and launch_dense_finish sums them in split order and runs the
+//     epilogue: no atomics, the same bits every run.
+// Rows, columns and k past the operands' extents are zero-filled by the TMA and never stored.
+// Every wait is bounded and reports a status code; no TMA multicast.
+#include <atomic>
+#include <type_traits>
+
+#include "common.cuh"
+#include "dense.h"
+#include "dense_act.cuh"
+
+namespace vmoe {
+namespace {
+
+constexpr int BK = 64;
+constexpr int PAIR_M = 256;
+constexpr int BN = 256;
+constexpr uint32_t CHUNK_BYTES = 64 * BK * 2;  // one MN-major box
+constexpr uint32_t HALF_BYTES = 128 * BK * 2;  // one operand's part of a stage in one CTA
+constexpr uint32_t STAGE_BYTES = 2 * HALF_BYTES;
+constexpr int STAGES = 6;
+constexpr uint32_t TMEM_COLS = 2 * BN;
+constexpr int EPI_WARPS = 8;
+constexpr int THREADS = 64 + 32 * EPI_WARPS;
+constexpr int kMaxDevices = 64;
+
+struct Shared {
+  uint64_t full[STAGES];
+  uint64_t empty[STAGES];
+  uint64_t tfull[2];
+  uint64_t tempty[2];  // the leader's are used: 16 arrivals (8 epilogue warps x 2 CTAs)
+  uint64_t done;
+  uint32_t tmem_base;
+  int abort;
+  alignas(16) float bias[EPI_WARPS][2][32];
+};
+
+constexpr size_t SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + sizeof(Shared) + 64;
+static_assert(SMEM_BYTES <= 232448, "shared memory budget");
+
+__device__ __forceinline__ bool aborted(const Shared* sh) {
+  return *reinterpret_cast<const volatile int*>(&sh->abort) != 0;
+}
+__device__ __forceinline__ void set_abort(Shared* sh, int* status, int code) {
+  *reinterpret_cast<volatile int*>(&sh->abort) = 1;
+  report(status, code);
+}
+
+__device__ __forceinline__ uint64_t desc_mn(uint32_t smem_addr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
+  d |= static_cast<uint64_t>(CHUNK_BYTES >> 4) << 16;
+  d |= static_cast<uint64_t>(1024 >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  d |= static_cast<uint64_t>(2) << 61;
+  return d;
+}
+
+// descriptor of the 16-wide k step `k` of a stage part at `addr`
+template <bool MN>
+__device__ __forceinline__ uint64_t op_desc(uint32_t addr, int k) {
+  if constexpr (MN) return desc_mn(addr + k * 2048);  // two 8-row groups further on
+  return umma_desc_sw128(addr + k * 32);
+}
+
+struct Item {
+  int g, m, n, kb, ke;
+};
+
+// Work item -> (group, tile, k-block range).  Tiles go in bands of `band` n tiles, all m tiles
+// of a band before the next, so the pairs running at one time share few A and B tiles.
+__device__ __forceinline__ Item item_of(const DenseGemm& a, int item) {
+  Item w;
+  const int split = item % a.splits;
+  int t = item / a.splits;
+  const int per_group = a.m_tiles * a.n_tiles;
+  w.g = t / per_group;
+  t -= w.g * per_group;
+  const int full = a.n_tiles / a.band;
+  const int band = t / (a.m_tiles * a.band);
+  if (band < full) {
+    const int r = t - band * a.m_tiles * a.band;
+    w.m = r / a.band;
+    w.n = band * a.band + r % a.band;
+  } else {
+    const int width = a.n_tiles - full * a.band;
+    const int r = t - full * a.m_tiles * a.band;
+    w.m = r / width;
+    w.n = full * a.band + r % width;
+  }
+  w.kb = split * a.kb_per_split;
+  w.ke = min(w.kb + a.kb_per_split, a.kb0 + a.kb1);
+  return w;
+}
+
+// 32 bias values of the columns [col, col + 32) into this warp's shared row (0 past N)
+__device__ __forceinline__ void stage_bias(float* dst, const void* bias, int64_t col, int64_t N,
+                                           int lane) {
+  const auto* b = static_cast<const __nv_bfloat16*>(bias);
+  dst[lane] = (b && col + lane < N) ? __bfloat162float(b[col + lane]) : 0.f;
+}
+
+__device__ __forceinline__ void add_bias(float (&v)[32], const float* b) {
+#pragma unroll
+  for (int j = 0; j < 32; j += 4) {
+    const float4 q = *reinterpret_cast<const float4*>(b + j);
+    v[j] += q.x;
+    v[j + 1] += q.y;
+    v[j + 2] += q.z;
+    v[j + 3] += q.w;
+  }
+}
+
+template <bool A_MN, bool B_MN, int EPI, bool SPLIT>
+__global__ void __launch_bounds__(THREADS, 1)
+gemm_dense_kernel(const __grid_constant__ DenseMaps maps, const __grid_constant__ DenseGemm args) {
+  constexpr uint32_t IDESC = umma_idesc_bf16(PAIR_M, BN) | (A_MN ? 1u << 15 : 0u) |
+                             (B_MN ? 1u << 16 : 0u);
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* gbase = smem_raw + (base - raw);
+  const uint32_t a_s = base;
+  const uint32_t b_s = base + STAGES * HALF_BYTES;
+  Shared* sh = reinterpret_cast<Shared*>(gbase + STAGES * STAGE_BYTES);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(smem_u32(&sh->full[s]), 1);
+      mbar_init(smem_u32(&sh->empty[s]), 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(smem_u32(&sh->tfull[a]), 1);
+      mbar_init(smem_u32(&sh->tempty[a]), 2 * EPI_WARPS);
+    }
+    mbar_init(smem_u32(&sh->done), 1);
+    sh->abort = 0;
+    fence_mbar_init();
+    prefetch_tmap(&maps.a0);
+    prefetch_tmap(&maps.b0);
+  }
+  cluster_sync_all();  // both CTAs' barriers exist before any cross-CTA arrive or copy
+  if (warp == 1) tmem_alloc_pair(smem_u32(&sh->tmem_base), TMEM_COLS);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh->tmem_base;
+  const int total = args.groups * args.m_tiles * args.n_tiles * args.splits;
+  const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
+
+  if (warp == 0) {
+    // ---------------- TMA producer (both CTAs) ----------------
+    if (lane == 0) {
+      int it = 0;
+      for (int item = pair; item < total; item += num_pairs) {
+        const Item w = item_of(args, item);
+        const int a_at = w.m * PAIR_M + static_cast<int>(rank) * 128;
+        // gated: this CTA's 128 rows are gate (leader) or up (follower) rows of one weight each
+        const int b_at = EPI == kEpiGated ? w.n * 128 : w.n * BN + static_cast<int>(rank) * 128;
+        bool ok = true;
+        for (int kb = w.kb; kb < w.ke; ++kb, ++it) {
+          const int s = it % STAGES;
+          const uint32_t ph = (it / STAGES) & 1;
+          if (!mbar_wait(smem_u32(&sh->empty[s]), ph ^ 1)) {
+            set_abort(sh, args.status, kStatusTimeoutProducer);
+            ok = false;
+            break;
+          }
+          if (aborted(sh)) { ok = false; break; }
+          const bool second = kb >= args.kb0;
+          const int k0 = (second ? kb - args.kb0 : kb) * BK;
+          const CUtensorMap* am = (second || w.g) ? &maps.a1 : &maps.a0;
+          const CUtensorMap* bm =
+              (second || (EPI == kEpiGated && !leader)) ? &maps.b1 : &maps.b0;
+          const uint32_t fb = smem_u32(&sh->full[s]);
+          if (leader) mbar_arrive_expect_tx(fb, 2 * STAGE_BYTES);
+          const uint32_t fb_leader = mapa_shared(fb, 0);
+          const uint32_t a_dst = a_s + s * HALF_BYTES, b_dst = b_s + s * HALF_BYTES;
+          if constexpr (A_MN) {
+            tma_load_2d_pair(a_dst, am, fb_leader, a_at, k0);
+            tma_load_2d_pair(a_dst + CHUNK_BYTES, am, fb_leader, a_at + 64, k0);
+          } else {
+            tma_load_2d_pair(a_dst, am, fb_leader, k0, a_at);
+          }
+          if constexpr (B_MN) {
+            tma_load_2d_pair(b_dst, bm, fb_leader, b_at, k0);
+            tma_load_2d_pair(b_dst + CHUNK_BYTES, bm, fb_leader, b_at + 64, k0);
+          } else {
+            tma_load_2d_pair(b_dst, bm, fb_leader, k0, b_at);
+          }
+        }
+        if (!ok) break;
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------- MMA issuer (leader only) ----------------
+    if (leader && lane == 0) {
+      int it = 0, local = 0;
+      for (int item = pair; item < total; item += num_pairs, ++local) {
+        const Item w = item_of(args, item);
+        const int acc = local & 1;
+        const uint32_t aph = (local >> 1) & 1;
+        if (!mbar_wait_cluster(smem_u32(&sh->tempty[acc]), aph ^ 1)) {
+          set_abort(sh, args.status, kStatusTimeoutMma);
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d_tmem = tmem + acc * BN;
+        bool ok = true;
+        for (int kb = w.kb; kb < w.ke; ++kb, ++it) {
+          const int s = it % STAGES;
+          const uint32_t ph = (it / STAGES) & 1;
+          if (!mbar_wait(smem_u32(&sh->full[s]), ph)) {
+            set_abort(sh, args.status, kStatusTimeoutMma);
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t a_addr = a_s + s * HALF_BYTES, b_addr = b_s + s * HALF_BYTES;
+#pragma unroll
+          for (int k = 0; k < BK / 16; ++k)
+            umma_bf16_pair(d_tmem, op_desc<A_MN>(a_addr, k), op_desc<B_MN>(b_addr, k), IDESC,
+                           (kb > w.kb || k > 0) ? 1u : 0u);
+          umma_commit_pair(smem_u32(&sh->empty[s]), 0x3);  // frees the stage in both CTAs
+        }
+        if (!ok) break;
+        umma_commit_pair(smem_u32(&sh->tfull[acc]), 0x3);
+        if (aborted(sh)) break;
+      }
+      umma_commit_pair(smem_u32(&sh->done), 0x1);
+      if (!mbar_wait(smem_u32(&sh->done), 0)) report(args.status, kStatusTimeoutDrain);
+    }
+  } else {
+    // ---------------- epilogue (warps 2..9, both CTAs) ----------------
+    const int q = warp & 3;            // TMEM lane quarter this warp may access
+    const int part = (warp - 2) >> 2;  // which half of the columns
+    float(*bias_s)[32] = sh->bias[warp - 2];
+    const DenseEpi& ep = args.epi;
+    int local = 0;
+    for (int item = pair; item < total; item += num_pairs, ++local) {
+      const Item w = item_of(args, item);
+      const int acc = local & 1;
+      const uint32_t aph = (local >> 1) & 1;
+      const bool got = mbar_wait(smem_u32(&sh->tfull[acc]), aph);
+      __syncwarp();
+      if (!__all_sync(0xffffffffu, got)) {
+        if (lane == 0) set_abort(sh, args.status, kStatusTimeoutEpilogue);
+        break;
+      }
+      tc_fence_after();
+      const int64_t row = static_cast<int64_t>(w.m) * PAIR_M + rank * 128 + q * 32 + lane;
+      const bool in = row < args.M;
+      const uint32_t t_row = tmem + (static_cast<uint32_t>(q * 32) << 16) + acc * BN;
+      if constexpr (SPLIT) {
+        // fp32 partials in the accumulator's own column order (gated: gate | up per tile)
+        const int split = item % args.splits;
+        float* dst = args.partial +
+                     ((static_cast<int64_t>(split) * args.groups + w.g) * args.M + row) * args.ldp +
+                     static_cast<int64_t>(w.n) * BN;
+#pragma unroll 1
+        for (int c = part * 128; c < (part + 1) * 128; c += 32) {
+          float v[32];
+          __syncwarp();  // the rows that stored before meet the others again
+          tmem_ld32(t_row + c, v);
+          if (in) store_row<32, float>(dst + c, v, 32, true);
+        }
+      } else if constexpr (EPI == kEpiGated) {
+#pragma unroll 1
+        for (int c = part * 64; c < (part + 1) * 64; c += 32) {
+          const int64_t col = static_cast<int64_t>(w.n) * 128 + c;
+          const int64_t valid = args.N - col;
+          float g[32], u[32];
+          __syncwarp();
+          tmem_ld32(t_row + c, g);
+          tmem_ld32(t_row + 128 + c, u);
+          if (valid <= 0) continue;  // the same for the whole warp
+          __syncwarp();
+          stage_bias(bias_s[0], ep.bias, col, args.N, lane);
+          stage_bias(bias_s[1], ep.bias2, col, args.N, lane);
+          __syncwarp();
+          add_bias(g, bias_s[0]);
+          add_bias(u, bias_s[1]);
+          if (!in) continue;
+          if (ep.z) {
+            auto* zp = static_cast<__nv_bfloat16*>(ep.z) + row * ep.ldz + col;
+            auto* zp2 = static_cast<__nv_bfloat16*>(ep.z2) + row * ep.ldz + col;
+            store_row<32>(zp, g, valid, ep.vec & kVecZ);
+            store_row<32>(zp2, u, valid, ep.vec & kVecZ);
+          }
+          act_switch(ep.act, [&](auto A) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) g[j] = act_value<true, decltype(A)::value>(g[j], ep.gamma) * u[j];
+          });
+          store_row<32>(static_cast<__nv_bfloat16*>(ep.out) + row * ep.ldo + col, g, valid,
+                        ep.vec & kVecOut);
+        }
+      } else if constexpr (EPI == kEpiGluBwd) {
+#pragma unroll 1
+        for (int c = part * 128; c < (part + 1) * 128; c += 32) {
+          const int64_t col = static_cast<int64_t>(w.n) * BN + c;
+          const int64_t valid = args.N - col;
+          float dh[32];
+          __syncwarp();
+          tmem_ld32(t_row + c, dh);
+          if (valid <= 0 || !in) continue;
+          float g[32], u[32];
+          load_row<32>(static_cast<const __nv_bfloat16*>(ep.z) + row * ep.ldz + col, g, valid,
+                       ep.vec & kVecZ);
+          load_row<32>(static_cast<const __nv_bfloat16*>(ep.z2) + row * ep.ldz + col, u, valid,
+                       ep.vec & kVecZ);
+          act_switch(ep.act, [&](auto A) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              float a, d;
+              act_grad<true, decltype(A)::value>(g[j], ep.gamma, a, d);
+              g[j] = dh[j] * u[j] * d;
+              u[j] = dh[j] * a;
+            }
+          });
+          store_row<32>(static_cast<__nv_bfloat16*>(ep.out) + row * ep.ldo + col, g, valid,
+                        ep.vec & kVecOut);
+          store_row<32>(static_cast<__nv_bfloat16*>(ep.out2) + row * ep.ldo + col, u, valid,
+                        ep.vec & kVecOut);
+        }
+      } else {
+        void* out = w.g ? ep.out2 : ep.out;
+#pragma unroll 1
+        for (int c = part * 128; c < (part + 1) * 128; c += 32) {
+          const int64_t col = static_cast<int64_t>(w.n) * BN + c;
+          const int64_t valid = args.N - col;
+          float v[32];
+          __syncwarp();
+          tmem_ld32(t_row + c, v);
+          if (valid <= 0) continue;
+          if (ep.bias) {
+            __syncwarp();
+            stage_bias(bias_s[0], ep.bias, col, args.N, lane);
+            __syncwarp();
+            add_bias(v, bias_s[0]);
+          }
+          if (!in) continue;
+          if (ep.z)
+            store_row<32>(static_cast<__nv_bfloat16*>(ep.z) + row * ep.ldz + col, v, valid,
+                          ep.vec & kVecZ);
+          if (ep.act != kActNone) {
+            act_switch(ep.act, [&](auto A) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = act_value<true, decltype(A)::value>(v[j], ep.gamma);
+            });
+          }
+          if (ep.res) {
+            float r[32];
+            load_row<32>(static_cast<const __nv_bfloat16*>(ep.res) + row * ep.ldr + col, r, valid,
+                         ep.vec & kVecRes);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] += r[j];
+          }
+          if (ep.out_f32)
+            store_row<32>(static_cast<float*>(out) + row * ep.ldo + col, v, valid, ep.vec & kVecOut);
+          else
+            store_row<32>(static_cast<__nv_bfloat16*>(out) + row * ep.ldo + col, v, valid,
+                          ep.vec & kVecOut);
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&sh->tempty[acc]), 0));
+    }
+  }
+
+  __syncthreads();
+  if (threadIdx.x == 0 && aborted(sh)) {
+    // copies issued by this CTA land on the leader's barriers; give any still in flight a
+    // bounded time to finish before the shared memory is released
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 200000ull) {
+    }
+  }
+  cluster_sync_all();  // the leader's MMAs (which read both CTAs' smem) are complete
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, TMEM_COLS);
+  }
+}
+
+template <bool A_MN, bool B_MN, int EPI, bool SPLIT>
+cudaError_t launch(const DenseMaps& maps, const DenseGemm& g, int num_sms, cudaStream_t s) {
+  auto kern = gemm_dense_kernel<A_MN, B_MN, EPI, SPLIT>;
+  cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         static_cast<int>(SMEM_BYTES));
+  if (err != cudaSuccess) return err;
+  const int64_t work = static_cast<int64_t>(g.groups) * g.m_tiles * g.n_tiles * g.splits;
+  if (work < 1 || work > 0x7fffffff || g.band < 1 || g.kb_per_split < 1)
+    return cudaErrorInvalidValue;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.blockDim = dim3(THREADS, 1, 1);
+  cfg.dynamicSmemBytes = SMEM_BYTES;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  // persistent, as many pairs as can be resident at once (a pair needs two free SMs of one
+  // GPC), so that no pair's share of the items starts after another's has ended
+  static std::atomic<int> resident[kMaxDevices];
+  int dev = 0;
+  if ((err = cudaGetDevice(&dev)) != cudaSuccess) return err;
+  int max_pairs = dev < kMaxDevices ? resident[dev].load(std::memory_order_relaxed) : 0;
+  if (max_pairs == 0) {
+    cfg.gridDim = dim3(static_cast<unsigned>(num_sms & ~1), 1, 1);
+    err = cudaOccupancyMaxActiveClusters(&max_pairs, reinterpret_cast<const void*>(kern), &cfg);
+    if (err != cudaSuccess) return err;
+    if (max_pairs < 1) return cudaErrorInvalidConfiguration;
+    if (dev < kMaxDevices) resident[dev].store(max_pairs, std::memory_order_relaxed);
+  }
+  int64_t pairs = num_sms / 2;
+  if (pairs > max_pairs) pairs = max_pairs;
+  if (pairs > work) pairs = work;
+  cfg.gridDim = dim3(static_cast<unsigned>(2 * pairs), 1, 1);
+  err = cudaLaunchKernelEx(&cfg, kern, maps, g);
+  return err != cudaSuccess ? err : cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_gemm_dense(bool a_mn, bool b_mn, int epi, const DenseMaps& maps,
+                              const DenseGemm& g, int num_sms, cudaStream_t s) {
+  if (g.splits > 1) {
+    if (!g.partial || g.ldp % 4) return cudaErrorInvalidValue;
+    if (!a_mn && !b_mn)
+      return epi == kEpiGated ? launch<false, false, kEpiGated, true>(maps, g, num_sms, s)
+                              : launch<false, false, kEpiLinear, true>(maps, g, num_sms, s);
+    if (!a_mn) return launch<false, true, kEpiLinear, true>(maps, g, num_sms, s);
+    return launch<true, true, kEpiLinear, true>(maps, g, num_sms, s);
+  }
+  if (!a_mn && !b_mn)
+    return epi == kEpiGated ? launch<false, false, kEpiGated, false>(maps, g, num_sms, s)
+                            : launch<false, false, kEpiLinear, false>(maps, g, num_sms, s);
+  if (!a_mn && b_mn)
+    return epi == kEpiGluBwd ? launch<false, true, kEpiGluBwd, false>(maps, g, num_sms, s)
+                             : launch<false, true, kEpiLinear, false>(maps, g, num_sms, s);
+  if (a_mn && b_mn && epi == kEpiLinear)
+    return launch<true, true, kEpiLinear, false>(maps, g, num_sms, s);
+  return cudaErrorInvalidValue;
+}
+
+}  // namespace vmoe
