@@ -429,6 +429,21 @@ VMOE_API int vmoe_gated_ffn_backward(vmoe_ops* ops, const vmoe_gated_ffn* d, con
                                      size_t saved_bytes, void* workspace, size_t workspace_bytes,
                                      void* stream);
 
+/* Global gradient norm and clipping, as the reference's training loop applies it to every
+ * gradient before the optimizer (python/train.py:465-480):
+ *   norm = (sum over all tensors |g|^p)^(1/p);  g *= min(1, max_norm / (norm + 1e-6))
+ * over n dense tensors given by device pointer, element count and dtype (host arrays, read
+ * before the call returns; any alignment to the element; empty tensors are skipped; no two may
+ * overlap).  total_norm: device fp32 scalar, optional.  max_norm < 0 leaves the tensors as they
+ * are; where the factor is 1 nothing is written.  A norm that is NaN makes every element NaN,
+ * an infinite one scales by 0.  Sums are held in fp64 in a fixed order. */
+enum { VMOE_NORM_INF = 0, VMOE_NORM_1 = 1, VMOE_NORM_2 = 2 };
+VMOE_API int vmoe_grad_norm_workspace_size(vmoe_ops* ops, int n, size_t* bytes);
+VMOE_API int vmoe_grad_norm(vmoe_ops* ops, void* const* tensors, const int64_t* counts,
+                            const int32_t* dtypes, int n, int norm_type, float max_norm,
+                            float* total_norm, void* workspace, size_t workspace_bytes,
+                            void* stream);
+
 /* Read (and clear) the device status word the kernels write when a bounded wait gives
  * up or an index check fails.  Synchronises `stream`.  *code = 0 when all is well. */
 VMOE_API int vmoe_device_status(vmoe_handle* h, int32_t* code, void* stream);

@@ -45,6 +45,7 @@ EXPORTED = (
     "vmoe_ops_create", "vmoe_ops_destroy", "vmoe_ops_last_error", "vmoe_ops_device_status",
     "vmoe_linear_workspace_size", "vmoe_linear_forward", "vmoe_linear_backward",
     "vmoe_gated_ffn_workspace_size", "vmoe_gated_ffn_forward", "vmoe_gated_ffn_backward",
+    "vmoe_grad_norm_workspace_size", "vmoe_grad_norm",
 )
 
 
@@ -242,6 +243,11 @@ def load() -> ctypes.CDLL:
                                             POINTER(VmoeFfnGrads), c_void_p, c_size_t, c_void_p,
                                             c_size_t, c_void_p]
     lib.vmoe_gated_ffn_backward.restype = c_int
+    lib.vmoe_grad_norm_workspace_size.argtypes = [H, c_int, POINTER(c_size_t)]
+    lib.vmoe_grad_norm_workspace_size.restype = c_int
+    lib.vmoe_grad_norm.argtypes = [H, c_void_p, c_void_p, c_void_p, c_int, c_int, c_float, c_void_p,
+                                   c_void_p, c_size_t, c_void_p]
+    lib.vmoe_grad_norm.restype = c_int
     lib.vmoe_abi_version.argtypes = []
     lib.vmoe_abi_version.restype = c_int
     _lib = lib
