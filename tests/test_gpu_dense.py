@@ -1,4 +1,6 @@
 """GPU: linear and gated_ffn against 64-bit forms of the same formulas, forward and backward."""
+import math
+
 import pytest
 import torch
 
@@ -455,7 +457,263 @@ def test_refusals():
         vb.gated_ffn(x, w, w[:8], w.t())
 
 
-def test_device_status_clean():
-    from velvetoptimizer_b200.dense import ops_for
+def test_gradients_have_no_gradient():
+    import velvetoptimizer_b200 as vb
+    for act in ("none", "silu"):
+        x = torch.randn(20, 16, device="cuda", requires_grad=True)
+        w = torch.randn(24, 16, device="cuda", requires_grad=True)
+        y = vb.linear(x, w, activation=act)
+        g, = torch.autograd.grad(y.square().sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="cannot be differentiated"):
+            g.square().sum().backward()
+
+
+def test_changed_input_is_noticed():
+    import velvetoptimizer_b200 as vb
+    x = torch.randn(20, 16, device="cuda", dtype=BF16).requires_grad_()
+    w = torch.randn(24, 16, device="cuda", dtype=BF16).requires_grad_()
+    y = vb.linear(x, w, activation="silu")
+    with torch.no_grad():
+        w.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+def test_first_call_of_a_thread_inside_a_capture():
+    """A new thread's first call makes its context: nothing in that may disturb a capture."""
+    import threading
+
+    import velvetoptimizer_b200 as vb
+    x = torch.randn(40, 64, device="cuda").to(BF16)
+    w = torch.randn(48, 64, device="cuda").to(BF16)
+    want = vb.linear(x, w)
     torch.cuda.synchronize()
-    assert ops_for(torch.device("cuda")).device_status(torch.cuda.current_stream().cuda_stream) == 0
+    got, failed = [], []
+
+    def work():
+        try:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                y = vb.linear(x, w)
+            graph.replay()
+            torch.cuda.synchronize()
+            got.append(y.clone())
+        except Exception as e:
+            failed.append(e)
+
+    t = threading.Thread(target=work)
+    t.start()
+    t.join()
+    assert not failed and torch.equal(got[0], want)
+
+
+def test_traced():
+    """Under a tracer the registered ops run, with the eager path's results and gradients."""
+    import velvetoptimizer_b200 as vb
+    gen = torch.Generator().manual_seed(0)
+    p = [rand(gen, 40, 64), rand(gen, 72, 64, std=0.1), rand(gen, 72, 64, std=0.1),
+         rand(gen, 64, 72, std=0.1), rand(gen, 72)]
+    p = [t.cuda().requires_grad_() for t in p]
+    dy = rand(gen, 40, 72).cuda()
+
+    def fn(x, wg, wu, wd, b):
+        return vb.linear(vb.gated_ffn(x, wg, wu, wd, b, residual=x), wg, b, activation="silu")
+
+    traced = torch.compile(fn, backend="aot_eager", fullgraph=True)
+    y, t = fn(*p), traced(*p)
+    assert torch.equal(y, t)
+    for a, b in zip(torch.autograd.grad(y, p, dy), torch.autograd.grad(t, p, dy)):
+        assert torch.equal(a, b)
+
+
+def test_errors_of_the_library_surface():
+    """A status of the C ABI arrives as VmoeError with its text."""
+    from velvetoptimizer_b200 import _lib
+    from velvetoptimizer_b200.dense import ops_for
+    o = ops_for(torch.device("cuda"))
+    d = _lib.VmoeLinear(4, 8, 8, 8, 8, 8, _lib.VMOE_BF16, 9, 0.1, _lib.VMOE_BF16)
+    import ctypes
+    with pytest.raises(_lib.VmoeError, match="unknown activation"):
+        o.check(o.lib.vmoe_linear_workspace_size(o.ptr, d, 0, ctypes.c_size_t()), "size")
+
+
+@pytest.mark.parametrize("change,code", [
+    (dict(tokens=-1), 1), (dict(in_features=0), 1), (dict(out_features=0), 1), (dict(ldx=7), 1),
+    (dict(ldw=7), 1), (dict(dtype=2), 1), (dict(activation=5), 1), (dict(grad_dtype=3), 1),
+    (dict(gamma=float("nan"), activation=4), 1), (dict(tokens=1 << 31), 1)])
+def test_abi_refusals(change, code):
+    import ctypes
+
+    from velvetoptimizer_b200 import _lib
+    from velvetoptimizer_b200.dense import ops_for
+    o = ops_for(torch.device("cuda"))
+    base = dict(tokens=4, in_features=8, out_features=8, ldx=8, ldw=8, ldr=8, dtype=_lib.VMOE_BF16,
+                activation=0, gamma=0.1, grad_dtype=_lib.VMOE_BF16)
+    d = _lib.VmoeLinear(**{**base, **change})
+    n = ctypes.c_size_t()
+    assert o.lib.vmoe_linear_workspace_size(o.ptr, d, 0, n) == code
+    x = torch.zeros(64, device="cuda", dtype=BF16)
+    p = x.data_ptr()
+    assert o.lib.vmoe_linear_forward(o.ptr, d, p, p, None, None, p, None, None, 0, None) == code
+
+
+def test_abi_pointer_refusals():
+    import ctypes
+
+    from velvetoptimizer_b200 import _lib
+    from velvetoptimizer_b200.dense import ops_for
+    o = ops_for(torch.device("cuda"))
+    bf = _lib.VMOE_BF16
+    d = _lib.VmoeLinear(40, 64, 64, 64, 64, 64, bf, 0, 0.1, bf)
+    buf = torch.zeros(1 << 20, device="cuda", dtype=torch.uint8)
+    p = buf.data_ptr()
+    ws = p + (1 << 19)
+    n = ctypes.c_size_t()
+    f, b = o.lib.vmoe_linear_forward, o.lib.vmoe_linear_backward
+    assert f(o.ptr, d, None, p, None, None, p, None, ws, 1 << 19, None) == 1   # no x
+    assert f(o.ptr, d, p, None, None, None, p, None, ws, 1 << 19, None) == 1   # no weight
+    assert f(o.ptr, d, p, p, None, None, None, None, ws, 1 << 19, None) == 1   # no y
+    assert f(o.ptr, d, p + 2, p, None, None, p, None, ws, 1 << 19, None) == 1  # unaligned x
+    assert f(o.ptr, d, p + 1, p, None, None, p, None, ws, 1 << 19, None) == 1
+    assert o.lib.vmoe_linear_workspace_size(o.ptr, d, 1, n) == 0 and n.value > 0
+    args = (p, p, None, p, 64, p, p, p)
+    assert b(o.ptr, d, *args, None, 0, None) == _lib.VMOE_ERR_WORKSPACE
+    assert b(o.ptr, d, *args, ws, n.value - 1, None) == _lib.VMOE_ERR_WORKSPACE
+    assert b(o.ptr, d, *args, ws + 16, n.value, None) == _lib.VMOE_ERR_WORKSPACE
+    assert b(o.ptr, d, p, p, None, p, 65, p, p, p, ws, n.value, None) == 1     # a pitch it cannot read
+    act = _lib.VmoeLinear(40, 64, 64, 64, 64, 64, bf, 2, 0.1, bf)
+    assert o.lib.vmoe_linear_workspace_size(o.ptr, act, 1, n) == 0
+    assert b(o.ptr, act, *args, ws, n.value, None) == 1                        # no z
+    ffn = _lib.VmoeGatedFfn(40, 64, 64, 64, 64, bf, 4, 0.1, bf)
+    w = _lib.VmoeFfnWeights(p, p, p)
+    s = ctypes.c_size_t()
+    assert o.lib.vmoe_gated_ffn_workspace_size(o.ptr, ffn, 0, n, s) == 0 and s.value > 0
+    g = o.lib.vmoe_gated_ffn_forward
+    assert g(o.ptr, ffn, p, w, None, p, None, 0, ws, n.value - 1, None) == _lib.VMOE_ERR_WORKSPACE
+    assert g(o.ptr, ffn, p, w, None, p, p, s.value - 1, ws, n.value, None) == _lib.VMOE_ERR_WORKSPACE
+    assert g(o.ptr, ffn, p, _lib.VmoeFfnWeights(p, None, p), None, p, None, 0, ws, n.value, None) == 1
+    torch.cuda.synchronize()
+    assert not buf.any()  # nothing ran
+
+
+def module_inputs(dtype, wdtype, T=50, H=72, I=104):
+    from velvetoptimizer_b200 import FeedForward, MoEConfig
+    torch.manual_seed(0)
+    m = FeedForward(MoEConfig(hidden_size=H, intermediate_size=I, flylora_rank=4, flylora_alpha=8.0))
+    with torch.no_grad():
+        for p in m.parameters():
+            p.copy_(torch.randn_like(p) * (0.2 if p.dim() == 1 else p.shape[1] ** -0.5))
+    m = m.cuda().to(wdtype)
+    x = torch.randn(2, T // 2, H).to(dtype).cuda()
+    return m, x, torch.randn(2, T // 2, H).to(dtype).cuda()
+
+
+@pytest.mark.parametrize("dtype,wdtype", [(BF16, F32), (BF16, BF16), (F32, F32)])
+def test_feed_forward_trains(dtype, wdtype):
+    """FeedForward's gradients, the FlyLoRA factors' among them, against 64-bit autograd of the
+    unfolded branch.  Norm-wise: the rounding of the folded weight, of g and u, of dg and du (or
+    h), and of the gradient: five."""
+    m, x, dy = module_inputs(dtype, wdtype)
+    r = torch.randn_like(x)
+    lx = x.clone().requires_grad_()
+    y = m(lx, residual=r)
+    grads = torch.autograd.grad(y, [lx, *m.parameters()], dy)
+
+    def fly(p, v):
+        q = dict(p)
+        base = v @ q["base.weight"].t() + q["base.bias"]
+        low = v @ q["lora_down.weight"].t() + q["lora_down.bias"]
+        return base + 2.0 * (low @ q["lora_up.weight"].t() + q["lora_up.bias"])
+
+    import copy
+    ref64 = copy.deepcopy(m).double().cpu()
+    v = x.double().cpu().requires_grad_()
+    g = fly(ref64.gate_proj.named_parameters(), v)
+    u = fly(ref64.up_proj.named_parameters(), v)
+    out = r.double().cpu() + ref64.down_proj(ref.act(g, "era", GAMMA) * u)
+    want = torch.autograd.grad(out, [v, *ref64.parameters()], dy.double().cpu())
+    limit = 5 * 2.0 ** -8 if BF16 in (dtype, wdtype) else 1e-5
+    names = ["x"] + [n for n, _ in m.named_parameters()]
+    for n, a, b in zip(["y"] + names, [y, *grads], [out, *want]):
+        assert a.dtype == (dtype if n in ("x", "y") else wdtype)
+        rel = float((a.double().cpu() - b).norm() / b.norm())
+        assert rel <= limit, (n, rel)
+
+
+def test_feed_forward_without_gradients_is_unchanged():
+    """Under no_grad the packed path runs, and agrees with the training path."""
+    m, x, _ = module_inputs(BF16, F32)
+    with torch.no_grad():
+        a = m(x)
+    assert len(m._packed) == 1
+    b = m(x)
+    assert b.requires_grad and not a.requires_grad
+    # two roundings each (h and out), and the packed path's tanh.approx (2^-11)
+    assert float((a.float() - b.float()).norm() / a.float().norm()) <= 4 * 2.0 ** -8
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_flylora_linear_alone(dtype):
+    from velvetoptimizer_b200 import FlyLoRALinear
+    torch.manual_seed(0)
+    m = FlyLoRALinear(40, 56, rank=4, alpha=8.0).cuda()
+    with torch.no_grad():
+        m.lora_up.weight.normal_(std=0.1)
+    x = torch.randn(3, 7, 40, device="cuda").to(dtype)
+    r = torch.randn(3, 7, 56, device="cuda").to(dtype)
+    y = m(x, residual=r, activation="silu")
+    d = lambda t: t.detach().double()  # noqa: E731
+    z = d(x) @ d(m.base.weight).t() + d(m.base.bias) + 2.0 * (
+        (d(x) @ d(m.lora_down.weight).t() + d(m.lora_down.bias)) @ d(m.lora_up.weight).t()
+        + d(m.lora_up.bias))
+    want = d(r) + z * torch.sigmoid(z)
+    # the folded weight and the result rounded
+    limit = 2 * 2.0 ** -8 if dtype == BF16 else 1e-6
+    assert float((d(y) - want).norm() / want.norm()) <= limit
+    y.sum().backward()
+    assert all(p.grad is not None and torch.isfinite(p.grad).all() for p in m.parameters())
+
+
+def test_training_steps_together():
+    """The operators as a step uses them: block, projection, backward, clipping, update; the
+    clipped gradients against the same step in 64 bits."""
+    import copy
+
+    import velvetoptimizer_b200 as vb
+    m, x, dy = module_inputs(BF16, F32)
+    head = vb.FlyLoRALinear(72, 40, rank=4, alpha=8.0).cuda()
+    with torch.no_grad():
+        head.lora_up.weight.normal_(std=0.1)
+    ps = [*m.parameters(), *head.parameters()]
+    opt = torch.optim.SGD(ps, lr=0.1)
+    for step in range(2):
+        ref_m, ref_h = copy.deepcopy(m).double().cpu(), copy.deepcopy(head).double().cpu()
+        opt.zero_grad()
+        y = head(m(x, residual=x), activation="gelu_tanh")
+        y.float().square().mean().backward()
+        norm = vb.clip_grad_norm_(ps, 0.05)
+
+        def eff(q):
+            return (q.base.weight + 2.0 * q.lora_up.weight @ q.lora_down.weight,
+                    q.base.bias + 2.0 * (q.lora_up.weight @ q.lora_down.bias + q.lora_up.bias))
+
+        v = x.double().cpu()
+        (gw, gb), (uw, ub), (hw, hb) = eff(ref_m.gate_proj), eff(ref_m.up_proj), eff(ref_h)
+        h = ref.act(v @ gw.t() + gb, "era", GAMMA) * (v @ uw.t() + ub)
+        out = ref.act((v + ref_m.down_proj(h)) @ hw.t() + hb, "gelu_tanh", GAMMA)
+        rp = [*ref_m.parameters(), *ref_h.parameters()]
+        want = torch.autograd.grad(out.square().mean(), rp)
+        n64 = math.sqrt(sum(float(g.square().sum()) for g in want))
+        # ten roundings lie between the inputs and a gradient: weights, g, u, h, y (twice: the
+        # loss's gradient squares it), z, dz, dg, and the block's output
+        assert abs(float(norm) - n64) <= 10 * 2.0 ** -8 * n64
+        for p, g in zip(ps, want):
+            g = g * min(1.0, 0.05 / (n64 + 1e-6))
+            assert float((p.grad.double().cpu() - g).norm()) <= 11 * 2.0 ** -8 * float(g.norm()) + 1e-9
+        opt.step()
+
+
+def test_device_status_clean():
+    from velvetoptimizer_b200.dense import _native
+    torch.cuda.synchronize()
+    assert _native().device_status(torch.zeros(1, device="cuda")) == 0

@@ -65,58 +65,71 @@ def _compile(src: str, verbose: bool, extra: list[str]) -> str:
     return obj
 
 
-PARAM_KEY_SRC = os.path.join(PKG, "csrc_py", "param_key.cpp")
-PARAM_KEY_LIB = os.path.join(LIB_DIR, "_param_key.so")
+CSRC_PY = os.path.join(PKG, "csrc_py")
 
 
-def build_param_key(force: bool = False, verbose: bool = False) -> str:
-    """The modules' host helper (csrc_py/param_key.cpp, a CPython extension against torch's
-    headers): g++ only, no GPU code.  Skips work when up to date."""
-    if (not force and os.path.exists(PARAM_KEY_LIB)
-            and os.path.getmtime(PARAM_KEY_SRC) <= os.path.getmtime(PARAM_KEY_LIB)):
-        return PARAM_KEY_LIB
+def build_host_module(name: str, force: bool = False, verbose: bool = False) -> str:
+    """A host helper of the PyTorch layer (csrc_py/<name>.cpp, a CPython extension against
+    torch's headers): g++ only, no GPU code.  Skips work when up to date."""
+    src = os.path.join(CSRC_PY, f"{name}.cpp")
+    out = os.path.join(LIB_DIR, f"_{name}.so")
+    deps = [src] + ([os.path.join(INCLUDE, "vesper_moe.h")] if name == "dense_ops" else [])
+    if (not force and os.path.exists(out)
+            and all(os.path.getmtime(d) <= os.path.getmtime(out) for d in deps)):
+        return out
     import sysconfig
 
     import torch
     tdir = os.path.dirname(torch.__file__)
     abi = int(getattr(torch._C, "_GLIBCXX_USE_CXX11_ABI", True))
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
-           f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-I", sysconfig.get_paths()["include"],
+    cuda = os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include")
+    # the host compiler nvcc takes, before $CXX: a toolchain that links libstdc++ statically
+    # would give the module streams and locales of its own, apart from torch's
+    cmd = [shutil.which("g++") or os.environ["CXX"], "-O2", "-std=c++17", "-fPIC", "-shared",
+           "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
+           "-I", sysconfig.get_paths()["include"], "-I", INCLUDE, "-I", cuda,
            "-I", os.path.join(tdir, "include"),
            "-I", os.path.join(tdir, "include", "torch", "csrc", "api", "include"),
-           PARAM_KEY_SRC, "-o", PARAM_KEY_LIB + ".tmp", "-L", os.path.join(tdir, "lib"),
-           "-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_python",
-           f"-Wl,-rpath,{os.path.join(tdir, 'lib')}"]
+           src, "-o", out + ".tmp", "-L", os.path.join(tdir, "lib"),
+           "-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_python"]
+    if name == "dense_ops":  # calls the C ABI library beside it
+        cmd += ["-lc10_cuda", LIB, "-Wl,-rpath,$ORIGIN"]
+    cmd += [f"-Wl,-rpath,{os.path.join(tdir, 'lib')}"]
     os.makedirs(LIB_DIR, exist_ok=True)
     if verbose:
         print(" ".join(cmd), flush=True)
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
-        raise RuntimeError(f"param_key build failed:\n{r.stdout}\n{r.stderr}")
-    os.replace(PARAM_KEY_LIB + ".tmp", PARAM_KEY_LIB)
-    return PARAM_KEY_LIB
+        raise RuntimeError(f"{name} build failed:\n{r.stdout}\n{r.stderr}")
+    os.replace(out + ".tmp", out)
+    return out
 
 
 def build(force: bool = False, verbose: bool = False, extra: list[str] | None = None) -> str:
-    """Compile and link the library (and the modules' host helper); returns the library's
-    path.  Skips work when up to date."""
-    build_param_key(force=force, verbose=verbose)
-    if not force and not extra and up_to_date():
-        return LIB
+    """Compile and link the library (and the PyTorch layer's host helpers); returns the
+    library's path.  Skips work when up to date."""
+    build_host_module("param_key", force=force, verbose=verbose)
+    if force or extra or not up_to_date():
+        _build_library(verbose, extra)
+    build_host_module("dense_ops", force=force, verbose=verbose)
+    return LIB
+
+
+def _build_library(verbose: bool, extra: list[str] | None) -> None:
     os.makedirs(BUILD, exist_ok=True)
     os.makedirs(LIB_DIR, exist_ok=True)
     srcs = sources()
     with cf.ThreadPoolExecutor(max_workers=min(8, len(srcs))) as ex:
         objs = list(ex.map(lambda s: _compile(s, verbose, extra or []), srcs))
     tmp = LIB + ".tmp"
-    cmd = [nvcc(), *ARCH, "-shared", "-o", tmp, *objs, "-Xcompiler", "-fPIC"]
+    cmd = [nvcc(), *ARCH, "-shared", "-o", tmp, *objs, "-Xcompiler", "-fPIC",
+           "-Xlinker", "-soname=libvesper_moe.so"]
     if verbose:
         print(" ".join(cmd), flush=True)
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, LIB)
-    return LIB
 
 
 if __name__ == "__main__":

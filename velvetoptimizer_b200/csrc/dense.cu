@@ -3,10 +3,17 @@
 //
 // Every call first lays its workspace out (Arena), then launches; the size functions run the
 // same layout without a base.  Nothing is allocated and the host never waits.
+#include <atomic>
+
 #include "dense.h"
 #include "ops_host.h"
 
 namespace {
+
+// Status words of the contexts, zero from the module's load on (contexts past this number
+// share them).
+constexpr int kStatusWords = 256;
+__device__ int g_ops_status[kStatusWords];
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 bool vec_ok(const void* p, int64_t ld, size_t elt) {
@@ -686,23 +693,26 @@ int vmoe_ops_create(int device, vmoe_ops** out) {
   cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device);
   cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, device);
   o->sm100 = major == 10 && minor == 0;
-  cudaError_t e = cudaMalloc(&o->status, sizeof(int));
-  if (e == cudaSuccess) e = cudaMemset(o->status, 0, sizeof(int));
+  // a status word of the library's own: a thread whose first call falls into a stream capture
+  // (a captured backward on autograd's thread) must allocate and clear nothing
+  static std::atomic<unsigned> next{0};
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  void* words = nullptr;
+  const cudaError_t e = cudaGetSymbolAddress(&words, g_ops_status);
+  cudaThreadExchangeStreamCaptureMode(&mode);
   if (e != cudaSuccess) {
     fprintf(stderr, "vmoe_ops_create: %s\n", cudaGetErrorString(e));
-    vmoe_ops_destroy(o);
+    delete o;
     return VMOE_ERR_CUDA;
   }
+  o->status = static_cast<int*>(words) + next.fetch_add(1) % kStatusWords;
   *out = o;
   return VMOE_OK;
 }
 
 int vmoe_ops_destroy(vmoe_ops* o) {
   if (!o) return VMOE_ERR_INVALID_ARG;
-  {
-    DeviceGuard g(o->device);
-    if (o->status) cudaFree(o->status);
-  }
   delete o;
   return VMOE_OK;
 }

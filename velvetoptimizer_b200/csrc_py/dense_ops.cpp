@@ -1,0 +1,507 @@
+// Host path of velvetoptimizer_b200.linear and .gated_ffn for eager calls: argument checks,
+// output and workspace tensors, the C-ABI call and the autograd node, in C++.  The same work
+// done in Python and ctypes takes 30 us a forward and 100 us a backward, several times what
+// the kernels of a one-token call take.
+#include <torch/extension.h>
+
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+
+#include <array>
+
+#include "vesper_moe.h"
+
+namespace {
+
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+using OptTensor = std::optional<Tensor>;
+
+// A status of the C ABI other than VMOE_OK; becomes _lib.VmoeError in Python.
+struct AbiError : std::runtime_error {
+  int code;
+  AbiError(int c, const std::string& what) : std::runtime_error(what), code(c) {}
+};
+
+// The calling thread's contexts, one per device (calls on one context must not overlap).
+struct Contexts {
+  std::array<vmoe_ops*, 64> of{};
+  ~Contexts() {
+    for (vmoe_ops* o : of)
+      if (o) vmoe_ops_destroy(o);
+  }
+};
+
+vmoe_ops* context(const Tensor& x) {
+  static thread_local Contexts contexts;
+  const int d = x.get_device();
+  TORCH_CHECK(d >= 0 && d < 64, "device index ", d, " is not supported");
+  if (!contexts.of[d]) {
+    const int rc = vmoe_ops_create(d, &contexts.of[d]);
+    if (rc != VMOE_OK)
+      throw AbiError(rc, std::string("vmoe_ops_create failed: ") + vmoe_status_string(rc));
+  }
+  return contexts.of[d];
+}
+
+void check(vmoe_ops* o, int rc, const char* what) {
+  if (rc == VMOE_OK) return;
+  throw AbiError(rc, std::string(what) + " failed: " + vmoe_status_string(rc) + " (" +
+                         vmoe_ops_last_error(o) + ")");
+}
+
+int32_t dtype_of(at::ScalarType t) { return t == at::kFloat ? VMOE_F32 : VMOE_BF16; }
+bool supported(at::ScalarType t) { return t == at::kFloat || t == at::kBFloat16; }
+
+bool misaligned(const Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) != 0; }
+
+// The matrix as the kernels read it, and its row pitch: itself where its rows are contiguous
+// (and 16-byte aligned where the pitch is), else a contiguous copy.
+Tensor rows(const Tensor& t, int64_t& ld) {
+  const int64_t r = t.size(0), c = t.size(1), s0 = t.stride(0), s1 = t.stride(1);
+  if ((s1 == 1 || c == 1) && (r <= 1 || s0 >= c)) {
+    ld = r > 1 ? s0 : c;
+    if (t.scalar_type() == at::kFloat || ld % 8 != 0 || !misaligned(t)) return t;
+    ld = c;
+    return t.clone(at::MemoryFormat::Contiguous);
+  }
+  ld = c;
+  return t.contiguous();
+}
+
+// The same for an output's gradient, whose pitch is its row length or a multiple of 8.
+Tensor grad_rows(const Tensor& t, int64_t& ld) {
+  Tensor m = rows(t, ld);
+  if (ld != t.size(1) && ld % 8 != 0 && t.scalar_type() == at::kBFloat16) {
+    m = m.contiguous();
+    ld = t.size(1);
+  }
+  return m;
+}
+
+Tensor packed(const Tensor& t) {
+  Tensor m = t.contiguous();
+  return misaligned(m) ? m.clone(at::MemoryFormat::Contiguous) : m;
+}
+
+const void* ptr(const OptTensor& t) { return t && t->defined() ? t->data_ptr() : nullptr; }
+
+struct Workspace {
+  Tensor t;
+  void* p = nullptr;
+  size_t n = 0;
+  Workspace(size_t bytes, const Tensor& like) {
+    if (bytes == 0) return;
+    t = at::empty({static_cast<int64_t>(bytes)}, like.options().dtype(at::kByte));
+    p = t.data_ptr();
+    n = bytes;
+  }
+};
+
+void* stream_of(const Tensor& x) {
+  return c10::cuda::getCurrentCUDAStream(x.get_device()).stream();
+}
+
+OptTensor contiguous(const OptTensor& b) {
+  return b && b->defined() ? OptTensor(b->contiguous()) : std::nullopt;
+}
+
+// ---- linear -----------------------------------------------------------------------------
+// (y [T, N], z [T, N] or empty) for x [T, K]
+std::tuple<Tensor, Tensor> linear_forward(const Tensor& x_in, const Tensor& w_in,
+                                          const OptTensor& bias, const OptTensor& residual,
+                                          int64_t act, double gamma, bool keep) {
+  vmoe_ops* o = context(x_in);
+  vmoe_linear d{};
+  d.tokens = x_in.size(0);
+  d.in_features = x_in.size(1);
+  d.out_features = w_in.size(0);
+  const Tensor x = rows(x_in, d.ldx), w = rows(w_in, d.ldw);
+  Tensor r;
+  d.ldr = d.out_features;
+  if (residual && residual->defined()) r = rows(*residual, d.ldr);
+  const OptTensor b = contiguous(bias);
+  d.dtype = d.grad_dtype = dtype_of(x.scalar_type());
+  d.activation = static_cast<int32_t>(act);
+  d.gamma = static_cast<float>(gamma);
+  Tensor y = at::empty({d.tokens, d.out_features}, x.options());
+  Tensor z = keep ? at::empty({d.tokens, d.out_features}, x.options()) : at::empty({0}, x.options());
+  size_t need = 0;
+  check(o, vmoe_linear_workspace_size(o, &d, 0, &need), "vmoe_linear_workspace_size");
+  const Workspace ws(need, x);
+  check(o,
+        vmoe_linear_forward(o, &d, x.data_ptr(), w.data_ptr(), ptr(b),
+                            r.defined() ? r.data_ptr() : nullptr, y.data_ptr(),
+                            keep ? z.data_ptr() : nullptr, ws.p, ws.n, stream_of(x)),
+        "vmoe_linear_forward");
+  return {y, z};
+}
+
+// (dx, dW, db), empty where not wanted
+std::tuple<Tensor, Tensor, Tensor> linear_backward(const Tensor& x_in, const Tensor& w_in,
+                                                   const Tensor& z, const Tensor& dy_in,
+                                                   int64_t act, double gamma,
+                                                   const std::vector<bool>& want, bool grad_f32) {
+  vmoe_ops* o = context(x_in);
+  vmoe_linear d{};
+  d.tokens = x_in.size(0);
+  d.in_features = x_in.size(1);
+  d.out_features = w_in.size(0);
+  int64_t lddy = 0;
+  const Tensor x = rows(x_in, d.ldx), w = rows(w_in, d.ldw), dy = grad_rows(dy_in, lddy);
+  d.ldr = d.out_features;
+  d.dtype = dtype_of(x.scalar_type());
+  d.activation = static_cast<int32_t>(act);
+  d.gamma = static_cast<float>(gamma);
+  d.grad_dtype = grad_f32 ? VMOE_F32 : d.dtype;
+  const auto xo = x.options();
+  const auto go = grad_f32 ? xo.dtype(at::kFloat) : xo;
+  Tensor dx = want[0] ? at::empty({d.tokens, d.in_features}, xo) : at::empty({0}, xo);
+  Tensor dw = want[1] ? at::empty({d.out_features, d.in_features}, go) : at::empty({0}, go);
+  Tensor db = want[2] ? at::empty({d.out_features}, go) : at::empty({0}, go);
+  size_t need = 0;
+  check(o, vmoe_linear_workspace_size(o, &d, 1, &need), "vmoe_linear_workspace_size");
+  const Workspace ws(need, x);
+  check(o,
+        vmoe_linear_backward(o, &d, x.data_ptr(), w.data_ptr(),
+                             z.numel() ? z.data_ptr() : nullptr, dy.data_ptr(), lddy,
+                             want[0] ? dx.data_ptr() : nullptr, want[1] ? dw.data_ptr() : nullptr,
+                             want[2] ? db.data_ptr() : nullptr, ws.p, ws.n, stream_of(x)),
+        "vmoe_linear_backward");
+  return {dx, dw, db};
+}
+
+// ---- gated feed-forward block -------------------------------------------------------------
+vmoe_gated_ffn ffn_desc(const Tensor& x, int64_t inter, int64_t act, double gamma) {
+  vmoe_gated_ffn d{};
+  d.tokens = x.size(0);
+  d.hidden = x.size(1);
+  d.inter = inter;
+  d.ldr = d.hidden;
+  d.dtype = d.grad_dtype = dtype_of(x.scalar_type());
+  d.activation = static_cast<int32_t>(act);
+  d.gamma = static_cast<float>(gamma);
+  return d;
+}
+
+// (y [T, H], what the backward reads, as bytes, or empty) for x [T, H]
+std::tuple<Tensor, Tensor> gated_ffn_forward(const Tensor& x_in, const Tensor& gate_w,
+                                             const Tensor& up_w, const Tensor& down_w,
+                                             const OptTensor& gate_b, const OptTensor& up_b,
+                                             const OptTensor& down_b, const OptTensor& residual,
+                                             int64_t act, double gamma, bool keep) {
+  vmoe_ops* o = context(x_in);
+  vmoe_gated_ffn d = ffn_desc(x_in, gate_w.size(0), act, gamma);
+  const Tensor x = rows(x_in, d.ldx);
+  Tensor r;
+  if (residual && residual->defined()) r = rows(*residual, d.ldr);
+  const Tensor wg = packed(gate_w), wu = packed(up_w), wd = packed(down_w);
+  const OptTensor bg = contiguous(gate_b), bu = contiguous(up_b), bd = contiguous(down_b);
+  const vmoe_ffn_weights w{wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), ptr(bg), ptr(bu), ptr(bd)};
+  size_t need = 0, saved_bytes = 0;
+  check(o, vmoe_gated_ffn_workspace_size(o, &d, 0, &need, &saved_bytes),
+        "vmoe_gated_ffn_workspace_size");
+  Tensor y = at::empty({d.tokens, d.hidden}, x.options());
+  Tensor saved = at::empty({keep ? static_cast<int64_t>(saved_bytes) : 0},
+                           x.options().dtype(at::kByte));
+  const Workspace ws(need, x);
+  const bool kept = saved.numel() > 0;
+  check(o,
+        vmoe_gated_ffn_forward(o, &d, x.data_ptr(), &w, r.defined() ? r.data_ptr() : nullptr,
+                               y.data_ptr(), kept ? saved.data_ptr() : nullptr,
+                               kept ? saved_bytes : 0, ws.p, ws.n, stream_of(x)),
+        "vmoe_gated_ffn_forward");
+  return {y, saved};
+}
+
+// (dx, dWg, dWu, dWd, dbg, dbu, dbd), empty where not wanted
+std::array<Tensor, 7> gated_ffn_backward_array(const Tensor& x_in, const Tensor& gate_w,
+                                               const Tensor& up_w, const Tensor& down_w,
+                                               const Tensor& saved, const Tensor& dy_in,
+                                               int64_t act, double gamma,
+                                               const std::vector<bool>& want, bool grad_f32) {
+  vmoe_ops* o = context(x_in);
+  const int64_t I = gate_w.size(0), H = x_in.size(1);
+  vmoe_gated_ffn d = ffn_desc(x_in, I, act, gamma);
+  if (grad_f32) d.grad_dtype = VMOE_F32;
+  int64_t lddy = 0;
+  const Tensor x = rows(x_in, d.ldx), dy = grad_rows(dy_in, lddy);
+  const Tensor wg = packed(gate_w), wu = packed(up_w), wd = packed(down_w);
+  const vmoe_ffn_weights w{wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), nullptr, nullptr, nullptr};
+  const std::array<std::vector<int64_t>, 7> shapes{
+      {{d.tokens, H}, {I, H}, {I, H}, {H, I}, {I}, {I}, {H}}};
+  std::array<Tensor, 7> out;
+  std::array<void*, 7> p{};
+  const auto xo = x.options();
+  const auto go = grad_f32 ? xo.dtype(at::kFloat) : xo;
+  for (size_t i = 0; i < 7; ++i) {
+    out[i] = want[i] ? at::empty(shapes[i], i ? go : xo) : at::empty({0}, i ? go : xo);
+    p[i] = want[i] ? out[i].data_ptr() : nullptr;
+  }
+  const vmoe_ffn_grads g{p[1], p[2], p[3], p[4], p[5], p[6]};
+  size_t need = 0;
+  check(o, vmoe_gated_ffn_workspace_size(o, &d, 1, &need, nullptr), "vmoe_gated_ffn_workspace_size");
+  const Workspace ws(need, x);
+  check(o,
+        vmoe_gated_ffn_backward(o, &d, x.data_ptr(), &w, dy.data_ptr(), lddy, p[0], &g,
+                                saved.data_ptr(), static_cast<size_t>(saved.numel()), ws.p, ws.n,
+                                stream_of(x)),
+        "vmoe_gated_ffn_backward");
+  return out;
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> gated_ffn_backward(
+    const Tensor& x, const Tensor& gate_w, const Tensor& up_w, const Tensor& down_w,
+    const Tensor& saved, const Tensor& dy, int64_t act, double gamma,
+    const std::vector<bool>& want, bool grad_f32) {
+  auto r = gated_ffn_backward_array(x, gate_w, up_w, down_w, saved, dy, act, gamma, want, grad_f32);
+  return {r[0], r[1], r[2], r[3], r[4], r[5], r[6]};
+}
+
+// ---- autograd -----------------------------------------------------------------------------
+OptTensor cast(const OptTensor& p, const Tensor& x) {
+  return p && p->defined() ? OptTensor(p->to(x.scalar_type())) : std::nullopt;
+}
+
+// Which of `n` optional inputs the running backward needs (absent ones have no edge).
+struct Needs {
+  AutogradContext* ctx;
+  size_t edge = 0;
+  bool next(bool present) { return present && ctx->needs_input_grad(edge++); }
+};
+
+// The gradients have no gradient: differentiating through them raises.
+variable_list once(variable_list grads) {
+  if (!at::GradMode::is_enabled()) return grads;
+  variable_list fake;
+  std::vector<size_t> at;
+  for (size_t i = 0; i < grads.size(); ++i) {
+    if (!grads[i].defined()) continue;
+    fake.push_back(grads[i].detach().set_requires_grad(true));
+    at.push_back(i);
+  }
+  auto node = std::make_shared<torch::autograd::DelayedError>(
+      "the gradients of linear and gated_ffn cannot be differentiated", static_cast<int64_t>(fake.size()));
+  variable_list out = (*node)(std::move(fake));
+  for (size_t i = 0; i < at.size(); ++i) grads[at[i]] = out[i];
+  return grads;
+}
+
+Tensor to_param(const Tensor& g, int64_t type) {
+  return g.to(static_cast<at::ScalarType>(type));
+}
+
+struct LinearFn : public torch::autograd::Function<LinearFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight,
+                        const OptTensor& bias, const OptTensor& residual, int64_t act,
+                        double gamma) {
+    const Tensor w = weight.to(x.scalar_type());
+    const bool has_b = bias && bias->defined(), has_r = residual && residual->defined();
+    const bool keep = act != VMOE_ACT_NONE && (x.requires_grad() || weight.requires_grad() ||
+                                               (has_b && bias->requires_grad()));
+    auto [y, z] = linear_forward(x, w, cast(bias, x), residual, act, gamma, keep);
+    ctx->save_for_backward({x, w, z});
+    ctx->saved_data["args"] = std::tuple<int64_t, double>(act, gamma);
+    ctx->saved_data["types"] = std::vector<int64_t>{
+        static_cast<int64_t>(weight.scalar_type()),
+        static_cast<int64_t>(has_b ? bias->scalar_type() : weight.scalar_type()), has_b, has_r};
+    return y;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list dys) {
+    const auto saved = ctx->get_saved_variables();
+    const auto types = ctx->saved_data["types"].toIntVector();
+    const auto args = ctx->saved_data["args"].toTuple();
+    Needs needs{ctx};
+    const bool nx = needs.next(true), nw = needs.next(true), nb = needs.next(types[2]),
+               nr = needs.next(types[3]);
+    variable_list out(6);
+    if (nx || nw || nb) {
+      at::NoGradGuard no_grad;
+      const bool f32 = types[0] == static_cast<int64_t>(at::kFloat) ||
+                       types[1] == static_cast<int64_t>(at::kFloat);
+      auto [dx, dw, db] = linear_backward(
+          saved[0], saved[1], saved[2], dys[0], args->elements()[0].toInt(),
+          args->elements()[1].toDouble(), {nx, nw, nb}, f32);
+      if (nx) out[0] = dx;
+      if (nw) out[1] = to_param(dw, types[0]);
+      if (nb) out[2] = to_param(db, types[1]);
+    }
+    out = once(std::move(out));
+    if (nr) out[3] = dys[0];
+    return out;
+  }
+};
+
+struct GatedFfnFn : public torch::autograd::Function<GatedFfnFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& gate_w,
+                        const Tensor& up_w, const Tensor& down_w, const OptTensor& gate_b,
+                        const OptTensor& up_b, const OptTensor& down_b, const OptTensor& residual,
+                        int64_t act, double gamma) {
+    const std::array<OptTensor, 6> params{gate_w, up_w, down_w, gate_b, up_b, down_b};
+    bool keep = x.requires_grad(), f32 = false;
+    std::vector<int64_t> types;
+    for (const auto& p : params) {
+      const bool has = p && p->defined();
+      keep = keep || (has && p->requires_grad());
+      f32 = f32 || (has && p->scalar_type() == at::kFloat);
+      types.push_back(has ? static_cast<int64_t>(p->scalar_type()) : -1);
+    }
+    types.push_back(residual && residual->defined());
+    types.push_back(f32);
+    const Tensor wg = gate_w.to(x.scalar_type()), wu = up_w.to(x.scalar_type()),
+                 wd = down_w.to(x.scalar_type());
+    auto [y, saved] = gated_ffn_forward(x, wg, wu, wd, cast(gate_b, x), cast(up_b, x),
+                                        cast(down_b, x), residual, act, gamma, keep);
+    ctx->save_for_backward({x, wg, wu, wd, saved});
+    ctx->saved_data["args"] = std::tuple<int64_t, double>(act, gamma);
+    ctx->saved_data["types"] = types;
+    return y;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list dys) {
+    const auto saved = ctx->get_saved_variables();
+    const auto types = ctx->saved_data["types"].toIntVector();
+    const auto args = ctx->saved_data["args"].toTuple();
+    Needs needs{ctx};
+    std::vector<bool> want{needs.next(true)};
+    for (size_t i = 0; i < 6; ++i) want.push_back(needs.next(types[i] >= 0));
+    const bool nr = needs.next(types[6]);
+    variable_list out(10);
+    bool any = false;
+    for (const bool b : want) any = any || b;
+    if (any) {
+      at::NoGradGuard no_grad;
+      auto got = gated_ffn_backward_array(saved[0], saved[1], saved[2], saved[3], saved[4], dys[0],
+                                          args->elements()[0].toInt(),
+                                          args->elements()[1].toDouble(), want, types[7]);
+      for (size_t i = 0; i < 7; ++i)
+        if (want[i]) out[i] = i ? to_param(got[i], types[i - 1]) : got[i];
+    }
+    out = once(std::move(out));
+    if (nr) out[7] = dys[0];
+    return out;
+  }
+};
+
+// ---- the operators ------------------------------------------------------------------------
+void check_x(const char* name, const Tensor& x) {
+  TORCH_CHECK_TYPE(supported(x.scalar_type()), name, " supports float32 and bfloat16 inputs, not ",
+                   x.scalar_type());
+  TORCH_CHECK(x.is_cuda(), name, " runs on CUDA tensors only (there is no CPU path)");
+  TORCH_CHECK_VALUE(x.dim() >= 1, name, ": x must have a feature dimension");
+}
+
+void check_param(const char* name, const char* label, const OptTensor& p, at::IntArrayRef shape,
+                 const Tensor& x) {
+  if (!p || !p->defined()) return;
+  TORCH_CHECK_VALUE(p->sizes() == shape, name, ": ", label, " must have shape ", shape, ", not ",
+                    p->sizes());
+  TORCH_CHECK_VALUE(p->device() == x.device(), name, ": ", label, " is on ", p->device(),
+                    ", x on ", x.device());
+  TORCH_CHECK_TYPE(supported(p->scalar_type()), name, ": ", label,
+                   " must be float32 or bfloat16, not ", p->scalar_type());
+}
+
+OptTensor check_residual(const char* name, const OptTensor& r, at::IntArrayRef shape,
+                         const Tensor& x) {
+  if (!r || !r->defined()) return std::nullopt;
+  TORCH_CHECK_VALUE(r->sizes() == shape, name, ": residual must have shape ", shape, ", not ",
+                    r->sizes());
+  TORCH_CHECK_TYPE(r->device() == x.device() && r->scalar_type() == x.scalar_type(), name,
+                   ": residual must be ", x.scalar_type(), " on ", x.device(), ", as x is");
+  return r;
+}
+
+// [rows, features] of a tensor with any leading dimensions
+Tensor flat(const Tensor& t) {
+  return t.dim() == 2 ? t : t.reshape({t.numel() / t.size(-1), t.size(-1)});
+}
+
+bool wants(const OptTensor& t) { return t && t->defined() && t->requires_grad(); }
+
+Tensor linear(const Tensor& x, const Tensor& weight, const OptTensor& bias,
+              const OptTensor& residual, int64_t act, double gamma) {
+  check_x("linear", x);
+  TORCH_CHECK_VALUE(weight.dim() == 2 && weight.size(1) == x.size(-1) && weight.numel() > 0,
+                    "linear: weight must be [N, ", x.size(-1), "] with N and K at least 1, not ",
+                    weight.sizes());
+  const int64_t N = weight.size(0);
+  check_param("linear", "weight", weight, weight.sizes(), x);
+  check_param("linear", "bias", bias, {N}, x);
+  auto shape = x.sizes().vec();
+  shape.back() = N;
+  OptTensor r = check_residual("linear", residual, shape, x);
+  if (r) r = flat(*r);
+  const Tensor x2 = flat(x);
+  Tensor y;
+  if (at::GradMode::is_enabled() && (wants(x) || wants(weight) || wants(bias) || wants(residual))) {
+    y = LinearFn::apply(x2, weight, bias, r, act, gamma);
+  } else {
+    at::NoGradGuard no_grad;
+    y = std::get<0>(linear_forward(x2, weight.to(x.scalar_type()), cast(bias, x), r, act, gamma, false));
+  }
+  return x.dim() == 2 ? y : y.reshape(shape);
+}
+
+Tensor gated_ffn(const Tensor& x, const Tensor& gate_w, const Tensor& up_w, const Tensor& down_w,
+                 const OptTensor& gate_b, const OptTensor& up_b, const OptTensor& down_b,
+                 const OptTensor& residual, int64_t act, double gamma) {
+  const char* name = "gated_ffn";
+  check_x(name, x);
+  const int64_t H = x.size(-1);
+  TORCH_CHECK_VALUE(gate_w.dim() == 2 && gate_w.size(1) == H && gate_w.numel() > 0, name,
+                    ": gate_weight must be [I, ", H, "] with I and H at least 1, not ",
+                    gate_w.sizes());
+  const int64_t I = gate_w.size(0);
+  check_param(name, "gate_weight", gate_w, {I, H}, x);
+  check_param(name, "up_weight", up_w, {I, H}, x);
+  check_param(name, "down_weight", down_w, {H, I}, x);
+  check_param(name, "gate_bias", gate_b, {I}, x);
+  check_param(name, "up_bias", up_b, {I}, x);
+  check_param(name, "down_bias", down_b, {H}, x);
+  OptTensor r = check_residual(name, residual, x.sizes(), x);
+  if (r) r = flat(*r);
+  const Tensor x2 = flat(x);
+  Tensor y;
+  if (at::GradMode::is_enabled() &&
+      (wants(x) || wants(gate_w) || wants(up_w) || wants(down_w) || wants(gate_b) || wants(up_b) ||
+       wants(down_b) || wants(residual))) {
+    y = GatedFfnFn::apply(x2, gate_w, up_w, down_w, gate_b, up_b, down_b, r, act, gamma);
+  } else {
+    at::NoGradGuard no_grad;
+    const auto t = x.scalar_type();
+    y = std::get<0>(gated_ffn_forward(x2, gate_w.to(t), up_w.to(t), down_w.to(t), cast(gate_b, x),
+                                      cast(up_b, x), cast(down_b, x), r, act, gamma, false));
+  }
+  return x.dim() == 2 ? y : y.reshape(x.sizes());
+}
+
+}  // namespace
+
+PYBIND11_MODULE(_dense_ops, m) {
+  py::register_exception_translator([](std::exception_ptr p) {
+    try {
+      if (p) std::rethrow_exception(p);
+    } catch (const AbiError& e) {
+      py::object type = py::module_::import("velvetoptimizer_b200._lib").attr("VmoeError");
+      py::object value = type(e.code, e.what());
+      PyErr_SetObject(type.ptr(), value.ptr());
+    }
+  });
+  using Release = py::call_guard<py::gil_scoped_release>;
+  m.def("linear", &linear, Release());
+  m.def("gated_ffn", &gated_ffn, Release());
+  m.def("linear_forward", &linear_forward, Release());
+  m.def("linear_backward", &linear_backward, Release());
+  m.def("gated_ffn_forward", &gated_ffn_forward, Release());
+  m.def("gated_ffn_backward", &gated_ffn_backward, Release());
+  m.def("device_status", [](const Tensor& x) {
+    int32_t code = 0;
+    vmoe_ops* o = context(x);
+    check(o, vmoe_ops_device_status(o, &code, stream_of(x)), "vmoe_ops_device_status");
+    return code;
+  });
+}

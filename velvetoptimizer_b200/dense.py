@@ -13,7 +13,6 @@ to x's type for the call, and their gradients come back in their own type, from 
 """
 from __future__ import annotations
 
-import ctypes
 import threading
 
 import torch
@@ -36,51 +35,21 @@ def ops_for(device: torch.device) -> _lib.Ops:
     return o
 
 
+def _native():
+    """The host module of the eager path (csrc_py/dense_ops.cpp, built beside the library)."""
+    global _module
+    if _module is None:
+        _lib.load()
+        from .lib import _dense_ops
+        _module = _dense_ops
+    return _module
+
+
+_module = None
+
+
 def _eager(x: torch.Tensor) -> bool:
     return type(x) in (torch.Tensor, torch.nn.Parameter) and not torch.compiler.is_compiling()
-
-
-def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
-    """The matrix ``t`` as the kernels read it, and its row pitch: itself where its rows are
-    contiguous (and 16-byte aligned where the pitch is), else a contiguous copy."""
-    r, c = t.shape
-    s0, s1 = t.stride()
-    if (s1 == 1 or c == 1) and (r <= 1 or s0 >= c):
-        ld = s0 if r > 1 else c
-        if t.dtype == torch.float32 or ld % 8 or t.data_ptr() % 16 == 0:
-            return t, ld
-        return t.clone(memory_format=torch.contiguous_format), c
-    return t.contiguous(), c
-
-
-def _packed(t: torch.Tensor) -> torch.Tensor:
-    """``t`` with contiguous, aligned rows."""
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
-
-
-def _grad_rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
-    t, ld = _rows(t)
-    if ld != t.shape[1] and ld % 8 and t.dtype == torch.bfloat16:
-        t = t.contiguous()
-        ld = t.shape[1]
-    return t, ld
-
-
-def _ptr(t: torch.Tensor | None):
-    return None if t is None else t.data_ptr()
-
-
-def _workspace(size: int, device) -> torch.Tensor | None:
-    return torch.empty(size, dtype=torch.uint8, device=device) if size else None
-
-
-def _ws_args(ws: torch.Tensor | None):
-    return (None, 0) if ws is None else (ws.data_ptr(), ws.numel())
-
-
-def _stream(t: torch.Tensor):
-    return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
 
 
 # ------------------------------------------------------------------------------ the kernels
@@ -88,58 +57,14 @@ def _linear_forward(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | 
                     residual: torch.Tensor | None, activation: int, gamma: float,
                     keep: bool) -> tuple[torch.Tensor, torch.Tensor]:
     """(y [T, N], z [T, N] or empty) for x [T, K]."""
-    o = ops_for(x.device)
-    T, N = x.shape[0], weight.shape[0]
-    x, ldx = _rows(x)
-    weight, ldw = _rows(weight)
-    ldr = N
-    if residual is not None:
-        residual, ldr = _rows(residual)
-    if bias is not None:
-        bias = bias.contiguous()
-    y = torch.empty((T, N), dtype=x.dtype, device=x.device)
-    z = torch.empty((T, N) if keep else (0,), dtype=x.dtype, device=x.device)
-    d = _lib.VmoeLinear(T, x.shape[1], N, ldx, ldw, ldr, _DTYPES[x.dtype], activation, gamma,
-                        _DTYPES[x.dtype])
-    n = ctypes.c_size_t()
-    o.check(o.lib.vmoe_linear_workspace_size(o.ptr, d, 0, n), "vmoe_linear_workspace_size")
-    ws = _workspace(n.value, x.device)
-    o.check(o.lib.vmoe_linear_forward(o.ptr, d, x.data_ptr(), weight.data_ptr(), _ptr(bias),
-                                      _ptr(residual), y.data_ptr(), z.data_ptr() if keep else None,
-                                      *_ws_args(ws), _stream(x)), "vmoe_linear_forward")
-    return y, z
+    return _native().linear_forward(x, weight, bias, residual, activation, gamma, keep)
 
 
 def _linear_backward(x: torch.Tensor, weight: torch.Tensor, z: torch.Tensor, dy: torch.Tensor,
                      activation: int, gamma: float, want: list[bool],
                      grad_f32: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(dx, dW, db), empty where not wanted."""
-    o = ops_for(x.device)
-    (T, K), N = x.shape, weight.shape[0]
-    x, ldx = _rows(x)
-    weight, ldw = _rows(weight)
-    dy, lddy = _grad_rows(dy)
-    gt = torch.float32 if grad_f32 else x.dtype
-    new = lambda on, shape, dt: torch.empty(shape if on else (0,), dtype=dt, device=x.device)  # noqa: E731
-    dx, dw, db = new(want[0], (T, K), x.dtype), new(want[1], (N, K), gt), new(want[2], (N,), gt)
-    d = _lib.VmoeLinear(T, K, N, ldx, ldw, N, _DTYPES[x.dtype], activation, gamma, _DTYPES[gt])
-    n = ctypes.c_size_t()
-    o.check(o.lib.vmoe_linear_workspace_size(o.ptr, d, 1, n), "vmoe_linear_workspace_size")
-    ws = _workspace(n.value, x.device)
-    o.check(o.lib.vmoe_linear_backward(
-        o.ptr, d, x.data_ptr(), weight.data_ptr(), z.data_ptr() if z.numel() else None,
-        dy.data_ptr(), lddy, dx.data_ptr() if want[0] else None, dw.data_ptr() if want[1] else None,
-        db.data_ptr() if want[2] else None, *_ws_args(ws), _stream(x)), "vmoe_linear_backward")
-    return dx, dw, db
-
-
-def _ffn_desc(x, ldx, ldr, inter, activation, gamma, grad_dtype) -> _lib.VmoeGatedFfn:
-    return _lib.VmoeGatedFfn(x.shape[0], x.shape[1], inter, ldx, ldr, _DTYPES[x.dtype], activation,
-                             gamma, grad_dtype)
-
-
-def _ffn_weights(weights) -> _lib.VmoeFfnWeights:
-    return _lib.VmoeFfnWeights(*(_ptr(w) for w in weights))
+    return _native().linear_backward(x, weight, z, dy, activation, gamma, want, grad_f32)
 
 
 def _gated_ffn_forward(x: torch.Tensor, gate_w: torch.Tensor, up_w: torch.Tensor,
@@ -148,24 +73,8 @@ def _gated_ffn_forward(x: torch.Tensor, gate_w: torch.Tensor, up_w: torch.Tensor
                        residual: torch.Tensor | None, activation: int, gamma: float,
                        keep: bool) -> tuple[torch.Tensor, torch.Tensor]:
     """(y [T, H], what the backward reads, as bytes, or empty) for x [T, H]."""
-    o = ops_for(x.device)
-    x, ldx = _rows(x)
-    ldr = x.shape[1]
-    if residual is not None:
-        residual, ldr = _rows(residual)
-    weights = [_packed(w) for w in (gate_w, up_w, down_w)]
-    weights += [None if b is None else b.contiguous() for b in (gate_b, up_b, down_b)]
-    d = _ffn_desc(x, ldx, ldr, gate_w.shape[0], activation, gamma, _DTYPES[x.dtype])
-    n, m = ctypes.c_size_t(), ctypes.c_size_t()
-    o.check(o.lib.vmoe_gated_ffn_workspace_size(o.ptr, d, 0, n, m), "vmoe_gated_ffn_workspace_size")
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    saved = torch.empty(m.value if keep else 0, dtype=torch.uint8, device=x.device)
-    ws = _workspace(n.value, x.device)
-    kept = (saved.data_ptr(), saved.numel()) if saved.numel() else (None, 0)
-    o.check(o.lib.vmoe_gated_ffn_forward(o.ptr, d, x.data_ptr(), _ffn_weights(weights),
-                                         _ptr(residual), y.data_ptr(), *kept, *_ws_args(ws),
-                                         _stream(x)), "vmoe_gated_ffn_forward")
-    return y, saved
+    return _native().gated_ffn_forward(x, gate_w, up_w, down_w, gate_b, up_b, down_b, residual,
+                                       activation, gamma, keep)
 
 
 def _gated_ffn_backward(x: torch.Tensor, gate_w: torch.Tensor, up_w: torch.Tensor,
@@ -174,29 +83,12 @@ def _gated_ffn_backward(x: torch.Tensor, gate_w: torch.Tensor, up_w: torch.Tenso
                             torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor,
                             torch.Tensor, torch.Tensor]:
     """(dx, dWg, dWu, dWd, dbg, dbu, dbd), empty where not wanted."""
-    o = ops_for(x.device)
-    x, ldx = _rows(x)
-    H, I = x.shape[1], gate_w.shape[0]
-    dy, lddy = _grad_rows(dy)
-    weights = [_packed(w) for w in (gate_w, up_w, down_w)]
-    gt = torch.float32 if grad_f32 else x.dtype
-    shapes = (x.shape, (I, H), (I, H), (H, I), (I,), (I,), (H,))
-    outs = [torch.empty(s if on else (0,), dtype=x.dtype if i == 0 else gt, device=x.device)
-            for i, (s, on) in enumerate(zip(shapes, want))]
-    ptrs = [t.data_ptr() if on else None for t, on in zip(outs, want)]
-    d = _ffn_desc(x, ldx, H, I, activation, gamma, _DTYPES[gt])
-    n = ctypes.c_size_t()
-    o.check(o.lib.vmoe_gated_ffn_workspace_size(o.ptr, d, 1, n, None),
-            "vmoe_gated_ffn_workspace_size")
-    ws = _workspace(n.value, x.device)
-    o.check(o.lib.vmoe_gated_ffn_backward(
-        o.ptr, d, x.data_ptr(), _ffn_weights(weights + [None] * 3), dy.data_ptr(), lddy, ptrs[0],
-        _lib.VmoeFfnGrads(*ptrs[1:]), saved.data_ptr(), saved.numel(), *_ws_args(ws), _stream(x)),
-        "vmoe_gated_ffn_backward")
-    return tuple(outs)
+    return _native().gated_ffn_backward(x, gate_w, up_w, down_w, saved, dy, activation, gamma, want,
+                                        grad_f32)
 
 
-# The bodies above are registered as custom ops for the tracers; eager calls run them directly.
+# Registered as custom ops for the tracers (torch.compile, export); an eager call goes through
+# the native module's own autograd node.
 _custom = lambda name, fn: torch.library.custom_op(  # noqa: E731
     f"vesper_moe::{name}", mutates_args=(), device_types="cuda")(fn)
 linear_forward_op = _custom("linear_forward", _linear_forward)
@@ -236,7 +128,7 @@ def _(x, gate_w, up_w, down_w, saved, dy, activation, gamma, want, grad_f32):
                  for i, (s, on) in enumerate(zip(shapes, want)))
 
 
-# ------------------------------------------------------------------------------ autograd
+# ------------------------------------------------------------------------------ autograd (traced)
 def _as(g: torch.Tensor, like: torch.Tensor) -> torch.Tensor:
     return g if g.dtype == like.dtype else g.to(like.dtype)
 
@@ -244,7 +136,7 @@ def _as(g: torch.Tensor, like: torch.Tensor) -> torch.Tensor:
 class _LinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, activation, gamma):
-        run = _linear_forward if _eager(x) else torch.ops.vesper_moe.linear_forward
+        run = torch.ops.vesper_moe.linear_forward
         w = weight.to(x.dtype)
         b = None if bias is None else bias.to(x.dtype)
         keep = activation != 0 and any(ctx.needs_input_grad[:3])
@@ -261,7 +153,7 @@ class _LinearFn(torch.autograd.Function):
         need = ctx.needs_input_grad
         dx = dw = db = None
         if any(need[:3]):
-            run = _linear_backward if _eager(x) else torch.ops.vesper_moe.linear_backward
+            run = torch.ops.vesper_moe.linear_backward
             grad_f32 = torch.float32 in ctx.types
             dx, dw, db = run(x, w, z, dy, *ctx.args, list(need[:3]), grad_f32)
         return (dx if need[0] else None, dw.to(ctx.types[0]) if need[1] else None,
@@ -271,7 +163,7 @@ class _LinearFn(torch.autograd.Function):
 class _GatedFfnFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate_w, up_w, down_w, gate_b, up_b, down_b, residual, activation, gamma):
-        run = _gated_ffn_forward if _eager(x) else torch.ops.vesper_moe.gated_ffn_forward
+        run = torch.ops.vesper_moe.gated_ffn_forward
         params = (gate_w, up_w, down_w, gate_b, up_b, down_b)
         cast = [None if p is None else p.to(x.dtype) for p in params]
         y, saved = run(x, *cast, residual, activation, gamma, any(ctx.needs_input_grad[:7]))
@@ -287,7 +179,7 @@ class _GatedFfnFn(torch.autograd.Function):
         need = ctx.needs_input_grad
         grads = [None] * 7
         if any(need[:7]):
-            run = _gated_ffn_backward if _eager(x) else torch.ops.vesper_moe.gated_ffn_backward
+            run = torch.ops.vesper_moe.gated_ffn_backward
             got = run(x, gate_w, up_w, down_w, saved, dy, *ctx.args, list(need[:7]),
                       torch.float32 in ctx.types)
             grads = [None if not on else g if i == 0 else g.to(ctx.types[i - 1])
@@ -296,9 +188,8 @@ class _GatedFfnFn(torch.autograd.Function):
 
 
 # ------------------------------------------------------------------------------ the operators
-def _check_x(name: str, x: torch.Tensor, activation: str, allowed) -> None:
-    if activation not in allowed:
-        raise ValueError(f"{name}: activation must be one of {', '.join(allowed)}, not {activation!r}")
+# The eager path checks the same in C++.
+def _check_x(name: str, x: torch.Tensor) -> None:
     if x.device.type != "cuda":
         raise RuntimeError(f"{name} runs on CUDA tensors only (there is no CPU path)")
     if x.dtype not in _DTYPES:
@@ -333,7 +224,12 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     ``gelu_tanh`` and ``era`` (``gelu_tanh + gamma * softplus``, python/vesper/model.py:69-76).
     A training call of an activation keeps the pre-activations in x's type.
     """
-    _check_x("linear", x, activation, ACTIVATIONS)
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"linear: activation must be one of {', '.join(ACTIVATIONS)}, "
+                         f"not {activation!r}")
+    if _eager(x):
+        return _native().linear(x, weight, bias, residual, ACTIVATIONS[activation], gamma)
+    _check_x("linear", x)
     if weight.dim() != 2 or weight.shape[1] != x.shape[-1] or 0 in weight.shape:
         raise ValueError(f"linear: weight must be [N, {x.shape[-1]}] with N and K at least 1, "
                          f"not {list(weight.shape)}")
@@ -350,7 +246,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     act, gamma = ACTIVATIONS[activation], float(gamma)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
         return _LinearFn.apply(*args, act, gamma).reshape(shape)
-    run = _linear_forward if _eager(x) else torch.ops.vesper_moe.linear_forward
+    run = torch.ops.vesper_moe.linear_forward
     cast = [None if t is None else _as(t, x) for t in args]
     return run(*cast, act, gamma, False)[0].reshape(shape)
 
@@ -368,7 +264,13 @@ def gated_ffn(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: torch.Tenso
     x and residual ``[..., H]`` (float32 or bfloat16, any strides), gate and up weights
     ``[I, H]``, down weight ``[H, I]``; ``activation`` as for ``linear``, except ``none``.
     """
-    _check_x("gated_ffn", x, activation, [a for a in ACTIVATIONS if a != "none"])
+    if activation == "none" or activation not in ACTIVATIONS:
+        raise ValueError(f"gated_ffn: activation must be one of {', '.join(ACTIVATIONS)} but none, "
+                         f"not {activation!r}")
+    if _eager(x):
+        return _native().gated_ffn(x, gate_weight, up_weight, down_weight, gate_bias, up_bias,
+                                   down_bias, residual, ACTIVATIONS[activation], gamma)
+    _check_x("gated_ffn", x)
     H = x.shape[-1]
     if gate_weight.dim() != 2 or gate_weight.shape[1] != H or 0 in gate_weight.shape:
         raise ValueError(f"gated_ffn: gate_weight must be [I, {H}] with I and H at least 1, "
@@ -388,6 +290,6 @@ def gated_ffn(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: torch.Tenso
     act, gamma = ACTIVATIONS[activation], float(gamma)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
         return _GatedFfnFn.apply(*args, act, gamma).reshape(x.shape)
-    run = _gated_ffn_forward if _eager(x) else torch.ops.vesper_moe.gated_ffn_forward
+    run = torch.ops.vesper_moe.gated_ffn_forward
     cast = [None if t is None else _as(t, x) for t in args]
     return run(*cast, act, gamma, False)[0].reshape(x.shape)

@@ -33,6 +33,7 @@ from torch.optim.optimizer import register_optimizer_step_post_hook
 
 from . import _lib
 from .config import MoEConfig
+from .dense import gated_ffn, linear
 
 try:  # the (data pointer, version) pairs of a parameter list in one native call
     from .lib._param_key import pairs as _native_pairs
@@ -83,7 +84,8 @@ class FlyLoRALinear(nn.Module):
 
     ``base`` [out,in], ``lora_down`` [r,in], ``lora_up`` [out,r] (zero-initialised, so the
     branch starts switched off, model.py:120) and the unused ``proj_a`` buffer [in,r]
-    (model.py:107-113).  Its math runs inside the fused op, folded into ``base``.
+    (model.py:107-113).  Inside the layers its math runs in their fused ops, folded into
+    ``base``; called by itself it is ``linear`` with the folded weight.
     """
 
     def __init__(self, in_features: int, out_features: int, rank: int = 16,
@@ -100,8 +102,22 @@ class FlyLoRALinear(nn.Module):
         nn.init.kaiming_uniform_(self.lora_down.weight, a=math.sqrt(5))
         nn.init.zeros_(self.lora_up.weight)
 
-    def forward(self, x):  # pragma: no cover - the fused op is the only compute path
-        raise RuntimeError("FlyLoRALinear is evaluated inside the fused MoE op")
+    def folded(self) -> tuple[torch.Tensor, torch.Tensor]:
+        """(weight, bias) with the low-rank branch folded in, fp32: W + s U D and
+        b + s (U b_D + b_U) (model.py:123-126).  Differentiable in every factor."""
+        with torch.autocast(self.base.weight.device.type, enabled=False):
+            up, s = self.lora_up.weight.float(), self.scaling
+            weight = torch.addmm(self.base.weight.float(), up, self.lora_down.weight.float(), alpha=s)
+            bias = self.base.bias.float() + s * (up @ self.lora_down.bias.float()
+                                                 + self.lora_up.bias.float())
+        return weight, bias
+
+    def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None,
+                activation: str = "none", gamma: float = 0.1) -> torch.Tensor:
+        """``residual + act(base(x) + s lora_up(lora_down(x)))`` of a CUDA tensor, with
+        gradients; the arguments are ``linear``'s."""
+        weight, bias = self.folded()
+        return linear(x, weight, bias, residual=residual, activation=activation, gamma=gamma)
 
 
 class ExpertFFN(nn.Module):
@@ -397,7 +413,9 @@ class FeedForward(_PackedHandleMixin, nn.Module):
 
     Same submodule names (``gate_proj``/``up_proj`` FlyLoRA linears, ``down_proj``), so the
     reference's state_dict loads unchanged; ``forward(x[..., H]) -> out[..., H]``.  It runs
-    on the same grouped tensor-core GEMMs as the MoE experts (one expert, no router).
+    on the same grouped tensor-core GEMMs as the MoE experts (one expert, no router), on
+    weights packed when they change.  A call that wants gradients (float32 or bfloat16), or a
+    ``residual`` to add, runs ``gated_ffn`` on the parameters as they are.
     """
 
     def __init__(self, config):
@@ -429,8 +447,15 @@ class FeedForward(_PackedHandleMixin, nn.Module):
         w["down_w"], w["down_b"] = one(self.down_proj.weight), one(self.down_proj.bias)
         return w
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
         shape = x.shape
+        if residual is not None or (torch.is_grad_enabled() and (
+                x.requires_grad or any(p.requires_grad for p in self._param_list()))):
+            gate_w, gate_b = self.gate_proj.folded()
+            up_w, up_b = self.up_proj.folded()
+            return gated_ffn(x, gate_w, up_w, self.down_proj.weight, gate_b, up_b,
+                             self.down_proj.bias, residual=residual, activation="era",
+                             gamma=self.config.era_gamma)
         packed = self.packed_for(x.device, x.dtype)
         x2d = x.reshape(-1, shape[-1])
         out = _ffn(x2d, packed.id) if _eager(x2d) else torch.ops.vesper_moe.ffn(x2d, packed.id)
