@@ -634,10 +634,19 @@ def test_feed_forward_trains(dtype, wdtype):
     want = torch.autograd.grad(out, [v, *ref64.parameters()], dy.double().cpu())
     limit = 5 * 2.0 ** -8 if BF16 in (dtype, wdtype) else 1e-5
     names = ["x"] + [n for n, _ in m.named_parameters()]
-    for n, a, b in zip(["y"] + names, [y, *grads], [out, *want]):
+    for n, a, b in zip(["y"] + names, [y.detach(), *grads], [out.detach(), *want]):
         assert a.dtype == (dtype if n in ("x", "y") else wdtype)
         rel = float((a.double().cpu() - b).norm() / b.norm())
         assert rel <= limit, (n, rel)
+
+
+def test_feed_forward_f32_is_forward_only():
+    m, x, _ = module_inputs(F32, F32)
+    with pytest.warns(UserWarning, match="no gradient"):
+        y = m(x)
+    assert not y.requires_grad
+    with torch.no_grad():
+        assert torch.equal(y, m(x))
 
 
 def test_feed_forward_without_gradients_is_unchanged():

@@ -414,8 +414,9 @@ class FeedForward(_PackedHandleMixin, nn.Module):
     Same submodule names (``gate_proj``/``up_proj`` FlyLoRA linears, ``down_proj``), so the
     reference's state_dict loads unchanged; ``forward(x[..., H]) -> out[..., H]``.  It runs
     on the same grouped tensor-core GEMMs as the MoE experts (one expert, no router), on
-    weights packed when they change.  A call that wants gradients (float32 or bfloat16), or a
-    ``residual`` to add, runs ``gated_ffn`` on the parameters as they are.
+    weights packed when they change.  A bfloat16 call that wants gradients, or any call with a
+    ``residual`` to add, runs ``gated_ffn`` on the parameters as they are.  As in ``MoELayer``, a
+    plain float32 call is the forward only (with a warning when gradients were wanted).
     """
 
     def __init__(self, config):
@@ -449,13 +450,18 @@ class FeedForward(_PackedHandleMixin, nn.Module):
 
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
         shape = x.shape
-        if residual is not None or (torch.is_grad_enabled() and (
-                x.requires_grad or any(p.requires_grad for p in self._param_list()))):
+        wants_grad = torch.is_grad_enabled() and (
+            x.requires_grad or any(p.requires_grad for p in self._param_list()))
+        if residual is not None or (wants_grad and x.dtype == torch.bfloat16):
             gate_w, gate_b = self.gate_proj.folded()
             up_w, up_b = self.up_proj.folded()
             return gated_ffn(x, gate_w, up_w, self.down_proj.weight, gate_b, up_b,
                              self.down_proj.bias, residual=residual, activation="era",
                              gamma=self.config.era_gamma)
+        if wants_grad and not getattr(self, "_warned_fp32_grad", False):
+            warnings.warn("velvetoptimizer_b200.FeedForward: the backward runs on bfloat16 inputs "
+                          "or with a residual; this float32 forward carries no gradient")
+            self._warned_fp32_grad = True
         packed = self.packed_for(x.device, x.dtype)
         x2d = x.reshape(-1, shape[-1])
         out = _ffn(x2d, packed.id) if _eager(x2d) else torch.ops.vesper_moe.ffn(x2d, packed.id)
