@@ -91,6 +91,14 @@ struct Product {
   const char* what = "";
 };
 
+int product_splits(const Call& c, const Product& p) {
+  const int64_t m_tiles = (p.M + 255) / 256;
+  const int64_t n_tiles = p.epi == kEpiGated ? (p.N + 127) / 128 : (p.N + 255) / 256;
+  return choose_splits(m_tiles * n_tiles * p.groups,
+                       static_cast<int>((p.k0 + 63) / 64 + (p.k1 + 63) / 64), c.o->num_sms / 2,
+                       p.M * n_tiles * 1024 * p.groups);
+}
+
 // One bf16 product on the CTA pairs, split over k where its tiles leave SMs idle.
 int run_product(Call& c, const Product& p) {
   const int64_t m_tiles = (p.M + 255) / 256;
@@ -108,7 +116,7 @@ int run_product(Call& c, const Product& p) {
   const int kb = g.kb0 + g.kb1;
   g.ldp = n_tiles * 256;
   const int64_t part = p.M * g.ldp * 4 * p.groups;
-  g.splits = choose_splits(m_tiles * n_tiles * p.groups, kb, c.o->num_sms / 2, part);
+  g.splits = product_splits(c, p);
   g.kb_per_split = (kb + g.splits - 1) / g.splits;
   g.band = n_tiles < 8 ? static_cast<int>(n_tiles) : 8;
   g.epi = p.e;
@@ -544,6 +552,9 @@ int ffn_backward(Call& c, const vmoe_gated_ffn& d, const FfnPtrs& p) {
   const void* u = p.saved ? p.saved + sv.part : nullptr;
   const void* h = p.saved ? p.saved + 2 * sv.part : nullptr;
   void* any = c.o;  // sizes count every output
+  const int64_t row_blocks = (T + 31) / 32;
+  float* colsum = nullptr;
+  bool summed = false;
   // the activation's side: dg and du
   const bool need_dgu = c.dry || p.dx || gr.gate_w || gr.up_w || gr.gate_b || gr.up_b;
   void *dg = nullptr, *du = nullptr;
@@ -609,6 +620,12 @@ int ffn_backward(Call& c, const vmoe_gated_ffn& d, const FfnPtrs& p) {
       q.k0 = H;
       q.e = e;
       q.what = "dh";
+      // the gate's and the up's bias gradients: column sums in the epilogue, where it runs once
+      if ((c.dry || gr.gate_b || gr.up_b) && product_splits(c, q) == 1) {
+        q.e.colsum_stride = row_blocks * I;
+        q.e.colsum = colsum = c.ws.take<float>(static_cast<size_t>(2 * row_blocks * I) * 4);
+        summed = true;
+      }
       TRY(run_product(c, q));
     }
     const Mat mdg{dg, T, I, sv.ld}, mdu{du, T, I, sv.ld};
@@ -664,6 +681,13 @@ int ffn_backward(Call& c, const vmoe_gated_ffn& d, const FfnPtrs& p) {
       q.what = "dW down";
       TRY(run_product(c, q));
     }
+  }
+  if (summed) {
+    if (c.dry) return VMOE_OK;
+    if (gr.gate_b) TRY(c.ok(launch_colsum_finish(colsum, row_blocks, I, gr.gate_b, gf32, c.s), "dbg"));
+    if (gr.up_b)
+      TRY(c.ok(launch_colsum_finish(colsum + row_blocks * I, row_blocks, I, gr.up_b, gf32, c.s), "dbu"));
+    return VMOE_OK;
   }
   TRY(run_dz(c, dg, sv.ld, nullptr, 0, nullptr, 0, T, I, kActNone, 0.f, c.dry ? any : gr.gate_b,
              gf32));

@@ -36,6 +36,10 @@ struct DenseEpi {
   int64_t ldz = 0;
   int out_f32 = 0;  // out is fp32 (gradients of fp32 parameters)
   int vec = 0;
+  // kEpiGluBwd, optional: column sums of every 32 rows of dg, [ceil(M / 32)][N], and of du
+  // colsum_stride floats further
+  float* colsum = nullptr;
+  int64_t colsum_stride = 0;
 };
 
 // One product C[M, N] = sum over k of A(m, k) B(n, k) on CTA pairs (gemm_dense.cu).
@@ -109,7 +113,7 @@ struct DzArgs {
   int64_t rows_per_block;
 };
 cudaError_t launch_dense_dz(int dtype, const DzArgs& a, cudaStream_t s);
-cudaError_t launch_colsum_finish(const float* partial, int row_blocks, int64_t N, void* out,
+cudaError_t launch_colsum_finish(const float* partial, int64_t row_blocks, int64_t N, void* out,
                                  bool out_f32, cudaStream_t s);
 // rows of bf16 to a buffer whose pitch is a multiple of 8
 cudaError_t launch_pad_copy(const void* src, int64_t lds, int64_t rows, int64_t cols, void* dst,

@@ -7,8 +7,9 @@
 //                                           gelu' = s + z s (1 - s) 2 sqrt(2/pi) (1 + 3 a z^2)
 //   era(z) = gelu_tanh(z) + gamma softplus(z)     (softplus is z above 20, as torch's)
 //   era' = gelu' + gamma s(z)
-// kFast uses the hardware's approximate exponential, logarithm and division (relative error
-// about 2^-21): its results are rounded to bf16.
+// kFast is for results that are rounded to bf16: the hardware's approximate exponential,
+// reciprocal and logarithm, relative errors of 2^-21 or so.  Near 1 the logarithm's error is
+// absolute, 2^-22: softplus below 2^-14 has fewer correct bits than bf16, by less than 2^-22.
 #pragma once
 
 #include <type_traits>
@@ -18,28 +19,40 @@
 
 namespace vmoe {
 
+__device__ __forceinline__ float ex2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float lg2_fast(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kGeluC2 = 1.5957691216057308f;  // 2 sqrt(2 / pi)
+constexpr float kGeluA = 0.044715f;
+
 template <bool kFast>
 __device__ __forceinline__ float act_sigmoid(float t) {
-  if constexpr (kFast) return __fdividef(1.f, 1.f + __expf(-t));
+  if constexpr (kFast) return rcp_fast(1.f + ex2_fast(-kLog2e * t));
   return 1.f / (1.f + expf(-t));
 }
 
-// log(1 + e^z) for z <= 20.  The fast form takes log(1 + e) from the series below e = 2^-6
-// (relative error under 2^-24), where the approximate logarithm near 1 would lose it.
+// s(2q) from z and z^2
 template <bool kFast>
-__device__ __forceinline__ float act_softplus(float z) {
-  if constexpr (!kFast) {
-    return z > 20.f ? z : log1pf(expf(z));
-  } else {
-    const float e = __expf(fminf(z, 20.f));
-    const float series = e * (1.f - e * (0.5f - e * (1.f / 3.f - e * 0.25f)));
-    const float l = e < 0.015625f ? series : __logf(1.f + e);
-    return z > 20.f ? z : l;
-  }
+__device__ __forceinline__ float gelu_gate(float z, float z2) {
+  if constexpr (kFast)
+    return rcp_fast(1.f + ex2_fast(z * fmaf(-kLog2e * kGeluC2 * kGeluA, z2, -kLog2e * kGeluC2)));
+  return 1.f / (1.f + expf(-(z * (kGeluC2 + kGeluC2 * kGeluA * z2))));
 }
-
-constexpr float kGeluC2 = 1.5957691216057308f;  // 2 sqrt(2 / pi)
-constexpr float kGeluA = 0.044715f;
 
 template <bool kFast, int ACT>
 __device__ __forceinline__ float act_value(float z, float gamma) {
@@ -48,9 +61,15 @@ __device__ __forceinline__ float act_value(float z, float gamma) {
   } else if constexpr (ACT == kActSilu) {
     return z * act_sigmoid<kFast>(z);
   } else if constexpr (ACT == kActGeluTanh || ACT == kActEra) {
-    const float g = z * act_sigmoid<kFast>(kGeluC2 * (z + kGeluA * z * z * z));
-    if constexpr (ACT == kActEra) return g + gamma * act_softplus<kFast>(z);
-    return g;
+    const float g = z * gelu_gate<kFast>(z, z * z);
+    if constexpr (ACT == kActGeluTanh) {
+      return g;
+    } else if constexpr (kFast) {
+      const float sp = kLn2 * lg2_fast(1.f + ex2_fast(kLog2e * fminf(z, 20.f)));
+      return fmaf(gamma, z > 20.f ? z : sp, g);
+    } else {
+      return g + gamma * (z > 20.f ? z : log1pf(expf(z)));
+    }
   } else {
     return z;
   }
@@ -65,16 +84,23 @@ __device__ __forceinline__ void act_grad(float z, float gamma, float& a, float& 
   } else if constexpr (ACT == kActSilu) {
     const float s = act_sigmoid<kFast>(z);
     a = z * s;
-    d = s * (1.f + z * (1.f - s));
+    d = fmaf(a, 1.f - s, s);
   } else if constexpr (ACT == kActGeluTanh || ACT == kActEra) {
-    const float s = act_sigmoid<kFast>(kGeluC2 * (z + kGeluA * z * z * z));
+    // far out s (1 - s) is 0: the bound keeps 0 * z^2 from becoming 0 * infinity
+    const float z2 = fminf(z * z, 1e30f);
+    const float s = gelu_gate<kFast>(z, z2);
     a = z * s;
-    // s (1 - s) is 0 in fp32 beyond |z| = 20; the clamp keeps 0 * z^2 from overflowing to NaN
-    const float c = fminf(fmaxf(z, -20.f), 20.f);
-    d = s + c * s * (1.f - s) * kGeluC2 * (1.f + 3.f * kGeluA * c * c);
+    d = fmaf(a * (1.f - s), fmaf(3.f * kGeluA * kGeluC2, z2, kGeluC2), s);
     if constexpr (ACT == kActEra) {
-      a += gamma * act_softplus<kFast>(z);
-      d += gamma * (z > 20.f ? 1.f : act_sigmoid<kFast>(z));
+      if constexpr (kFast) {  // e^z / (1 + e^z) is 1 in fp32 from 20 on
+        const float e = ex2_fast(kLog2e * fminf(z, 20.f));
+        const float sp = kLn2 * lg2_fast(1.f + e);
+        a = fmaf(gamma, z > 20.f ? z : sp, a);
+        d = fmaf(gamma, e * rcp_fast(1.f + e), d);
+      } else {
+        a += gamma * (z > 20.f ? z : log1pf(expf(z)));
+        d += gamma * (z > 20.f ? 1.f : act_sigmoid<false>(z));
+      }
     }
   } else {
     a = z;

@@ -149,13 +149,22 @@ dense_dz_kernel(const DzArgs a, bool vec_dy, bool vec_z, bool vec_dz) {
 
 template <typename T>
 __global__ void __launch_bounds__(256)
-colsum_finish_kernel(const float* partial, int row_blocks, int64_t N, T* out) {
-  const int64_t n = blockIdx.x * 256ll + threadIdx.x;
-  if (n >= N) return;
+colsum_finish_kernel(const float* partial, int64_t row_blocks, int64_t N, T* out) {
+  __shared__ float red[8][32];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int64_t n = blockIdx.x * 32ll + tx;
   float s = 0.f;
+  if (n < N) {
 #pragma unroll 8
-  for (int b = 0; b < row_blocks; ++b) s += partial[b * N + n];
-  out[n] = Elt<T>::from_f(s);
+    for (int64_t b = ty; b < row_blocks; b += 8) s += partial[b * N + n];
+  }
+  red[ty][tx] = s;
+  __syncthreads();
+  if (ty == 0 && n < N) {
+#pragma unroll
+    for (int k = 1; k < 8; ++k) s += red[k][tx];
+    out[n] = Elt<T>::from_f(s);
+  }
 }
 
 __global__ void __launch_bounds__(256)
@@ -210,9 +219,9 @@ cudaError_t launch_dense_dz(int dtype, const DzArgs& a, cudaStream_t s) {
   return cudaGetLastError();
 }
 
-cudaError_t launch_colsum_finish(const float* partial, int row_blocks, int64_t N, void* out,
+cudaError_t launch_colsum_finish(const float* partial, int64_t row_blocks, int64_t N, void* out,
                                  bool out_f32, cudaStream_t s) {
-  const unsigned grid = static_cast<unsigned>((N + 255) / 256);
+  const unsigned grid = static_cast<unsigned>((N + 31) / 32);
   if (out_f32)
     colsum_finish_kernel<float><<<grid, 256, 0, s>>>(partial, row_blocks, N, static_cast<float*>(out));
   else

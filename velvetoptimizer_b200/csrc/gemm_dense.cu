@@ -54,10 +54,15 @@ struct Shared {
   uint64_t done;
   uint32_t tmem_base;
   int abort;
-  alignas(16) float bias[EPI_WARPS][2][32];
+  alignas(16) __nv_bfloat16 bias[EPI_WARPS][2][32];
 };
 
-constexpr size_t SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + sizeof(Shared) + 64;
+// Each epilogue warp turns 32 x 32 blocks between a thread per row (the accumulator's layout)
+// and coalesced rows through 4 KB of its own: two bf16 blocks or one fp32 block.
+constexpr uint32_t BLOCK_BYTES = 32 * 64;
+constexpr uint32_t TURN_BYTES = EPI_WARPS * 2 * BLOCK_BYTES;
+
+constexpr size_t SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + TURN_BYTES + sizeof(Shared) + 16;
 static_assert(SMEM_BYTES <= 232448, "shared memory budget");
 
 __device__ __forceinline__ bool aborted(const Shared* sh) {
@@ -116,20 +121,138 @@ __device__ __forceinline__ Item item_of(const DenseGemm& a, int item) {
 }
 
 // 32 bias values of the columns [col, col + 32) into this warp's shared row (0 past N)
-__device__ __forceinline__ void stage_bias(float* dst, const void* bias, int64_t col, int64_t N,
-                                           int lane) {
+__device__ __forceinline__ void stage_bias(__nv_bfloat16* dst, const void* bias, int64_t col,
+                                           int64_t N, int lane) {
   const auto* b = static_cast<const __nv_bfloat16*>(bias);
-  dst[lane] = (b && col + lane < N) ? __bfloat162float(b[col + lane]) : 0.f;
+  dst[lane] = (b && col + lane < N) ? b[col + lane] : __float2bfloat16_rn(0.f);
 }
 
-__device__ __forceinline__ void add_bias(float (&v)[32], const float* b) {
+__device__ __forceinline__ void add_bias(float (&v)[32], const __nv_bfloat16* b) {
 #pragma unroll
-  for (int j = 0; j < 32; j += 4) {
-    const float4 q = *reinterpret_cast<const float4*>(b + j);
-    v[j] += q.x;
-    v[j + 1] += q.y;
-    v[j + 2] += q.z;
-    v[j + 3] += q.w;
+  for (int j = 0; j < 32; j += 8) {
+    float f[8];
+    load16_to_f(b + j, f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[j + i] += f[i];
+  }
+}
+
+// A 32 x 32 block of a bf16 matrix: where it starts, its pitch, and how much of it is inside.
+struct Block {
+  __nv_bfloat16* p;
+  int64_t ld;
+  int rows, cols;  // valid, at most 32; rows may be <= 0
+  bool vec;
+};
+
+// shared address of 16-byte unit c of row r (bf16: 4 units a row, fp32: 8); the XOR keeps both
+// a unit of every row and whole rows free of bank conflicts
+__device__ __forceinline__ uint4* unit16(uint8_t* buf, int r, int c) {
+  return reinterpret_cast<uint4*>(buf + r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
+}
+__device__ __forceinline__ uint4* unit32(uint8_t* buf, int r, int c) {
+  return reinterpret_cast<uint4*>(buf + r * 128 + ((c ^ (r & 7)) << 4));
+}
+
+// Block -> registers, four lanes per 64-byte row (aligned whole units only; see fetch_odd)
+__device__ __forceinline__ void fetch(const Block& b, uint4 (&v)[4], int lane) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = i * 8 + (lane >> 2), c = lane & 3;
+    v[i] = make_uint4(0, 0, 0, 0);
+    if (b.vec && r < b.rows && c * 8 + 8 <= b.cols)
+      v[i] = __ldg(reinterpret_cast<const uint4*>(b.p + r * b.ld + c * 8));
+  }
+}
+
+// Registers -> shared, then what `fetch` left out: a lane per column
+__device__ __forceinline__ void land(const Block& b, const uint4 (&v)[4], uint8_t* buf, int lane) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) *unit16(buf, i * 8 + (lane >> 2), lane & 3) = v[i];
+  const int whole = b.vec ? b.cols & ~7 : 0;
+  if (whole < b.cols) {
+    __syncwarp();
+    const bool mine = lane >= whole && lane < b.cols;
+#pragma unroll 8
+    for (int r = 0; r < 32; ++r)
+      if (mine && r < b.rows)
+        reinterpret_cast<__nv_bfloat16*>(unit16(buf, r, lane >> 3))[lane & 7] = b.p[r * b.ld + lane];
+  }
+}
+
+__device__ __forceinline__ void get_row(uint8_t* buf, float (&v)[32], int lane) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    load16_to_f(reinterpret_cast<const __nv_bfloat16*>(unit16(buf, lane, c)), v + 8 * c);
+}
+
+__device__ __forceinline__ void put_row(uint8_t* buf, const float (&v)[32], int lane) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    store16_from_f(reinterpret_cast<__nv_bfloat16*>(unit16(buf, lane, c)), v + 8 * c);
+}
+
+// shared -> Block, coalesced
+__device__ __forceinline__ void flush(const Block& b, uint8_t* buf, int lane) {
+  if (b.vec) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = i * 8 + (lane >> 2), c = lane & 3;
+      if (r < b.rows && c * 8 + 8 <= b.cols)
+        *reinterpret_cast<uint4*>(b.p + r * b.ld + c * 8) = *unit16(buf, r, c);
+    }
+  }
+  const int whole = b.vec ? b.cols & ~7 : 0;
+  if (whole < b.cols) {
+    const bool mine = lane >= whole && lane < b.cols;
+#pragma unroll 8
+    for (int r = 0; r < 32; ++r)
+      if (mine && r < b.rows)
+        b.p[r * b.ld + lane] = reinterpret_cast<__nv_bfloat16*>(unit16(buf, r, lane >> 3))[lane & 7];
+  }
+}
+
+// a thread's row of fp32 values -> an fp32 matrix, coalesced (the whole 4 KB buffer)
+__device__ __forceinline__ void flush_f32(float* p, int64_t ld, int rows, int cols, bool vec,
+                                          const float (&v)[32], uint8_t* buf, int lane) {
+#pragma unroll
+  for (int c = 0; c < 8; ++c)
+    *reinterpret_cast<float4*>(unit32(buf, lane, c)) =
+        make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+  __syncwarp();
+  if (vec && cols == 32) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = i * 4 + (lane >> 3), c = lane & 7;
+      if (r < rows) *reinterpret_cast<uint4*>(p + r * ld + c * 4) = *unit32(buf, r, c);
+    }
+  } else {
+#pragma unroll 8
+    for (int r = 0; r < 32; ++r)
+      if (lane < cols && r < rows)
+        p[r * ld + lane] = reinterpret_cast<const float*>(unit32(buf, r, lane >> 2))[lane & 3];
+  }
+}
+
+// Column sums of the block in `buf` (rows past `rows` count nothing): 32 sums to dst[0..cols)
+__device__ __forceinline__ void column_sums(uint8_t* buf, int rows, int cols, float* dst, int lane) {
+  float s[8] = {};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = i * 8 + (lane >> 2);
+    float f[8];
+    load16_to_f(reinterpret_cast<const __nv_bfloat16*>(unit16(buf, r, lane & 3)), f);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s[j] += r < rows ? f[j] : 0.f;
+  }
+#pragma unroll
+  for (int o = 4; o < 32; o <<= 1)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s[j] += __shfl_xor_sync(0xffffffffu, s[j], o);
+  if (lane < 4) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (lane * 8 + j < cols) dst[lane * 8 + j] = s[j];
   }
 }
 
@@ -144,7 +267,7 @@ gemm_dense_kernel(const __grid_constant__ DenseMaps maps, const __grid_constant_
   uint8_t* gbase = smem_raw + (base - raw);
   const uint32_t a_s = base;
   const uint32_t b_s = base + STAGES * HALF_BYTES;
-  Shared* sh = reinterpret_cast<Shared*>(gbase + STAGES * STAGE_BYTES);
+  Shared* sh = reinterpret_cast<Shared*>(gbase + STAGES * STAGE_BYTES + TURN_BYTES);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
@@ -260,13 +383,36 @@ gemm_dense_kernel(const __grid_constant__ DenseMaps maps, const __grid_constant_
     // ---------------- epilogue (warps 2..9, both CTAs) ----------------
     const int q = warp & 3;            // TMEM lane quarter this warp may access
     const int part = (warp - 2) >> 2;  // which half of the columns
-    float(*bias_s)[32] = sh->bias[warp - 2];
+    __nv_bfloat16(*bias_s)[32] = sh->bias[warp - 2];
+    uint8_t* turn_a = gbase + STAGES * STAGE_BYTES + (warp - 2) * 2 * BLOCK_BYTES;
+    uint8_t* turn_b = turn_a + BLOCK_BYTES;
     const DenseEpi& ep = args.epi;
+    constexpr int COLS = EPI == kEpiGated ? 64 : 128;  // columns (features) of a warp's share
     int local = 0;
     for (int item = pair; item < total; item += num_pairs, ++local) {
       const Item w = item_of(args, item);
       const int acc = local & 1;
       const uint32_t aph = (local >> 1) & 1;
+      const int64_t row0 = static_cast<int64_t>(w.m) * PAIR_M + rank * 128 + q * 32;
+      const int rows = static_cast<int>(args.M - row0 < 32 ? args.M - row0 : 32);
+      const int64_t col0 =
+          static_cast<int64_t>(w.n) * (EPI == kEpiGated ? 128 : BN) + part * COLS;
+      // block of the matrix p at column offset c of this warp's share
+      auto block = [&](const void* p, int64_t ld, int c, int flag) {
+        const int64_t left = args.N - col0 - c;
+        return Block{static_cast<__nv_bfloat16*>(const_cast<void*>(p)) + row0 * ld + col0 + c, ld,
+                     rows, static_cast<int>(left < 32 ? (left > 0 ? left : 0) : 32),
+                     (ep.vec & flag) != 0};
+      };
+      // what the epilogue reads besides the accumulator is asked for before the product is done
+      uint4 pre0[4], pre1[4];
+      const bool has_res = !SPLIT && EPI == kEpiLinear && ep.res;
+      if constexpr (!SPLIT && EPI == kEpiGluBwd) {
+        fetch(block(ep.z, ep.ldz, 0, kVecZ), pre0, lane);
+        fetch(block(ep.z2, ep.ldz, 0, kVecZ), pre1, lane);
+      } else if (has_res) {
+        fetch(block(ep.res, ep.ldr, 0, kVecRes), pre0, lane);
+      }
       const bool got = mbar_wait(smem_u32(&sh->tfull[acc]), aph);
       __syncwarp();
       if (!__all_sync(0xffffffffu, got)) {
@@ -274,123 +420,148 @@ gemm_dense_kernel(const __grid_constant__ DenseMaps maps, const __grid_constant_
         break;
       }
       tc_fence_after();
-      const int64_t row = static_cast<int64_t>(w.m) * PAIR_M + rank * 128 + q * 32 + lane;
-      const bool in = row < args.M;
-      const uint32_t t_row = tmem + (static_cast<uint32_t>(q * 32) << 16) + acc * BN;
-      if constexpr (SPLIT) {
-        // fp32 partials in the accumulator's own column order (gated: gate | up per tile)
-        const int split = item % args.splits;
-        float* dst = args.partial +
-                     ((static_cast<int64_t>(split) * args.groups + w.g) * args.M + row) * args.ldp +
-                     static_cast<int64_t>(w.n) * BN;
+      const uint32_t t_row =
+          tmem + (static_cast<uint32_t>(q * 32) << 16) + acc * BN + part * COLS;
+      // the accumulator is free for the next item once this warp's last columns are read
+      auto release = [&](int c) {
+        if (c != COLS - 32) return;
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&sh->tempty[acc]), 0));
+      };
 #pragma unroll 1
-        for (int c = part * 128; c < (part + 1) * 128; c += 32) {
+      for (int c = 0; c < COLS; c += 32) {
+        __syncwarp();
+        if constexpr (SPLIT) {
+          // fp32 partials in the accumulator's own column order (gated: gate | up per tile)
+          const int split = item % args.splits;
+          float* dst = args.partial +
+                       ((static_cast<int64_t>(split) * args.groups + w.g) * args.M + row0) * args.ldp +
+                       static_cast<int64_t>(w.n) * BN + part * COLS + c;
           float v[32];
-          __syncwarp();  // the rows that stored before meet the others again
           tmem_ld32(t_row + c, v);
-          if (in) store_row<32, float>(dst + c, v, 32, true);
-        }
-      } else if constexpr (EPI == kEpiGated) {
-#pragma unroll 1
-        for (int c = part * 64; c < (part + 1) * 64; c += 32) {
-          const int64_t col = static_cast<int64_t>(w.n) * 128 + c;
-          const int64_t valid = args.N - col;
+          if constexpr (EPI == kEpiGated) {
+            flush_f32(dst, args.ldp, rows, 32, true, v, turn_a, lane);
+            tmem_ld32(t_row + 128 + c, v);
+            release(c);
+            __syncwarp();
+            flush_f32(dst + 128, args.ldp, rows, 32, true, v, turn_a, lane);
+          } else {
+            release(c);
+            flush_f32(dst, args.ldp, rows, 32, true, v, turn_a, lane);
+          }
+        } else if constexpr (EPI == kEpiGated) {
           float g[32], u[32];
-          __syncwarp();
           tmem_ld32(t_row + c, g);
           tmem_ld32(t_row + 128 + c, u);
-          if (valid <= 0) continue;  // the same for the whole warp
-          __syncwarp();
-          stage_bias(bias_s[0], ep.bias, col, args.N, lane);
-          stage_bias(bias_s[1], ep.bias2, col, args.N, lane);
-          __syncwarp();
-          add_bias(g, bias_s[0]);
-          add_bias(u, bias_s[1]);
-          if (!in) continue;
+          release(c);
+          const Block h = block(ep.out, ep.ldo, c, kVecOut);
+          if (h.cols == 0) continue;  // the same for the whole warp
+          if (ep.bias || ep.bias2) {
+            stage_bias(bias_s[0], ep.bias, col0 + c, args.N, lane);
+            stage_bias(bias_s[1], ep.bias2, col0 + c, args.N, lane);
+            __syncwarp();
+            add_bias(g, bias_s[0]);
+            add_bias(u, bias_s[1]);
+          }
           if (ep.z) {
-            auto* zp = static_cast<__nv_bfloat16*>(ep.z) + row * ep.ldz + col;
-            auto* zp2 = static_cast<__nv_bfloat16*>(ep.z2) + row * ep.ldz + col;
-            store_row<32>(zp, g, valid, ep.vec & kVecZ);
-            store_row<32>(zp2, u, valid, ep.vec & kVecZ);
+            put_row(turn_a, g, lane);
+            put_row(turn_b, u, lane);
+            __syncwarp();
+            flush(block(ep.z, ep.ldz, c, kVecZ), turn_a, lane);
+            flush(block(ep.z2, ep.ldz, c, kVecZ), turn_b, lane);
+            __syncwarp();
           }
           act_switch(ep.act, [&](auto A) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) g[j] = act_value<true, decltype(A)::value>(g[j], ep.gamma) * u[j];
           });
-          store_row<32>(static_cast<__nv_bfloat16*>(ep.out) + row * ep.ldo + col, g, valid,
-                        ep.vec & kVecOut);
-        }
-      } else if constexpr (EPI == kEpiGluBwd) {
-#pragma unroll 1
-        for (int c = part * 128; c < (part + 1) * 128; c += 32) {
-          const int64_t col = static_cast<int64_t>(w.n) * BN + c;
-          const int64_t valid = args.N - col;
-          float dh[32];
+          put_row(turn_a, g, lane);
           __syncwarp();
+          flush(h, turn_a, lane);
+        } else if constexpr (EPI == kEpiGluBwd) {
+          const Block bg = block(ep.z, ep.ldz, c, kVecZ), bu = block(ep.z2, ep.ldz, c, kVecZ);
+          float dh[32];
           tmem_ld32(t_row + c, dh);
-          if (valid <= 0 || !in) continue;
-          float g[32], u[32];
-          load_row<32>(static_cast<const __nv_bfloat16*>(ep.z) + row * ep.ldz + col, g, valid,
-                       ep.vec & kVecZ);
-          load_row<32>(static_cast<const __nv_bfloat16*>(ep.z2) + row * ep.ldz + col, u, valid,
-                       ep.vec & kVecZ);
+          release(c);
+          if (bg.cols == 0) continue;
+          land(bg, pre0, turn_a, lane);
+          land(bu, pre1, turn_b, lane);
+          __syncwarp();
+          if (c + 32 < COLS) {
+            fetch(block(ep.z, ep.ldz, c + 32, kVecZ), pre0, lane);
+            fetch(block(ep.z2, ep.ldz, c + 32, kVecZ), pre1, lane);
+          }
+          // a unit of 8 columns at a time, g and u replaced by dg and du where they lie: a row
+          // is read and rewritten by its own thread, the others' units meet at the sync
           act_switch(ep.act, [&](auto A) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              float a, d;
-              act_grad<true, decltype(A)::value>(g[j], ep.gamma, a, d);
-              g[j] = dh[j] * u[j] * d;
-              u[j] = dh[j] * a;
+            for (int k = 0; k < 4; ++k) {
+              auto* ug = reinterpret_cast<__nv_bfloat16*>(unit16(turn_a, lane, k));
+              auto* uu = reinterpret_cast<__nv_bfloat16*>(unit16(turn_b, lane, k));
+              float g[8], u[8];
+              load16_to_f(ug, g);
+              load16_to_f(uu, u);
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                float a, d;
+                act_grad<true, decltype(A)::value>(g[j], ep.gamma, a, d);
+                g[j] = dh[8 * k + j] * u[j] * d;
+                u[j] = dh[8 * k + j] * a;
+              }
+              store16_from_f(ug, g);
+              store16_from_f(uu, u);
             }
           });
-          store_row<32>(static_cast<__nv_bfloat16*>(ep.out) + row * ep.ldo + col, g, valid,
-                        ep.vec & kVecOut);
-          store_row<32>(static_cast<__nv_bfloat16*>(ep.out2) + row * ep.ldo + col, u, valid,
-                        ep.vec & kVecOut);
-        }
-      } else {
-        void* out = w.g ? ep.out2 : ep.out;
-#pragma unroll 1
-        for (int c = part * 128; c < (part + 1) * 128; c += 32) {
-          const int64_t col = static_cast<int64_t>(w.n) * BN + c;
-          const int64_t valid = args.N - col;
-          float v[32];
           __syncwarp();
-          tmem_ld32(t_row + c, v);
-          if (valid <= 0) continue;
-          if (ep.bias) {
-            __syncwarp();
-            stage_bias(bias_s[0], ep.bias, col, args.N, lane);
-            __syncwarp();
-            add_bias(v, bias_s[0]);
+          flush(block(ep.out, ep.ldo, c, kVecOut), turn_a, lane);
+          flush(block(ep.out2, ep.ldo, c, kVecOut), turn_b, lane);
+          if (ep.colsum) {
+            float* dst = ep.colsum + row0 / 32 * args.N + col0 + c;
+            if (rows > 0) {
+              column_sums(turn_a, rows, bg.cols, dst, lane);
+              column_sums(turn_b, rows, bg.cols, dst + ep.colsum_stride, lane);
+            }
           }
-          if (!in) continue;
-          if (ep.z)
-            store_row<32>(static_cast<__nv_bfloat16*>(ep.z) + row * ep.ldz + col, v, valid,
-                          ep.vec & kVecZ);
+        } else {
+          float v[32];
+          tmem_ld32(t_row + c, v);
+          release(c);
+          const Block out = block(w.g ? ep.out2 : ep.out, ep.ldo, c, kVecOut);
+          if (out.cols == 0) continue;
+          if (has_res) land(block(ep.res, ep.ldr, c, kVecRes), pre0, turn_a, lane);
+          if (ep.bias) stage_bias(bias_s[0], ep.bias, col0 + c, args.N, lane);
+          __syncwarp();
+          if (has_res && c + 32 < COLS) fetch(block(ep.res, ep.ldr, c + 32, kVecRes), pre0, lane);
+          if (ep.bias) add_bias(v, bias_s[0]);
+          if (ep.z) {
+            put_row(turn_b, v, lane);
+            __syncwarp();
+            flush(block(ep.z, ep.ldz, c, kVecZ), turn_b, lane);
+          }
           if (ep.act != kActNone) {
             act_switch(ep.act, [&](auto A) {
 #pragma unroll
               for (int j = 0; j < 32; ++j) v[j] = act_value<true, decltype(A)::value>(v[j], ep.gamma);
             });
           }
-          if (ep.res) {
+          if (has_res) {
             float r[32];
-            load_row<32>(static_cast<const __nv_bfloat16*>(ep.res) + row * ep.ldr + col, r, valid,
-                         ep.vec & kVecRes);
+            get_row(turn_a, r, lane);
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] += r[j];
           }
-          if (ep.out_f32)
-            store_row<32>(static_cast<float*>(out) + row * ep.ldo + col, v, valid, ep.vec & kVecOut);
-          else
-            store_row<32>(static_cast<__nv_bfloat16*>(out) + row * ep.ldo + col, v, valid,
-                          ep.vec & kVecOut);
+          if (ep.out_f32) {
+            __syncwarp();
+            flush_f32(static_cast<float*>(w.g ? ep.out2 : ep.out) + row0 * ep.ldo + col0 + c, ep.ldo,
+                      rows, out.cols, out.vec, v, turn_a, lane);
+          } else {
+            put_row(turn_a, v, lane);
+            __syncwarp();
+            flush(out, turn_a, lane);
+          }
         }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&sh->tempty[acc]), 0));
     }
   }
 
