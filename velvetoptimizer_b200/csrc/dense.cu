@@ -16,9 +16,14 @@ constexpr int kStatusWords = 256;
 __device__ int g_ops_status[kStatusWords];
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-bool vec_ok(const void* p, int64_t ld, size_t elt) {
+bool pitch16(const void* p, int64_t ld, size_t elt) {
   return ((reinterpret_cast<uintptr_t>(p) | static_cast<uintptr_t>(ld * static_cast<int64_t>(elt))) &
           15u) == 0;
+}
+
+// rows of n elements in whole 16-byte units (DenseEpi::vec)
+bool vec_ok(const void* p, int64_t ld, int64_t n, size_t elt) {
+  return pitch16(p, ld, elt) && n * static_cast<int64_t>(elt) % 16 == 0;
 }
 
 // A bf16 matrix [rows, cols] as the TMA reads it.
@@ -325,8 +330,8 @@ int linear_forward(Call& c, const vmoe_linear& d, const LinearPtrs& p) {
   e.ldo = N;
   e.z = p.z;
   e.ldz = N;
-  e.vec = (vec_ok(p.y, N, elt) ? kVecOut : 0) | (vec_ok(p.r, d.ldr, elt) ? kVecRes : 0) |
-          (vec_ok(p.z, N, elt) ? kVecZ : 0);
+  e.vec = (vec_ok(p.y, N, N, elt) ? kVecOut : 0) | (vec_ok(p.r, d.ldr, N, elt) ? kVecRes : 0) |
+          (vec_ok(p.z, N, N, elt) ? kVecZ : 0);
   if (d.dtype == VMOE_F32) {
     const SimtPart part{static_cast<const float*>(p.x), static_cast<const float*>(p.w), d.ldx, 1,
                         d.ldw, 1, K};
@@ -343,7 +348,7 @@ int linear_forward(Call& c, const vmoe_linear& d, const LinearPtrs& p) {
     g.N = N;
     g.K = K;
     g.epi = e;
-    g.vec_in = K % 8 == 0 && vec_ok(p.x, d.ldx, 2) && vec_ok(p.w, d.ldw, 2);
+    g.vec_in = K % 8 == 0 && pitch16(p.x, d.ldx, 2) && pitch16(p.w, d.ldw, 2);
     return c.ok(launch_dense_small(kEpiLinear, g, c.s), "linear");
   }
   Product q;
@@ -379,11 +384,11 @@ int linear_backward(Call& c, const vmoe_linear& d, const LinearPtrs& p) {
   DenseEpi ex, ew;
   ex.out = p.dx;
   ex.ldo = K;
-  ex.vec = vec_ok(p.dx, K, elt) ? kVecOut : 0;
+  ex.vec = vec_ok(p.dx, K, K, elt) ? kVecOut : 0;
   ew.out = p.dw;
   ew.ldo = K;
   ew.out_f32 = gf32;
-  ew.vec = vec_ok(p.dw, K, gelt) ? kVecOut : 0;
+  ew.vec = vec_ok(p.dw, K, K, gelt) ? kVecOut : 0;
   if (f32) {
     const auto* fz = static_cast<const float*>(dz);
     const auto* fx = static_cast<const float*>(p.x);
@@ -477,7 +482,7 @@ int ffn_forward(Call& c, const vmoe_gated_ffn& d, const FfnPtrs& p) {
   e2.ldr = d.ldr;
   e2.out = p.y;
   e2.ldo = H;
-  e2.vec = (vec_ok(p.y, H, elt) ? kVecOut : 0) | (vec_ok(p.r, d.ldr, elt) ? kVecRes : 0);
+  e2.vec = (vec_ok(p.y, H, H, elt) ? kVecOut : 0) | (vec_ok(p.r, d.ldr, H, elt) ? kVecRes : 0);
   if (d.dtype == VMOE_F32) {
     const auto* x = static_cast<const float*>(p.x);
     const SimtPart gu[2] = {{x, static_cast<const float*>(p.w.gate_w), d.ldx, 1, H, 1, H},
@@ -499,7 +504,7 @@ int ffn_forward(Call& c, const vmoe_gated_ffn& d, const FfnPtrs& p) {
     g.N = I;
     g.K = H;
     g.epi = e1;
-    g.vec_in = H % 8 == 0 && vec_ok(p.x, d.ldx, 2) && aligned16(p.w.gate_w) && aligned16(p.w.up_w);
+    g.vec_in = H % 8 == 0 && pitch16(p.x, d.ldx, 2) && aligned16(p.w.gate_w) && aligned16(p.w.up_w);
     TRY(c.ok(launch_dense_small(kEpiGated, g, c.s), "gate|up"));
     SmallGemm q{};
     q.x = h;
@@ -582,7 +587,7 @@ int ffn_backward(Call& c, const vmoe_gated_ffn& d, const FfnPtrs& p) {
     q.out = out;
     q.ldo = ld;
     q.out_f32 = grad && gf32;
-    q.vec = vec_ok(out, ld, grad ? gelt : elt) ? kVecOut : 0;
+    q.vec = vec_ok(out, ld, ld, grad ? gelt : elt) ? kVecOut : 0;
     return q;
   };
   if (f32) {
@@ -660,7 +665,7 @@ int ffn_backward(Call& c, const vmoe_gated_ffn& d, const FfnPtrs& p) {
       q.e = plain(both || gr.gate_w ? gr.gate_w : gr.up_w, H, true);
       if (both) {
         q.e.out2 = gr.up_w;
-        if (!vec_ok(gr.up_w, H, gelt)) q.e.vec = 0;
+        if (!vec_ok(gr.up_w, H, H, gelt)) q.e.vec = 0;
       }
       q.what = "dW gate|up";
       TRY(run_product(c, q));

@@ -18,7 +18,9 @@ enum Act : int { kActNone = 0, kActRelu = 1, kActSilu = 2, kActGeluTanh = 3, kAc
 //   kEpiGluBwd  acc = dh, g and u read: out = dh * u * act'(g), out2 = dh * act(g)
 enum EpiKind : int { kEpiLinear = 0, kEpiGated = 1, kEpiGluBwd = 2 };
 
-// `vec` bits: the buffer's base and row pitch allow 16-byte accesses
+// `vec` bits: every row of the buffer is whole aligned 16-byte units: base and pitch are
+// multiples of 16 bytes, and so are the columns, or what follows them up to the pitch is the
+// buffer's own padding (it may be read and overwritten)
 enum : int { kVecOut = 1, kVecRes = 2, kVecZ = 4 };
 
 struct DenseEpi {

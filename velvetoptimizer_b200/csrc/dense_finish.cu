@@ -45,11 +45,12 @@ dense_finish_kernel(const DenseGemm g) {
       load_row<V>(static_cast<const T*>(ep.z) + row * ep.ldz + col, gg, valid, ep.vec & kVecZ);
       load_row<V>(static_cast<const T*>(ep.z2) + row * ep.ldz + col, u, valid, ep.vec & kVecZ);
       act_switch(ep.act, [&](auto A) {
+        float d[V];
+        act_grads<kFast, decltype(A)::value>(gg, d, ep.gamma);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          float a, d;
-          act_grad<kFast, decltype(A)::value>(gg[j], ep.gamma, a, d);
-          gg[j] = v[j] * u[j] * d;
+          const float a = gg[j];
+          gg[j] = v[j] * u[j] * d[j];
           u[j] = v[j] * a;
         }
       });
@@ -75,15 +76,13 @@ dense_finish_kernel(const DenseGemm g) {
         store_row<V>(static_cast<T*>(ep.z2) + row * ep.ldz + col, u, valid, ep.vec & kVecZ);
       }
       act_switch(ep.act, [&](auto A) {
+        act_values<kFast, decltype(A)::value>(v, ep.gamma);
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = act_value<kFast, decltype(A)::value>(v[j], ep.gamma) * u[j];
+        for (int j = 0; j < V; ++j) v[j] *= u[j];
       });
     } else {
       if (ep.z) store_row<V>(static_cast<T*>(ep.z) + row * ep.ldz + col, v, valid, ep.vec & kVecZ);
-      act_switch(ep.act, [&](auto A) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = act_value<kFast, decltype(A)::value>(v[j], ep.gamma);
-      });
+      act_switch(ep.act, [&](auto A) { act_values<kFast, decltype(A)::value>(v, ep.gamma); });
       if (ep.res) {
         float r[V];
         load_row<V>(static_cast<const T*>(ep.res) + row * ep.ldr + col, r, valid, ep.vec & kVecRes);
@@ -119,12 +118,10 @@ dense_dz_kernel(const DzArgs a, bool vec_dy, bool vec_z, bool vec_dz) {
         float z[W];
         load_row<W>(static_cast<const T*>(a.z) + r * a.ldz + col, z, valid, vec_z);
         act_switch(a.act, [&](auto A) {
+          float d[W];
+          act_grads<kFast, decltype(A)::value>(z, d, a.gamma);
 #pragma unroll
-          for (int j = 0; j < W; ++j) {
-            float y, d;
-            act_grad<kFast, decltype(A)::value>(z[j], a.gamma, y, d);
-            v[j] *= d;
-          }
+          for (int j = 0; j < W; ++j) v[j] *= d[j];
         });
       }
       if (a.dz)

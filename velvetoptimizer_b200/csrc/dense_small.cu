@@ -12,6 +12,8 @@
 // flight.  A block owns 16 weight rows, its 8 warps take every eighth chunk and add their
 // sums through shared memory in warp order.  The gated form takes 8 gate rows and 8 up rows
 // of the same features as the 16, so one thread ends up with both.
+#include <stdlib.h>
+
 #include "common.cuh"
 #include "dense.h"
 #include "dense_act.cuh"
@@ -19,7 +21,6 @@
 namespace vmoe {
 namespace {
 
-constexpr int WARPS = 8;
 constexpr int UNROLL = 4;
 
 __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
@@ -48,12 +49,12 @@ __device__ __forceinline__ uint4 load8(const __nv_bfloat16* row, int64_t k, int6
   return v;
 }
 
-template <int EPI, bool VEC, int NT>
+template <int EPI, bool VEC, int NT, int WARPS>
 __global__ void __launch_bounds__(32 * WARPS)
 dense_small_kernel(const SmallGemm g) {
   constexpr bool kGate = EPI == kEpiGated;
   constexpr int ROWS = kGate ? 8 : 16;  // output features per block
-  __shared__ float red[WARPS][NT][32][4];
+  __shared__ float4 red[WARPS][NT][32];
   __shared__ float sum[NT][16][8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int gid = lane >> 2, tig = lane & 3;
@@ -97,14 +98,13 @@ dense_small_kernel(const SmallGemm g) {
   }
 #pragma unroll
   for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) red[warp][n][lane][i] = acc[n][i];
+    red[warp][n][lane] = make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
   __syncthreads();
   if (threadIdx.x < NT * 128) {
     const int n = threadIdx.x >> 7, l = (threadIdx.x >> 2) & 31, i = threadIdx.x & 3;
     float s = 0.f;
 #pragma unroll
-    for (int k = 0; k < WARPS; ++k) s += red[k][n][l][i];
+    for (int k = 0; k < WARPS; ++k) s += reinterpret_cast<const float*>(&red[k][n][l])[i];
     sum[n][(l >> 2) + 8 * (i >> 1)][(l & 3) * 2 + (i & 1)] = s;
   }
   __syncthreads();
@@ -124,20 +124,29 @@ dense_small_kernel(const SmallGemm g) {
       zp[t * ep.ldz + col] = __float2bfloat16_rn(z);
       static_cast<__nv_bfloat16*>(ep.z2)[t * ep.ldz + col] = __float2bfloat16_rn(up);
     }
-    act_switch(ep.act, [&](auto A) { z = act_value<true, decltype(A)::value>(z, ep.gamma) * up; });
+    act_switch(ep.act, [&](auto A) { z = act_value2<decltype(A)::value>(both(z), ep.gamma).x * up; });
   } else {
     if (zp) zp[t * ep.ldz + col] = __float2bfloat16_rn(z);
-    act_switch(ep.act, [&](auto A) { z = act_value<true, decltype(A)::value>(z, ep.gamma); });
+    act_switch(ep.act, [&](auto A) { z = act_value2<decltype(A)::value>(both(z), ep.gamma).x; });
     if (ep.res) z += __bfloat162float(static_cast<const __nv_bfloat16*>(ep.res)[t * ep.ldr + col]);
   }
   out[t * ep.ldo + col] = __float2bfloat16_rn(z);
 }
 
+template <int EPI, bool VEC, int NT>
+cudaError_t launch_warps(const SmallGemm& g, unsigned blocks, cudaStream_t s) {
+  static const int forced = getenv("SMALL_WARPS") ? atoi(getenv("SMALL_WARPS")) : 0;
+  int w = forced ? forced : 8;
+  if (w >= 32)
+    return launch_kernel(dense_small_kernel<EPI, VEC, NT, 32>, dim3(blocks), dim3(1024), 0, s, g);
+  if (w >= 16)
+    return launch_kernel(dense_small_kernel<EPI, VEC, NT, 16>, dim3(blocks), dim3(512), 0, s, g);
+  return launch_kernel(dense_small_kernel<EPI, VEC, NT, 8>, dim3(blocks), dim3(256), 0, s, g);
+}
+
 template <int EPI, bool VEC>
 cudaError_t launch_nt(const SmallGemm& g, unsigned blocks, cudaStream_t s) {
-  if (g.T <= 8)
-    return launch_kernel(dense_small_kernel<EPI, VEC, 1>, dim3(blocks), dim3(32 * WARPS), 0, s, g);
-  return launch_kernel(dense_small_kernel<EPI, VEC, 2>, dim3(blocks), dim3(32 * WARPS), 0, s, g);
+  return g.T <= 8 ? launch_warps<EPI, VEC, 1>(g, blocks, s) : launch_warps<EPI, VEC, 2>(g, blocks, s);
 }
 
 }  // namespace

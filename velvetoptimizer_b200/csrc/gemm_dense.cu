@@ -90,6 +90,13 @@ __device__ __forceinline__ uint64_t op_desc(uint32_t addr, int k) {
   return umma_desc_sw128(addr + k * 32);
 }
 
+// Arrive on another CTA's barrier to say that TMEM has been read.  Only the TMEM reads are
+// ordered (tcgen05 fences on both sides); a release at cluster scope would also wait for every
+// global store of the epilogue so far.
+__device__ __forceinline__ void arrive_remote(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
 struct Item {
   int g, m, n, kb, ke;
 };
@@ -138,11 +145,13 @@ __device__ __forceinline__ void add_bias(float (&v)[32], const __nv_bfloat16* b)
 }
 
 // A 32 x 32 block of a bf16 matrix: where it starts, its pitch, and how much of it is inside.
+// With `vec` its rows are whole aligned 16-byte units (cols a multiple of 8).
 struct Block {
   __nv_bfloat16* p;
   int64_t ld;
   int rows, cols;  // valid, at most 32; rows may be <= 0
   bool vec;
+  __device__ __forceinline__ bool whole() const { return vec && rows == 32 && cols == 32; }
 };
 
 // shared address of 16-byte unit c of row r (bf16: 4 units a row, fp32: 8); the XOR keeps both
@@ -154,29 +163,53 @@ __device__ __forceinline__ uint4* unit32(uint8_t* buf, int r, int c) {
   return reinterpret_cast<uint4*>(buf + r * 128 + ((c ^ (r & 7)) << 4));
 }
 
-// Block -> registers, four lanes per 64-byte row (aligned whole units only; see fetch_odd)
+// Block -> registers: units with four lanes per row, or single elements with a lane per column
+// and two rows per register
 __device__ __forceinline__ void fetch(const Block& b, uint4 (&v)[4], int lane) {
+  if (b.vec) {
+    const __nv_bfloat16* p = b.p + (lane >> 2) * b.ld + (lane & 3) * 8;
+    if (b.whole()) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i, p += 8 * b.ld) v[i] = __ldg(reinterpret_cast<const uint4*>(p));
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i, p += 8 * b.ld) {
+      v[i] = make_uint4(0, 0, 0, 0);
+      if (i * 8 + (lane >> 2) < b.rows && (lane & 3) * 8 < b.cols)
+        v[i] = __ldg(reinterpret_cast<const uint4*>(p));
+    }
+    return;
+  }
+  const auto* p = reinterpret_cast<const unsigned short*>(b.p) + lane;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int r = i * 8 + (lane >> 2), c = lane & 3;
-    v[i] = make_uint4(0, 0, 0, 0);
-    if (b.vec && r < b.rows && c * 8 + 8 <= b.cols)
-      v[i] = __ldg(reinterpret_cast<const uint4*>(b.p + r * b.ld + c * 8));
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j, p += 2 * b.ld) {
+      const int r = 8 * i + 2 * j;
+      const uint32_t lo = lane < b.cols && r < b.rows ? __ldg(p) : 0u;
+      const uint32_t hi = lane < b.cols && r + 1 < b.rows ? __ldg(p + b.ld) : 0u;
+      w[j] = lo | hi << 16;
+    }
+    v[i] = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 
-// Registers -> shared, then what `fetch` left out: a lane per column
+// registers -> shared
 __device__ __forceinline__ void land(const Block& b, const uint4 (&v)[4], uint8_t* buf, int lane) {
+  if (b.vec) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) *unit16(buf, i * 8 + (lane >> 2), lane & 3) = v[i];
-  const int whole = b.vec ? b.cols & ~7 : 0;
-  if (whole < b.cols) {
-    __syncwarp();
-    const bool mine = lane >= whole && lane < b.cols;
-#pragma unroll 8
-    for (int r = 0; r < 32; ++r)
-      if (mine && r < b.rows)
-        reinterpret_cast<__nv_bfloat16*>(unit16(buf, r, lane >> 3))[lane & 7] = b.p[r * b.ld + lane];
+    for (int i = 0; i < 4; ++i) *unit16(buf, i * 8 + (lane >> 2), lane & 3) = v[i];
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      reinterpret_cast<unsigned short*>(unit16(buf, 8 * i + j, lane >> 3))[lane & 7] =
+          static_cast<unsigned short>(w[j >> 1] >> (16 * (j & 1)));
   }
 }
 
@@ -195,21 +228,24 @@ __device__ __forceinline__ void put_row(uint8_t* buf, const float (&v)[32], int 
 // shared -> Block, coalesced
 __device__ __forceinline__ void flush(const Block& b, uint8_t* buf, int lane) {
   if (b.vec) {
+    __nv_bfloat16* p = b.p + (lane >> 2) * b.ld + (lane & 3) * 8;
+    if (b.whole()) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = i * 8 + (lane >> 2), c = lane & 3;
-      if (r < b.rows && c * 8 + 8 <= b.cols)
-        *reinterpret_cast<uint4*>(b.p + r * b.ld + c * 8) = *unit16(buf, r, c);
+      for (int i = 0; i < 4; ++i, p += 8 * b.ld)
+        *reinterpret_cast<uint4*>(p) = *unit16(buf, i * 8 + (lane >> 2), lane & 3);
+      return;
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i, p += 8 * b.ld)
+      if (i * 8 + (lane >> 2) < b.rows && (lane & 3) * 8 < b.cols)
+        *reinterpret_cast<uint4*>(p) = *unit16(buf, i * 8 + (lane >> 2), lane & 3);
+    return;
   }
-  const int whole = b.vec ? b.cols & ~7 : 0;
-  if (whole < b.cols) {
-    const bool mine = lane >= whole && lane < b.cols;
+  __nv_bfloat16* p = b.p + lane;
 #pragma unroll 8
-    for (int r = 0; r < 32; ++r)
-      if (mine && r < b.rows)
-        b.p[r * b.ld + lane] = reinterpret_cast<__nv_bfloat16*>(unit16(buf, r, lane >> 3))[lane & 7];
-  }
+  for (int r = 0; r < 32; ++r, p += b.ld)
+    if (lane < b.cols && r < b.rows)
+      *p = reinterpret_cast<__nv_bfloat16*>(unit16(buf, r, lane >> 3))[lane & 7];
 }
 
 // a thread's row of fp32 values -> an fp32 matrix, coalesced (the whole 4 KB buffer)
@@ -234,26 +270,29 @@ __device__ __forceinline__ void flush_f32(float* p, int64_t ld, int rows, int co
   }
 }
 
-// Column sums of the block in `buf` (rows past `rows` count nothing): 32 sums to dst[0..cols)
-__device__ __forceinline__ void column_sums(uint8_t* buf, int rows, int cols, float* dst, int lane) {
+// Column sums of the 32 x 32 block in `buf` (rows outside hold zeros) to dst[0..cols): a lane
+// adds 4 rows of its 8 columns, then the 8 lanes of the same columns halve their columns with
+// a partner's three times.
+__device__ __forceinline__ void column_sums(uint8_t* buf, int cols, float* dst, int lane) {
   float s[8] = {};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int r = i * 8 + (lane >> 2);
     float f[8];
-    load16_to_f(reinterpret_cast<const __nv_bfloat16*>(unit16(buf, r, lane & 3)), f);
+    load16_to_f(reinterpret_cast<const __nv_bfloat16*>(unit16(buf, i * 8 + (lane >> 2), lane & 3)), f);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) s[j] += r < rows ? f[j] : 0.f;
+    for (int j = 0; j < 8; ++j) s[j] += f[j];
   }
 #pragma unroll
-  for (int o = 4; o < 32; o <<= 1)
+  for (int o = 4; o >= 1; o >>= 1) {
+    const bool upper = (lane & (4 * o)) != 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) s[j] += __shfl_xor_sync(0xffffffffu, s[j], o);
-  if (lane < 4) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (lane * 8 + j < cols) dst[lane * 8 + j] = s[j];
+    for (int j = 0; j < o; ++j) {
+      const float other = __shfl_xor_sync(0xffffffffu, upper ? s[j] : s[j + o], 4 * o);
+      s[j] = (upper ? s[j + o] : s[j]) + other;
+    }
   }
+  const int col = (lane & 3) * 8 + ((lane >> 4) & 1) * 4 + ((lane >> 3) & 1) * 2 + ((lane >> 2) & 1);
+  if (col < cols) dst[col] = s[0];
 }
 
 template <bool A_MN, bool B_MN, int EPI, bool SPLIT>
@@ -400,9 +439,10 @@ gemm_dense_kernel(const __grid_constant__ DenseMaps maps, const __grid_constant_
       // block of the matrix p at column offset c of this warp's share
       auto block = [&](const void* p, int64_t ld, int c, int flag) {
         const int64_t left = args.N - col0 - c;
+        const bool vec = (ep.vec & flag) != 0;
+        const int cols = static_cast<int>(left < 32 ? (left > 0 ? left : 0) : 32);
         return Block{static_cast<__nv_bfloat16*>(const_cast<void*>(p)) + row0 * ld + col0 + c, ld,
-                     rows, static_cast<int>(left < 32 ? (left > 0 ? left : 0) : 32),
-                     (ep.vec & flag) != 0};
+                     rows, vec ? (cols + 7) & ~7 : cols, vec};
       };
       // what the epilogue reads besides the accumulator is asked for before the product is done
       uint4 pre0[4], pre1[4];
@@ -427,7 +467,7 @@ gemm_dense_kernel(const __grid_constant__ DenseMaps maps, const __grid_constant_
         if (c != COLS - 32) return;
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&sh->tempty[acc]), 0));
+        if (lane == 0) arrive_remote(mapa_shared(smem_u32(&sh->tempty[acc]), 0));
       };
 #pragma unroll 1
       for (int c = 0; c < COLS; c += 32) {
@@ -473,8 +513,9 @@ gemm_dense_kernel(const __grid_constant__ DenseMaps maps, const __grid_constant_
             __syncwarp();
           }
           act_switch(ep.act, [&](auto A) {
+            act_values<true, decltype(A)::value>(g, ep.gamma);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) g[j] = act_value<true, decltype(A)::value>(g[j], ep.gamma) * u[j];
+            for (int j = 0; j < 32; ++j) g[j] *= u[j];
           });
           put_row(turn_a, g, lane);
           __syncwarp();
@@ -503,11 +544,15 @@ gemm_dense_kernel(const __grid_constant__ DenseMaps maps, const __grid_constant_
               load16_to_f(ug, g);
               load16_to_f(uu, u);
 #pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                float a, d;
-                act_grad<true, decltype(A)::value>(g[j], ep.gamma, a, d);
-                g[j] = dh[8 * k + j] * u[j] * d;
-                u[j] = dh[8 * k + j] * a;
+              for (int j = 0; j < 8; j += 2) {
+                const float2 p = make_float2(dh[8 * k + j], dh[8 * k + j + 1]);
+                float2 a, d;
+                act_grad2<decltype(A)::value>(make_float2(g[j], g[j + 1]), ep.gamma, a, d);
+                const float2 dg = mul2(mul2(p, make_float2(u[j], u[j + 1])), d), du = mul2(p, a);
+                g[j] = dg.x;
+                g[j + 1] = dg.y;
+                u[j] = du.x;
+                u[j + 1] = du.y;
               }
               store16_from_f(ug, g);
               store16_from_f(uu, u);
@@ -518,9 +563,10 @@ gemm_dense_kernel(const __grid_constant__ DenseMaps maps, const __grid_constant_
           flush(block(ep.out2, ep.ldo, c, kVecOut), turn_b, lane);
           if (ep.colsum) {
             float* dst = ep.colsum + row0 / 32 * args.N + col0 + c;
+            const int cols = static_cast<int>(min(args.N - col0 - c, static_cast<int64_t>(32)));
             if (rows > 0) {
-              column_sums(turn_a, rows, bg.cols, dst, lane);
-              column_sums(turn_b, rows, bg.cols, dst + ep.colsum_stride, lane);
+              column_sums(turn_a, cols, dst, lane);
+              column_sums(turn_b, cols, dst + ep.colsum_stride, lane);
             }
           }
         } else {
@@ -540,10 +586,8 @@ gemm_dense_kernel(const __grid_constant__ DenseMaps maps, const __grid_constant_
             flush(block(ep.z, ep.ldz, c, kVecZ), turn_b, lane);
           }
           if (ep.act != kActNone) {
-            act_switch(ep.act, [&](auto A) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = act_value<true, decltype(A)::value>(v[j], ep.gamma);
-            });
+            act_switch(ep.act,
+                       [&](auto A) { act_values<true, decltype(A)::value>(v, ep.gamma); });
           }
           if (has_res) {
             float r[32];
