@@ -57,7 +57,7 @@ def run_linear(T, K, N, act="none", dtype=BF16, bias=True, residual=True, seed=0
 
 
 # one token, the small-batch form's edges (8, 9, 16 | 17), tiles and their edges (256, 257)
-@pytest.mark.parametrize("T", [1, 2, 8, 9, 16, 17, 63, 256, 257])
+@pytest.mark.parametrize("T", [1, 2, 8, 9, 16, 17, 63, 128, 129, 256, 257])
 @pytest.mark.parametrize("K,N", [(64, 64), (40, 24), (136, 264)])
 def test_linear_sizes(T, K, N):
     run_linear(T, K, N, act="silu", seed=T + K)
@@ -92,7 +92,8 @@ def test_linear_parameters_of_another_type(T, dtype, wdtype):
 
 
 # k divided over SMs (few tiles, long sums) and many tiles
-@pytest.mark.parametrize("T,K,N", [(64, 4096, 256), (40, 2048, 520), (2100, 72, 136),
+@pytest.mark.parametrize("T,K,N", [(64, 4096, 256), (40, 2048, 520), (33, 1000, 1100), (17, 130, 2500),
+                                   (128, 6000, 136), (65, 64, 20000), (200, 4096, 256), (2100, 72, 136),
                                    (3000, 256, 2304), (513, 512, 4096)])
 def test_linear_splits(T, K, N):
     run_linear(T, K, N, act="gelu_tanh", seed=1)
@@ -211,7 +212,7 @@ def run_ffn(T, H, I, act="era", dtype=BF16, bias=True, residual=True, seed=0, wd
             ref.check(n, g, *want[n], 4, dtype)
 
 
-@pytest.mark.parametrize("T", [1, 8, 9, 16, 17, 100, 256, 300])
+@pytest.mark.parametrize("T", [1, 8, 9, 16, 17, 100, 128, 129, 256, 300])
 @pytest.mark.parametrize("H,I", [(64, 128), (40, 72), (136, 264)])
 def test_gated_ffn_sizes(T, H, I):
     run_ffn(T, H, I, seed=T)
@@ -308,6 +309,43 @@ def test_nan_and_inf_pass_through():
                 y = vb.linear(x, w, activation=act)
                 assert torch.isnan(y[1]).all() and torch.isinf(y[2]).all(), (act, dtype, T)
                 assert torch.isfinite(y[0]).all() and torch.isfinite(y[3:]).all()
+
+
+@pytest.mark.parametrize("T", [3, 40, 300])
+@pytest.mark.parametrize("bad", [float("inf"), -float("inf"), float("nan"), 3.4e38])
+def test_f32_special_values(T, bad):
+    """fp32 products with an operand that has no sum of bf16 parts: the same infinities and NaNs
+    as fp32 arithmetic gives, and the other values as exact as ever."""
+    import velvetoptimizer_b200 as vb
+    gen = torch.Generator().manual_seed(T)
+    K, N = 72, 40
+    for where in ("x", "w", "dy", None):
+        x, w, dy = (rand(gen, *s, dtype=F32) for s in ((T, K), (N, K), (T, N)))
+        w[5, 7] = 0.0  # infinity times zero
+        if where:
+            {"x": x, "w": w, "dy": dy}[where][2, 7] = bad
+        lx, lw = leaf(x), leaf(w)
+        y = vb.linear(lx, lw)
+        dx, dw = torch.autograd.grad(y, (lx, lw), dy.cuda())
+        for got, a, b in ((y, x, w.t()), (dx, dy, w), (dw, dy.t(), x)):
+            want, got = a @ b, got.detach().cpu()
+            assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isinf(), want.isinf())
+            assert torch.equal(got[want.isinf()], want[want.isinf()])
+            ok = want.isfinite()
+            a64, b64 = a.double(), b.double()
+            exact = (a64 @ b64)[ok]
+            bound = ((a64.abs() @ b64.abs()) * (a.shape[1] + 2) * 2.0 ** -23)[ok]
+            assert ((got[ok].double() - exact).abs() <= bound + 2.0 ** -24 * exact.abs()).all()
+    p = [rand(gen, T, 24, dtype=F32), rand(gen, 48, 24, dtype=F32), rand(gen, 48, 24, dtype=F32),
+         rand(gen, 24, 48, dtype=F32)]
+    p[0][1, 3] = bad
+    leaves = [leaf(t) for t in p]
+    y = vb.gated_ffn(*leaves)
+    grads = torch.autograd.grad(y, leaves, torch.ones_like(y))
+    assert not torch.isfinite(y[1]).all() and torch.isfinite(y[0]).all()
+    if math.isfinite(bad):
+        return
+    assert not torch.isfinite(grads[0][1]).all() and torch.isfinite(grads[0][0]).all()
 
 
 @pytest.mark.parametrize("T", [5, 100])

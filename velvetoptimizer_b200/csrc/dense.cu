@@ -4,6 +4,7 @@
 // Every call first lays its workspace out (Arena), then launches; the size functions run the
 // same layout without a base.  Nothing is allocated and the host never waits.
 #include <atomic>
+#include <initializer_list>
 
 #include "dense.h"
 #include "ops_host.h"
@@ -41,7 +42,20 @@ struct Call {
   bool dry;
   int dtype;
 
-  int ok(cudaError_t e, const char* what) {
+  bool overlap = true;
+  bool first = true;
+
+  // Runs a launch.  Every kernel here waits for the one before it (griddepcontrol.wait) before
+  // it touches memory, so all but a call's first, which follows the caller's work, may be
+  // launched while their predecessor still runs (`overlap`).  That shortens the backward's
+  // chains (777 x 520 x 1304 block, both ways: 99 -> 92 us) and the short kernels' (one-token
+  // block 27.3 -> 26.6 us), but not a product followed by its finish (64-row block 39.2 ->
+  // 42.0 us), so bf16 forwards beyond the small batches leave it off.
+  template <typename F>
+  int run(F&& launch, const char* what) {
+    PdlScope pdl(!first && overlap);
+    first = false;
+    const cudaError_t e = launch();
     return e == cudaSuccess ? VMOE_OK : ops_cuda_fail(o, e, what);
   }
 
@@ -54,7 +68,7 @@ struct Call {
     m.p = dst;
     m.ld = ld;
     if (dry || m.rows == 0) return VMOE_OK;
-    return ok(launch_pad_copy(src.p, src.ld, src.rows, src.cols, dst, ld, s), what);
+    return run([&] { return launch_pad_copy(src.p, src.ld, src.rows, src.cols, dst, ld, s); }, what);
   }
 };
 
@@ -85,114 +99,196 @@ int choose_splits(int64_t tiles, int kb, int pairs, int64_t partial_bytes) {
   return best;
 }
 
+// A product on the CTA pairs.  Its operand pairs (a[i], b[j]) are summed in one accumulator;
+// with two groups the second reads a[.. + group_a], and a gated one's follower b[.. + follower_b].
 struct Product {
   bool a_mn = false, b_mn = false;
   int epi = kEpiLinear;
-  Mat a0, a1, b0, b1;
-  int64_t M = 0, N = 0;
-  int64_t k0 = 0, k1 = 0;  // reduction lengths of the operand pairs
-  int groups = 1;
+  Mat a[6], b[6];
+  int segs = 1;
+  unsigned char seg_a[12] = {}, seg_b[12] = {};
+  int64_t M = 0, N = 0, K = 0;  // K: one pair's reduction length
+  int groups = 1, group_a = 0, follower_b = 0;
   DenseEpi e;
   const char* what = "";
+
+  int kbs() const { return static_cast<int>((K + 63) / 64); }
+  int64_t m_tiles() const { return (M + 255) / 256; }
+  int64_t n_tiles() const { return epi == kEpiGated ? (N + 127) / 128 : (N + 255) / 256; }
+  int splits(const vmoe_ops* o) const {
+    return choose_splits(m_tiles() * n_tiles() * groups, segs * kbs(), o->num_sms / 2,
+                         M * n_tiles() * 1024 * groups);
+  }
 };
 
-int product_splits(const Call& c, const Product& p) {
-  const int64_t m_tiles = (p.M + 255) / 256;
-  const int64_t n_tiles = p.epi == kEpiGated ? (p.N + 127) / 128 : (p.N + 255) / 256;
-  return choose_splits(m_tiles * n_tiles * p.groups,
-                       static_cast<int>((p.k0 + 63) / 64 + (p.k1 + 63) / 64), c.o->num_sms / 2,
-                       p.M * n_tiles * 1024 * p.groups);
-}
-
-// One bf16 product on the CTA pairs, split over k where its tiles leave SMs idle.
-int run_product(Call& c, const Product& p) {
-  const int64_t m_tiles = (p.M + 255) / 256;
-  const int64_t n_tiles = p.epi == kEpiGated ? (p.N + 127) / 128 : (p.N + 255) / 256;
-  if (m_tiles * n_tiles * p.groups * 16 > 0x7fffffff)
-    return ops_fail(c.o, VMOE_ERR_UNSUPPORTED_SHAPE, "%s: too many output tiles", p.what);
+// Lays a product out: its tiles, its splits and, where it has splits or `partials` asks for
+// them, its partial sums.
+DenseGemm plan_product(Call& c, const Product& p, bool partials) {
   DenseGemm g;
   g.M = p.M;
   g.N = p.N;
-  g.m_tiles = static_cast<int>(m_tiles);
-  g.n_tiles = static_cast<int>(n_tiles);
+  g.m_tiles = static_cast<int>(p.m_tiles());
+  g.n_tiles = static_cast<int>(p.n_tiles());
+  g.segs = p.segs;
+  g.kbs = p.kbs();
+  memcpy(g.seg_a, p.seg_a, sizeof(g.seg_a));
+  memcpy(g.seg_b, p.seg_b, sizeof(g.seg_b));
   g.groups = p.groups;
-  g.kb0 = static_cast<int>((p.k0 + 63) / 64);
-  g.kb1 = static_cast<int>((p.k1 + 63) / 64);
-  const int kb = g.kb0 + g.kb1;
-  g.ldp = n_tiles * 256;
-  const int64_t part = p.M * g.ldp * 4 * p.groups;
-  g.splits = product_splits(c, p);
-  g.kb_per_split = (kb + g.splits - 1) / g.splits;
-  g.band = n_tiles < 8 ? static_cast<int>(n_tiles) : 8;
+  g.group_a = p.group_a;
+  g.follower_b = p.follower_b;
+  g.ldp = p.n_tiles() * 256;
+  g.splits = p.splits(c.o);
+  g.kb_per_split = (p.segs * g.kbs + g.splits - 1) / g.splits;
+  g.band = g.n_tiles < 8 ? g.n_tiles : 8;
   g.epi = p.e;
   g.status = c.o->status;
-  if (g.splits > 1) g.partial = c.ws.take<float>(static_cast<size_t>(part) * g.splits);
-  if (c.dry) return VMOE_OK;
+  if (g.splits > 1 || partials)
+    g.partial = c.ws.take<float>(static_cast<size_t>(p.M * g.ldp * 4 * p.groups) * g.splits);
+  return g;
+}
+
+int launch_product(Call& c, const Product& p, const DenseGemm& g) {
   DenseMaps maps;
   char why[256];
-  const uint32_t abox = p.a_mn ? 64 : 128, bbox = p.b_mn ? 64 : 128;
-  auto map = [&](CUtensorMap* m, const Mat& x, uint32_t box) {
-    return make_tmap_bf16(m, x.p, static_cast<uint64_t>(x.rows), static_cast<uint64_t>(x.cols),
-                          static_cast<uint64_t>(x.ld), box, why, sizeof(why));
-  };
-  bool good = map(&maps.a0, p.a0, abox) && map(&maps.b0, p.b0, bbox);
-  if (good && p.a1.p) good = map(&maps.a1, p.a1, abox); else maps.a1 = maps.a0;
-  if (good && p.b1.p) good = map(&maps.b1, p.b1, bbox); else maps.b1 = maps.b0;
-  if (!good) return ops_fail(c.o, VMOE_ERR_CUDA, "%s: %s", p.what, why);
-  TRY(c.ok(launch_gemm_dense(p.a_mn, p.b_mn, p.epi, maps, g, c.o->num_sms, c.s), p.what));
-  if (g.splits > 1) return c.ok(launch_dense_finish(kBF16, p.epi, g, c.s), p.what);
+  for (int i = 0; i < 6; ++i) {
+    const struct { CUtensorMap* map; const Mat& m; bool mn; } two[2] = {
+        {&maps.a[i], p.a[i], p.a_mn}, {&maps.b[i], p.b[i], p.b_mn}};
+    for (const auto& t : two) {
+      if (t.m.p && !make_tmap_bf16(t.map, t.m.p, static_cast<uint64_t>(t.m.rows),
+                                   static_cast<uint64_t>(t.m.cols), static_cast<uint64_t>(t.m.ld),
+                                   t.mn ? 64 : 128, why, sizeof(why)))
+        return ops_fail(c.o, VMOE_ERR_CUDA, "%s: %s", p.what, why);
+    }
+  }
+  return c.run(
+      [&] { return launch_gemm_dense(p.a_mn, p.b_mn, p.epi, maps, g, c.o->num_sms, c.s); }, p.what);
+}
+
+int check_tiles(Call& c, const Product& p) {
+  if (p.m_tiles() * p.n_tiles() * p.groups * 16 > 0x7fffffff)
+    return ops_fail(c.o, VMOE_ERR_UNSUPPORTED_SHAPE, "%s: too many output tiles", p.what);
   return VMOE_OK;
 }
 
-// The fp32 counterpart: partial sums of one or two operand pairs (or a gate and an up part),
-// then the epilogue.
-struct SimtPart {
-  const float *a, *b;
-  int64_t am, ak, bn, bk, K;
+// One bf16 product, split over k where its tiles leave SMs idle.
+int run_product(Call& c, const Product& p) {
+  TRY(check_tiles(c, p));
+  const DenseGemm g = plan_product(c, p, false);
+  if (c.dry) return VMOE_OK;
+  TRY(launch_product(c, p, g));
+  if (!g.partial) return VMOE_OK;
+  return c.run([&] { return launch_dense_finish(kBF16, p.epi, g, c.s); }, p.what);
+}
+
+// The same for a decode batch's forward: x [T, K] and weights [N, K] (gated: two of them).
+int run_skinny(Call& c, int epi, Mat x, Mat w, Mat w2, const DenseEpi& e, const char* what) {
+  TRY(c.tma_ready(x, what));
+  TRY(c.tma_ready(w, what));
+  if (epi == kEpiGated) TRY(c.tma_ready(w2, what));
+  if (c.dry) return VMOE_OK;
+  CUtensorMap mw, mw2, mx;
+  char why[256];
+  auto map = [&](CUtensorMap* m, const Mat& t, int64_t box) {
+    return make_tmap_bf16(m, t.p, static_cast<uint64_t>(t.rows), static_cast<uint64_t>(t.cols),
+                          static_cast<uint64_t>(t.ld), static_cast<uint32_t>(box), why, sizeof(why));
+  };
+  const bool gated = epi == kEpiGated;
+  if (!map(&mx, x, round_up(x.rows, 16)) || !map(&mw, w, gated ? 64 : 128) ||
+      (gated && !map(&mw2, w2, 64)))
+    return ops_fail(c.o, VMOE_ERR_CUDA, "%s: %s", what, why);
+  if (!gated) mw2 = mw;
+  SkinnyGemm g{};
+  g.T = x.rows;
+  g.N = w.rows;
+  g.kbs = static_cast<int>((x.cols + 63) / 64);
+  g.epi = e;
+  g.status = c.o->status;
+  return c.run([&] { return launch_dense_skinny(epi, mw, mw2, mx, g, c.s); }, what);
+}
+
+// ---- fp32 products: six bf16 ones (dense_f32.cu) -------------------------------------------
+struct F32Mat {
+  const float* p = nullptr;
+  int64_t rows = 0, cols = 0, ld = 0;
+  Mat plane[3];
 };
 
-int run_simt(Call& c, int epi, const SimtPart* parts, int n_parts, int64_t M, int64_t N,
-             const DenseEpi& e, const char* what) {
-  const bool gated = epi == kEpiGated;
-  const int64_t tiles = ((M + 127) / 128) * ((N + 127) / 128) * (gated ? 2 : 1);
-  int64_t kmax = 1;
-  for (int i = 0; i < n_parts; ++i) kmax = parts[i].K > kmax ? parts[i].K : kmax;
-  // about two blocks per SM, each with 64 or more k
-  int64_t splits = 2 * c.o->num_sms / (tiles > 0 ? tiles : 1);
-  if (splits > kmax / 64) splits = kmax / 64;
-  if (splits > 64) splits = 64;
-  if (splits < 1) splits = 1;
-  const int64_t per = round_up((kmax + splits - 1) / splits, 16);
-  splits = (kmax + per - 1) / per;
-  DenseGemm g;
-  g.M = M;
-  g.N = N;
-  g.ldp = gated ? (N + 127) / 128 * 256 : round_up(N, 8);
-  g.splits = static_cast<int>(gated ? splits : splits * n_parts);
-  g.epi = e;
-  const int64_t stride = M * g.ldp;
-  g.partial = c.ws.take<float>(static_cast<size_t>(stride) * g.splits * 4);
-  if (c.dry) return VMOE_OK;
-  for (int i = 0; i < n_parts; ++i) {
-    SimtGemm q{};
-    q.a = parts[i].a;
-    q.b = parts[i].b;
-    q.am = parts[i].am;
-    q.ak = parts[i].ak;
-    q.bn = parts[i].bn;
-    q.bk = parts[i].bk;
-    q.M = M;
-    q.N = N;
-    q.K = parts[i].K;
-    q.splits = static_cast<int>(splits);
-    q.k_per_split = per;
-    q.partial = g.partial + (gated ? 0 : static_cast<int64_t>(i) * splits * stride);
-    q.ldp = g.ldp;
-    q.split_stride = stride;
-    q.gated_cols = gated ? 1 + i : 0;
-    TRY(c.ok(launch_dense_simt(q, c.s), what));
+// The planes of up to kMats matrices of one call, and their flags.
+struct F32Planes {
+  static constexpr int kMats = 8;
+  int* flags = nullptr;
+  int n = 0;
+
+  explicit F32Planes(Call& c) { flags = c.ws.take<int>(kMats * kSplitBlocks * 4); }
+
+  int split(Call& c, std::initializer_list<F32Mat*> mats) {
+    Split3 s[3];
+    int k = 0;
+    for (F32Mat* m : mats) {
+      const int64_t ld = round_up(m->cols, 8), plane = m->rows * ld;
+      auto* out = c.ws.take<uint16_t>(static_cast<size_t>(3 * plane) * 2);
+      for (int i = 0; i < 3; ++i)
+        m->plane[i] = {out ? out + i * plane : nullptr, m->rows, m->cols, ld};
+      s[k++] = {m->p, m->ld, m->rows, m->cols, out, ld, plane};
+    }
+    int* f = flags ? flags + n * kSplitBlocks : nullptr;
+    n += k;
+    if (c.dry) return VMOE_OK;
+    return c.run([&] { return launch_split3(s, k, f, c.s); }, "fp32 planes");
   }
-  return c.ok(launch_dense_finish(kF32, epi, g, c.s), what);
+};
+
+// C = sum over the pairs of A B, or with two groups (gated: two Bs) one product for each, then
+// the epilogue.  p.a / p.b and the pairs' lists are filled in here.
+int run_f32(Call& c, Product p, const F32Planes& planes, std::initializer_list<const F32Mat*> as,
+            std::initializer_list<const F32Mat*> bs) {
+  TRY(check_tiles(c, p));
+  const int na = static_cast<int>(as.size()), nb = static_cast<int>(bs.size());
+  const bool two_pairs = na == 2 && nb == 2;
+  int i = 0;
+  for (const F32Mat* m : as)
+    for (int k = 0; k < 3; ++k) p.a[i++] = m->plane[k];
+  i = 0;
+  for (const F32Mat* m : bs)
+    for (int k = 0; k < 3; ++k) p.b[i++] = m->plane[k];
+  static const unsigned char ka[6] = {2, 0, 1, 1, 0, 0}, kb[6] = {0, 2, 1, 0, 1, 0};
+  p.segs = two_pairs ? 12 : 6;
+  for (int s = 0; s < p.segs; ++s) {  // both pairs' small terms first
+    const int pair = two_pairs ? s % 2 : 0, t = two_pairs ? s / 2 : s;
+    p.seg_a[s] = static_cast<unsigned char>(3 * pair + ka[t]);
+    p.seg_b[s] = static_cast<unsigned char>(3 * pair + kb[t]);
+  }
+  p.group_a = 3;
+  p.follower_b = p.epi == kEpiGated ? 3 : 0;
+  const DenseGemm g = plan_product(c, p, true);
+  if (c.dry) return VMOE_OK;
+  TRY(launch_product(c, p, g));
+  const int64_t area = p.M * g.ldp;
+  for (int q = 0; q < (na > nb ? na : nb); ++q) {
+    const F32Mat& a = *as.begin()[na == 2 ? q : 0];
+    const F32Mat& b = *bs.begin()[nb == 2 ? q : 0];
+    SimtGemm r{};
+    r.a = a.p;
+    r.b = b.p;
+    r.am = p.a_mn ? 1 : a.ld;
+    r.ak = p.a_mn ? a.ld : 1;
+    r.bn = p.b_mn ? 1 : b.ld;
+    r.bk = p.b_mn ? b.ld : 1;
+    r.M = p.M;
+    r.N = p.N;
+    r.K = p.K;
+    r.splits = g.splits;
+    r.k_per_split = (p.K + g.splits - 1) / g.splits;
+    r.partial = g.partial + (p.groups == 2 ? q * area : 0);
+    r.ldp = g.ldp;
+    r.split_stride = p.groups * area;
+    r.gated_cols = p.epi == kEpiGated ? 1 + q : 0;
+    r.accumulate = two_pairs && q > 0;
+    r.flags = planes.flags;
+    r.n_flags = planes.n * kSplitBlocks;
+    TRY(c.run([&] { return launch_dense_simt(r, c.s); }, p.what));
+  }
+  return c.run([&] { return launch_dense_finish(kF32, p.epi, g, c.s); }, p.what);
 }
 
 // dz = dy act'(z) (written when `dz` is given) and the column sums into `db`.
@@ -220,9 +316,9 @@ int run_dz(Call& c, const void* dy, int64_t lddy, const void* z, int64_t ldz, vo
   a.row_blocks = static_cast<int>((T + a.rows_per_block - 1) / a.rows_per_block);
   if (db) a.colsum = c.ws.take<float>(static_cast<size_t>(a.row_blocks) * N * 4);
   if (c.dry) return VMOE_OK;
-  TRY(c.ok(launch_dense_dz(c.dtype, a, c.s), "activation gradient"));
+  TRY(c.run([&] { return launch_dense_dz(c.dtype, a, c.s); }, "activation gradient"));
   if (db)
-    return c.ok(launch_colsum_finish(a.colsum, a.row_blocks, N, db, db_f32, c.s), "bias gradient");
+    return c.run([&] { return launch_colsum_finish(a.colsum, a.row_blocks, N, db, db_f32, c.s); }, "bias gradient");
   return VMOE_OK;
 }
 
@@ -332,11 +428,6 @@ int linear_forward(Call& c, const vmoe_linear& d, const LinearPtrs& p) {
   e.ldz = N;
   e.vec = (vec_ok(p.y, N, N, elt) ? kVecOut : 0) | (vec_ok(p.r, d.ldr, N, elt) ? kVecRes : 0) |
           (vec_ok(p.z, N, N, elt) ? kVecZ : 0);
-  if (d.dtype == VMOE_F32) {
-    const SimtPart part{static_cast<const float*>(p.x), static_cast<const float*>(p.w), d.ldx, 1,
-                        d.ldw, 1, K};
-    return run_simt(c, kEpiLinear, &part, 1, T, N, e, "linear");
-  }
   if (T <= kSmallTokens) {
     if (c.dry) return VMOE_OK;
     SmallGemm g{};
@@ -348,19 +439,29 @@ int linear_forward(Call& c, const vmoe_linear& d, const LinearPtrs& p) {
     g.N = N;
     g.K = K;
     g.epi = e;
-    g.vec_in = K % 8 == 0 && pitch16(p.x, d.ldx, 2) && pitch16(p.w, d.ldw, 2);
-    return c.ok(launch_dense_small(kEpiLinear, g, c.s), "linear");
+    g.num_sms = c.o->num_sms;
+    g.vec_in = K * elt % 16 == 0 && pitch16(p.x, d.ldx, elt) && pitch16(p.w, d.ldw, elt);
+    return c.run([&] { return launch_dense_small(d.dtype, kEpiLinear, g, c.s); }, "linear");
   }
+  c.overlap = d.dtype == VMOE_F32;
+  if (d.dtype == VMOE_BF16 && T <= kSkinnyTokens)
+    return run_skinny(c, kEpiLinear, {p.x, T, K, d.ldx}, {p.w, N, K, d.ldw}, {}, e, "linear");
   Product q;
-  q.a0 = {p.x, T, K, d.ldx};
-  q.b0 = {p.w, N, K, d.ldw};
-  TRY(c.tma_ready(q.a0, "linear"));
-  TRY(c.tma_ready(q.b0, "linear"));
   q.M = T;
   q.N = N;
-  q.k0 = K;
+  q.K = K;
   q.e = e;
   q.what = "linear";
+  if (d.dtype == VMOE_F32) {
+    F32Mat x{static_cast<const float*>(p.x), T, K, d.ldx}, w{static_cast<const float*>(p.w), N, K, d.ldw};
+    F32Planes planes(c);
+    TRY(planes.split(c, {&x, &w}));
+    return run_f32(c, q, planes, {&x}, {&w});
+  }
+  q.a[0] = {p.x, T, K, d.ldx};
+  q.b[0] = {p.w, N, K, d.ldw};
+  TRY(c.tma_ready(q.a[0], "linear"));
+  TRY(c.tma_ready(q.b[0], "linear"));
   return run_product(c, q);
 }
 
@@ -389,46 +490,44 @@ int linear_backward(Call& c, const vmoe_linear& d, const LinearPtrs& p) {
   ew.ldo = K;
   ew.out_f32 = gf32;
   ew.vec = vec_ok(p.dw, K, K, gelt) ? kVecOut : 0;
+  Product qx, qw;
+  qx.b_mn = true;
+  qx.M = T;
+  qx.N = K;
+  qx.K = N;
+  qx.e = ex;
+  qx.what = "linear dx";
+  qw.a_mn = qw.b_mn = true;
+  qw.M = N;
+  qw.N = K;
+  qw.K = T;
+  qw.e = ew;
+  qw.what = "linear dW";
+  const bool need_x = c.dry || p.dx, need_w = c.dry || p.dw;
+  if (!need_x && !need_w) return VMOE_OK;
   if (f32) {
-    const auto* fz = static_cast<const float*>(dz);
-    const auto* fx = static_cast<const float*>(p.x);
-    const auto* fw = static_cast<const float*>(p.w);
-    if (c.dry || p.dx) {
-      const SimtPart part{fz, fw, lddz, 1, 1, d.ldw, N};
-      TRY(run_simt(c, kEpiLinear, &part, 1, T, K, ex, "linear dx"));
-    }
-    if (c.dry || p.dw) {
-      const SimtPart part{fz, fx, 1, lddz, 1, d.ldx, T};
-      TRY(run_simt(c, kEpiLinear, &part, 1, N, K, ew, "linear dW"));
-    }
+    F32Mat z{static_cast<const float*>(dz), T, N, lddz}, x{static_cast<const float*>(p.x), T, K, d.ldx},
+        w{static_cast<const float*>(p.w), N, K, d.ldw};
+    F32Planes planes(c);
+    if (need_x && need_w) TRY(planes.split(c, {&z, &x, &w}));
+    else if (need_x) TRY(planes.split(c, {&z, &w}));
+    else TRY(planes.split(c, {&z, &x}));
+    if (need_x) TRY(run_f32(c, qx, planes, {&z}, {&w}));
+    if (need_w) TRY(run_f32(c, qw, planes, {&z}, {&x}));
     return VMOE_OK;
   }
   const Mat z{dz, T, N, lddz};
-  if (c.dry || p.dx) {
-    Product q;
-    q.b_mn = true;
-    q.a0 = z;
-    q.b0 = {p.w, N, K, d.ldw};
-    TRY(c.tma_ready(q.b0, "linear dx"));
-    q.M = T;
-    q.N = K;
-    q.k0 = N;
-    q.e = ex;
-    q.what = "linear dx";
-    TRY(run_product(c, q));
+  if (need_x) {
+    qx.a[0] = z;
+    qx.b[0] = {p.w, N, K, d.ldw};
+    TRY(c.tma_ready(qx.b[0], "linear dx"));
+    TRY(run_product(c, qx));
   }
-  if (c.dry || p.dw) {
-    Product q;
-    q.a_mn = q.b_mn = true;
-    q.a0 = z;
-    q.b0 = {p.x, T, K, d.ldx};
-    TRY(c.tma_ready(q.b0, "linear dW"));
-    q.M = N;
-    q.N = K;
-    q.k0 = T;
-    q.e = ew;
-    q.what = "linear dW";
-    TRY(run_product(c, q));
+  if (need_w) {
+    qw.a[0] = z;
+    qw.b[0] = {p.x, T, K, d.ldx};
+    TRY(c.tma_ready(qw.b[0], "linear dW"));
+    TRY(run_product(c, qw));
   }
   return VMOE_OK;
 }
@@ -483,15 +582,6 @@ int ffn_forward(Call& c, const vmoe_gated_ffn& d, const FfnPtrs& p) {
   e2.out = p.y;
   e2.ldo = H;
   e2.vec = (vec_ok(p.y, H, H, elt) ? kVecOut : 0) | (vec_ok(p.r, d.ldr, H, elt) ? kVecRes : 0);
-  if (d.dtype == VMOE_F32) {
-    const auto* x = static_cast<const float*>(p.x);
-    const SimtPart gu[2] = {{x, static_cast<const float*>(p.w.gate_w), d.ldx, 1, H, 1, H},
-                            {x, static_cast<const float*>(p.w.up_w), d.ldx, 1, H, 1, H}};
-    TRY(run_simt(c, kEpiGated, gu, 2, T, I, e1, "gate|up"));
-    const SimtPart dn{static_cast<const float*>(h), static_cast<const float*>(p.w.down_w), sv.ld, 1,
-                      I, 1, I};
-    return run_simt(c, kEpiLinear, &dn, 1, T, H, e2, "down");
-  }
   if (T <= kSmallTokens) {
     if (c.dry) return VMOE_OK;
     SmallGemm g{};
@@ -504,8 +594,10 @@ int ffn_forward(Call& c, const vmoe_gated_ffn& d, const FfnPtrs& p) {
     g.N = I;
     g.K = H;
     g.epi = e1;
-    g.vec_in = H % 8 == 0 && pitch16(p.x, d.ldx, 2) && aligned16(p.w.gate_w) && aligned16(p.w.up_w);
-    TRY(c.ok(launch_dense_small(kEpiGated, g, c.s), "gate|up"));
+    g.num_sms = c.o->num_sms;
+    g.vec_in = H * elt % 16 == 0 && pitch16(p.x, d.ldx, elt) && aligned16(p.w.gate_w) &&
+               aligned16(p.w.up_w);
+    TRY(c.run([&] { return launch_dense_small(d.dtype, kEpiGated, g, c.s); }, "gate|up"));
     SmallGemm q{};
     q.x = h;
     q.w = p.w.down_w;
@@ -515,33 +607,49 @@ int ffn_forward(Call& c, const vmoe_gated_ffn& d, const FfnPtrs& p) {
     q.N = H;
     q.K = I;
     q.epi = e2;
-    q.vec_in = I % 8 == 0 && aligned16(p.w.down_w);
-    PdlScope pdl(true);  // its launch overlaps the gate|up kernel's end
-    return c.ok(launch_dense_small(kEpiLinear, q, c.s), "down");
+    q.num_sms = c.o->num_sms;
+    q.vec_in = I * elt % 16 == 0 && aligned16(p.w.down_w);
+    return c.run([&] { return launch_dense_small(d.dtype, kEpiLinear, q, c.s); }, "down");
   }
-  Product g;
+  if (d.dtype == VMOE_BF16 && T <= kSkinnyTokens) {
+    TRY(run_skinny(c, kEpiGated, {p.x, T, H, d.ldx}, {p.w.gate_w, I, H, H}, {p.w.up_w, I, H, H}, e1,
+                   "gate|up"));
+    return run_skinny(c, kEpiLinear, {h, T, I, sv.ld}, {p.w.down_w, H, I, I}, {}, e2, "down");
+  }
+  c.overlap = d.dtype == VMOE_F32;
+  Product g, q;
   g.epi = kEpiGated;
-  g.a0 = {p.x, T, H, d.ldx};
-  g.b0 = {p.w.gate_w, I, H, H};
-  g.b1 = {p.w.up_w, I, H, H};
-  TRY(c.tma_ready(g.a0, "gate|up"));
-  TRY(c.tma_ready(g.b0, "gate|up"));
-  TRY(c.tma_ready(g.b1, "gate|up"));
   g.M = T;
   g.N = I;
-  g.k0 = H;
+  g.K = H;
   g.e = e1;
   g.what = "gate|up";
-  TRY(run_product(c, g));
-  Product q;
-  q.a0 = {h, T, I, sv.ld};
-  q.b0 = {p.w.down_w, H, I, I};
-  TRY(c.tma_ready(q.b0, "down"));
   q.M = T;
   q.N = H;
-  q.k0 = I;
+  q.K = I;
   q.e = e2;
   q.what = "down";
+  if (d.dtype == VMOE_F32) {
+    auto F = [](const void* m) { return static_cast<const float*>(m); };
+    F32Mat x{F(p.x), T, H, d.ldx}, wg{F(p.w.gate_w), I, H, H}, wu{F(p.w.up_w), I, H, H},
+        hm{F(h), T, I, sv.ld}, wd{F(p.w.down_w), H, I, I};
+    F32Planes planes(c);
+    TRY(planes.split(c, {&x, &wg, &wu}));
+    TRY(run_f32(c, g, planes, {&x}, {&wg, &wu}));
+    TRY(planes.split(c, {&hm, &wd}));
+    return run_f32(c, q, planes, {&hm}, {&wd});
+  }
+  g.follower_b = 1;
+  g.a[0] = {p.x, T, H, d.ldx};
+  g.b[0] = {p.w.gate_w, I, H, H};
+  g.b[1] = {p.w.up_w, I, H, H};
+  TRY(c.tma_ready(g.a[0], "gate|up"));
+  TRY(c.tma_ready(g.b[0], "gate|up"));
+  TRY(c.tma_ready(g.b[1], "gate|up"));
+  TRY(run_product(c, g));
+  q.a[0] = {h, T, I, sv.ld};
+  q.b[0] = {p.w.down_w, H, I, I};
+  TRY(c.tma_ready(q.b[0], "down"));
   return run_product(c, q);
 }
 
@@ -590,108 +698,117 @@ int ffn_backward(Call& c, const vmoe_gated_ffn& d, const FfnPtrs& p) {
     q.vec = vec_ok(out, ld, ld, grad ? gelt : elt) ? kVecOut : 0;
     return q;
   };
+  Product qh, qx, qgu, qd;
+  qh.b_mn = true;
+  qh.epi = kEpiGluBwd;
+  qh.M = T;
+  qh.N = I;
+  qh.K = H;
+  qh.e = e;
+  qh.what = "dh";
+  qx.b_mn = true;
+  qx.M = T;
+  qx.N = H;
+  qx.K = I;
+  qx.e = plain(p.dx, H, false);
+  qx.what = "dx";
+  const bool need_x = c.dry || p.dx;
+  // the gate's and the up's weight gradients in one launch where both are asked for
+  const bool need_gu = c.dry || gr.gate_w || gr.up_w, both = c.dry || (gr.gate_w && gr.up_w);
+  const bool only_up = !both && gr.up_w;
+  qgu.a_mn = qgu.b_mn = true;
+  qgu.M = I;
+  qgu.N = H;
+  qgu.K = T;
+  qgu.groups = both ? 2 : 1;
+  qgu.e = plain(only_up ? gr.up_w : gr.gate_w, H, true);
+  if (both) {
+    qgu.e.out2 = gr.up_w;
+    if (!vec_ok(gr.up_w, H, H, gelt)) qgu.e.vec = 0;
+  }
+  qgu.what = "dW gate|up";
+  const bool need_d = c.dry || gr.down_w;
+  qd.a_mn = qd.b_mn = true;
+  qd.M = H;
+  qd.N = I;
+  qd.K = T;
+  qd.e = plain(gr.down_w, I, true);
+  qd.what = "dW down";
   if (f32) {
-    const auto* fx = static_cast<const float*>(p.x);
-    const auto* fdy = static_cast<const float*>(p.dy);
-    auto F = [](const void* q) { return static_cast<const float*>(q); };
+    auto F = [](const void* m) { return static_cast<const float*>(m); };
+    F32Mat mdy{F(p.dy), T, H, p.lddy}, wd{F(p.w.down_w), H, I, I}, mdg{F(dg), T, I, sv.ld},
+        mdu{F(du), T, I, sv.ld}, x{F(p.x), T, H, d.ldx}, wg{F(p.w.gate_w), I, H, H},
+        wu{F(p.w.up_w), I, H, H}, hm{F(h), T, I, sv.ld};
+    F32Planes planes(c);
     if (need_dgu) {
-      const SimtPart part{fdy, F(p.w.down_w), p.lddy, 1, 1, I, H};
-      TRY(run_simt(c, kEpiGluBwd, &part, 1, T, I, e, "dh"));
+      TRY(planes.split(c, {&mdy, &wd}));
+      TRY(run_f32(c, qh, planes, {&mdy}, {&wd}));
+      if (need_x || need_gu) TRY(planes.split(c, {&mdg, &mdu}));
+    } else if (need_d) {
+      TRY(planes.split(c, {&mdy}));
     }
-    if (c.dry || p.dx) {
-      const SimtPart parts[2] = {{F(dg), F(p.w.gate_w), sv.ld, 1, 1, H, I},
-                                 {F(du), F(p.w.up_w), sv.ld, 1, 1, H, I}};
-      TRY(run_simt(c, kEpiLinear, parts, 2, T, H, plain(p.dx, H, false), "dx"));
+    if (need_x) {
+      TRY(planes.split(c, {&wg, &wu}));
+      TRY(run_f32(c, qx, planes, {&mdg, &mdu}, {&wg, &wu}));
     }
-    const struct { const void* a; int64_t lda; const float* b; int64_t ldb, M, N; void* out; } wg[3] = {
-        {dg, sv.ld, fx, d.ldx, I, H, gr.gate_w},
-        {du, sv.ld, fx, d.ldx, I, H, gr.up_w},
-        {fdy, p.lddy, F(h), sv.ld, H, I, gr.down_w}};
-    for (const auto& q : wg) {
-      if (!c.dry && !q.out) continue;
-      const SimtPart part{F(q.a), q.b, 1, q.lda, 1, q.ldb, T};
-      TRY(run_simt(c, kEpiLinear, &part, 1, q.M, q.N, plain(q.out, q.N, true), "dW"));
+    if (need_gu) {
+      TRY(planes.split(c, {&x}));
+      if (both) TRY(run_f32(c, qgu, planes, {&mdg, &mdu}, {&x}));
+      if (c.dry) qgu.groups = 1;  // one gradient alone may be split into more parts
+      if (c.dry || !both) TRY(run_f32(c, qgu, planes, {only_up ? &mdu : &mdg}, {&x}));
+    }
+    if (need_d) {
+      TRY(planes.split(c, {&hm}));
+      TRY(run_f32(c, qd, planes, {&mdy}, {&hm}));
     }
   } else {
     if (need_dgu) {
-      Product q;
-      q.b_mn = true;
-      q.epi = kEpiGluBwd;
-      q.a0 = dy;
-      q.b0 = {p.w.down_w, H, I, I};
-      TRY(c.tma_ready(q.b0, "dh"));
-      q.M = T;
-      q.N = I;
-      q.k0 = H;
-      q.e = e;
-      q.what = "dh";
+      qh.a[0] = dy;
+      qh.b[0] = {p.w.down_w, H, I, I};
+      TRY(c.tma_ready(qh.b[0], "dh"));
       // the gate's and the up's bias gradients: column sums in the epilogue, where it runs once
-      if ((c.dry || gr.gate_b || gr.up_b) && product_splits(c, q) == 1) {
-        q.e.colsum_stride = row_blocks * I;
-        q.e.colsum = colsum = c.ws.take<float>(static_cast<size_t>(2 * row_blocks * I) * 4);
+      if ((c.dry || gr.gate_b || gr.up_b) && qh.splits(c.o) == 1) {
+        qh.e.colsum_stride = row_blocks * I;
+        qh.e.colsum = colsum = c.ws.take<float>(static_cast<size_t>(2 * row_blocks * I) * 4);
         summed = true;
       }
-      TRY(run_product(c, q));
+      TRY(run_product(c, qh));
     }
     const Mat mdg{dg, T, I, sv.ld}, mdu{du, T, I, sv.ld};
-    if (c.dry || p.dx) {
-      Product q;
-      q.b_mn = true;
-      q.a0 = mdg;
-      q.a1 = mdu;
-      q.b0 = {p.w.gate_w, I, H, H};
-      q.b1 = {p.w.up_w, I, H, H};
-      TRY(c.tma_ready(q.b0, "dx"));
-      TRY(c.tma_ready(q.b1, "dx"));
-      q.M = T;
-      q.N = H;
-      q.k0 = q.k1 = I;
-      q.e = plain(p.dx, H, false);
-      q.what = "dx";
-      TRY(run_product(c, q));
+    if (need_x) {
+      qx.segs = 2;
+      qx.seg_a[1] = qx.seg_b[1] = 1;
+      qx.a[0] = mdg;
+      qx.a[1] = mdu;
+      qx.b[0] = {p.w.gate_w, I, H, H};
+      qx.b[1] = {p.w.up_w, I, H, H};
+      TRY(c.tma_ready(qx.b[0], "dx"));
+      TRY(c.tma_ready(qx.b[1], "dx"));
+      TRY(run_product(c, qx));
     }
-    if (c.dry || gr.gate_w || gr.up_w) {
-      Product q;
-      q.a_mn = q.b_mn = true;
-      q.b0 = {p.x, T, H, d.ldx};
-      TRY(c.tma_ready(q.b0, "dW gate|up"));
-      q.M = I;
-      q.N = H;
-      q.k0 = T;
-      const bool both = c.dry || (gr.gate_w && gr.up_w);
-      q.groups = both ? 2 : 1;
-      q.a0 = both || gr.gate_w ? mdg : mdu;
-      if (both) q.a1 = mdu;
-      q.e = plain(both || gr.gate_w ? gr.gate_w : gr.up_w, H, true);
-      if (both) {
-        q.e.out2 = gr.up_w;
-        if (!vec_ok(gr.up_w, H, H, gelt)) q.e.vec = 0;
-      }
-      q.what = "dW gate|up";
-      TRY(run_product(c, q));
-      if (c.dry) {  // one gradient alone may be split into more parts
-        q.groups = 1;
-        TRY(run_product(c, q));
+    if (need_gu) {
+      qgu.b[0] = {p.x, T, H, d.ldx};
+      TRY(c.tma_ready(qgu.b[0], "dW gate|up"));
+      qgu.group_a = 1;
+      qgu.a[0] = only_up ? mdu : mdg;
+      if (both) qgu.a[1] = mdu;
+      TRY(run_product(c, qgu));
+      if (c.dry) {
+        qgu.groups = 1;
+        TRY(run_product(c, qgu));
       }
     }
-    if (c.dry || gr.down_w) {
-      Product q;
-      q.a_mn = q.b_mn = true;
-      q.a0 = dy;
-      q.b0 = {h, T, I, sv.ld};
-      q.M = H;
-      q.N = I;
-      q.k0 = T;
-      q.e = plain(gr.down_w, I, true);
-      q.what = "dW down";
-      TRY(run_product(c, q));
+    if (need_d) {
+      qd.a[0] = dy;
+      qd.b[0] = {h, T, I, sv.ld};
+      TRY(run_product(c, qd));
     }
   }
   if (summed) {
     if (c.dry) return VMOE_OK;
-    if (gr.gate_b) TRY(c.ok(launch_colsum_finish(colsum, row_blocks, I, gr.gate_b, gf32, c.s), "dbg"));
+    if (gr.gate_b) TRY(c.run([&] { return launch_colsum_finish(colsum, row_blocks, I, gr.gate_b, gf32, c.s); }, "dbg"));
     if (gr.up_b)
-      TRY(c.ok(launch_colsum_finish(colsum + row_blocks * I, row_blocks, I, gr.up_b, gf32, c.s), "dbu"));
+      TRY(c.run([&] { return launch_colsum_finish(colsum + row_blocks * I, row_blocks, I, gr.up_b, gf32, c.s); }, "dbu"));
     return VMOE_OK;
   }
   TRY(run_dz(c, dg, sv.ld, nullptr, 0, nullptr, 0, T, I, kActNone, 0.f, c.dry ? any : gr.gate_b,

@@ -48,18 +48,22 @@ struct DenseEpi {
 struct DenseGemm {
   int64_t M = 0, N = 0;  // valid rows and columns (kEpiGated: N = features)
   int m_tiles = 0, n_tiles = 0;
-  int groups = 1;        // independent products sharing B: A map g, output out / out2
-  int kb0 = 0, kb1 = 0;  // 64-wide k blocks of the first and second operand pair
+  // the k loop: `segs` operand pairs of `kbs` 64-wide k blocks each, in one accumulator
+  int segs = 1, kbs = 0;
+  unsigned char seg_a[12] = {}, seg_b[12] = {};  // a pair's maps
+  int groups = 1;   // independent products sharing B: A maps group_a further, out / out2
+  int group_a = 0;
+  int follower_b = 0;  // kEpiGated: the follower's B maps (the up weight)
   int splits = 1, kb_per_split = 0;
   int band = 0;          // n tiles per band of the tile order
-  float* partial = nullptr;  // splits > 1: [splits][groups][M][ldp]
+  float* partial = nullptr;  // given: [splits][groups][M][ldp], and no epilogue
   int64_t ldp = 0;
   DenseEpi epi;
   int* status = nullptr;
 };
 
 struct DenseMaps {
-  CUtensorMap a0, a1, b0, b1;
+  CUtensorMap a[6], b[6];
 };
 
 // a_mn / b_mn: the operand is stored [k rows, M (or N) columns] and read MN-major;
@@ -71,17 +75,32 @@ cudaError_t launch_gemm_dense(bool a_mn, bool b_mn, int epi, const DenseMaps& ma
 // Sum of a split product's partials in split order, then its epilogue (dense_finish.cu).
 cudaError_t launch_dense_finish(int dtype, int epi, const DenseGemm& g, cudaStream_t s);
 
-// fp32 products on the CUDA cores, partials only (dense_simt.cu): element (m, k) of A at
-// a[m * am + k * ak], (n, k) of B at b[n * bn + k * bk].
+// fp32 as three bf16 planes (dense_f32.cu): x = hi + mid + lo to 2^-26.  Matrices of one
+// launch; plane k of a matrix is at out + k * plane elements, rows ldo apart.
+struct Split3 {
+  const float* x;
+  int64_t ldx, rows, cols;
+  void* out;
+  int64_t ldo, plane;
+};
+constexpr int kSplitBlocks = 592;  // blocks per matrix, each with a flag
+cudaError_t launch_split3(const Split3* m, int n, int* flags, cudaStream_t s);
+
+// fp32 products on the CUDA cores (dense_f32.cu), overwriting a product's partials, where any
+// of the n_flags flags is set: element (m, k) of A at a[m * am + k * ak], (n, k) of B at
+// b[n * bn + k * bk].
 struct SimtGemm {
   const float *a, *b;
   int64_t am, ak, bn, bk;
   int64_t M, N, K;
   int splits;
   int64_t k_per_split;
-  float* partial;  // [splits][.][ldp]; split s at partial + s * split_stride
+  float* partial;  // split s at partial + s * split_stride
   int64_t ldp, split_stride;
   int gated_cols;  // 0 plain; 1 / 2: gate / up columns of the 128-feature interleave
+  int accumulate;  // add to what is stored
+  const int* flags;
+  int n_flags;
 };
 cudaError_t launch_dense_simt(const SimtGemm& g, cudaStream_t s);
 
@@ -95,8 +114,25 @@ struct SmallGemm {
   int64_t T, N, K;
   DenseEpi epi;
   int vec_in;  // x and the weights allow 16-byte loads
+  int num_sms;
 };
-cudaError_t launch_dense_small(int epi, const SmallGemm& g, cudaStream_t s);
+cudaError_t launch_dense_small(int dtype, int epi, const SmallGemm& g, cudaStream_t s);
+
+// A decode batch (at most kSkinnyTokens rows): weights as the MMA's M operand, k divided over a
+// cluster (dense_skinny.cu).  Maps: weights in boxes of 64 k x 128 rows (gated: 64 rows of gate
+// and of up), x in boxes of 64 k x t_pad rows.
+constexpr int kSkinnyTokens = 128;
+struct SkinnyGemm {
+  int64_t T, N;
+  int kbs;  // 64-wide k blocks
+  DenseEpi epi;
+  int* status;
+  // set by the launcher
+  int t_pad, parts, kb_per_part, stages;
+  uint32_t tmem_cols, ring_bytes, exchange_bytes;
+};
+cudaError_t launch_dense_skinny(int epi, const CUtensorMap& w, const CUtensorMap& w2,
+                                const CUtensorMap& x, const SkinnyGemm& g, cudaStream_t s);
 
 // Elementwise and column work (dense_finish.cu).
 // dz = dy * act'(z) into dz [T, ld_dz] (null: not written), and the column sums of dz.

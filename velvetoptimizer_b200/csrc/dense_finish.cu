@@ -18,6 +18,7 @@ template <typename T, int EPI>
 __global__ void __launch_bounds__(256)
 dense_finish_kernel(const DenseGemm g) {
   constexpr bool kFast = sizeof(T) == 2;
+  pdl_wait_and_trigger();
   const DenseEpi& ep = g.epi;
   const int64_t per_row = (g.N + V - 1) / V;
   const int64_t total = g.M * per_row;
@@ -104,6 +105,7 @@ dense_dz_kernel(const DzArgs a, bool vec_dy, bool vec_z, bool vec_dz) {
   constexpr int W = Vec16<T>::N;
   constexpr bool kFast = sizeof(T) == 2;
   __shared__ float red[8][32 * W];
+  pdl_wait_and_trigger();
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int64_t col = (static_cast<int64_t>(blockIdx.x) * 32 + tx) * W;
   const int64_t valid = a.N - col;
@@ -148,6 +150,7 @@ template <typename T>
 __global__ void __launch_bounds__(256)
 colsum_finish_kernel(const float* partial, int64_t row_blocks, int64_t N, T* out) {
   __shared__ float red[8][32];
+  pdl_wait_and_trigger();
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int64_t n = blockIdx.x * 32ll + tx;
   float s = 0.f;
@@ -164,13 +167,21 @@ colsum_finish_kernel(const float* partial, int64_t row_blocks, int64_t N, T* out
   }
 }
 
+// 8 elements per thread: scalar reads from anywhere, one 16-byte store
 __global__ void __launch_bounds__(256)
 pad_copy_kernel(const unsigned short* src, int64_t lds, int64_t rows, int64_t cols,
                 unsigned short* dst, int64_t ldd) {
-  const int64_t total = rows * ldd;
-  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
-    const int64_t r = i / ldd, c = i - r * ldd;
-    dst[i] = c < cols ? src[r * lds + c] : 0;
+  pdl_wait_and_trigger();
+  const int units = static_cast<int>(ldd / 8);
+  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
+    const unsigned short* p = src + r * lds;
+    for (int64_t u = threadIdx.x; u < units; u += 256) {
+      uint32_t e[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) e[j] = u * 8 + j < cols ? __ldg(p + u * 8 + j) : 0u;
+      *reinterpret_cast<uint4*>(dst + r * ldd + u * 8) =
+          make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+    }
   }
 }
 
@@ -188,51 +199,49 @@ bool vec_ok(const void* p, int64_t ld) {
 
 cudaError_t launch_dense_finish(int dtype, int epi, const DenseGemm& g, cudaStream_t s) {
   const dim3 grid(blocks_for(g.M * ((g.N + V - 1) / V)), static_cast<unsigned>(g.groups));
+  cudaError_t e;
   if (dtype == kF32) {
-    if (epi == kEpiGated) dense_finish_kernel<float, kEpiGated><<<grid, 256, 0, s>>>(g);
-    else if (epi == kEpiGluBwd) dense_finish_kernel<float, kEpiGluBwd><<<grid, 256, 0, s>>>(g);
-    else dense_finish_kernel<float, kEpiLinear><<<grid, 256, 0, s>>>(g);
+    if (epi == kEpiGated) e = launch_kernel(dense_finish_kernel<float, kEpiGated>, grid, dim3(256), 0, s, g);
+    else if (epi == kEpiGluBwd) e = launch_kernel(dense_finish_kernel<float, kEpiGluBwd>, grid, dim3(256), 0, s, g);
+    else e = launch_kernel(dense_finish_kernel<float, kEpiLinear>, grid, dim3(256), 0, s, g);
   } else {
     using B = __nv_bfloat16;
-    if (epi == kEpiGated) dense_finish_kernel<B, kEpiGated><<<grid, 256, 0, s>>>(g);
-    else if (epi == kEpiGluBwd) dense_finish_kernel<B, kEpiGluBwd><<<grid, 256, 0, s>>>(g);
-    else dense_finish_kernel<B, kEpiLinear><<<grid, 256, 0, s>>>(g);
+    if (epi == kEpiGated) e = launch_kernel(dense_finish_kernel<B, kEpiGated>, grid, dim3(256), 0, s, g);
+    else if (epi == kEpiGluBwd) e = launch_kernel(dense_finish_kernel<B, kEpiGluBwd>, grid, dim3(256), 0, s, g);
+    else e = launch_kernel(dense_finish_kernel<B, kEpiLinear>, grid, dim3(256), 0, s, g);
   }
-  return cudaGetLastError();
+  return e;
 }
 
 cudaError_t launch_dense_dz(int dtype, const DzArgs& a, cudaStream_t s) {
   const int width = 32 * (dtype == kF32 ? 4 : 8);
   const dim3 grid(static_cast<unsigned>((a.N + width - 1) / width),
                   static_cast<unsigned>(a.row_blocks));
+  using B = __nv_bfloat16;
   if (dtype == kF32)
-    dense_dz_kernel<float><<<grid, 256, 0, s>>>(a, vec_ok<float>(a.dy, a.lddy),
-                                                vec_ok<float>(a.z, a.ldz),
-                                                vec_ok<float>(a.dz, a.lddz));
-  else
-    dense_dz_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(a, vec_ok<__nv_bfloat16>(a.dy, a.lddy),
-                                                        vec_ok<__nv_bfloat16>(a.z, a.ldz),
-                                                        vec_ok<__nv_bfloat16>(a.dz, a.lddz));
-  return cudaGetLastError();
+    return launch_kernel(dense_dz_kernel<float>, grid, dim3(256), 0, s, a,
+                         vec_ok<float>(a.dy, a.lddy), vec_ok<float>(a.z, a.ldz),
+                         vec_ok<float>(a.dz, a.lddz));
+  return launch_kernel(dense_dz_kernel<B>, grid, dim3(256), 0, s, a, vec_ok<B>(a.dy, a.lddy),
+                       vec_ok<B>(a.z, a.ldz), vec_ok<B>(a.dz, a.lddz));
 }
 
 cudaError_t launch_colsum_finish(const float* partial, int64_t row_blocks, int64_t N, void* out,
                                  bool out_f32, cudaStream_t s) {
   const unsigned grid = static_cast<unsigned>((N + 31) / 32);
   if (out_f32)
-    colsum_finish_kernel<float><<<grid, 256, 0, s>>>(partial, row_blocks, N, static_cast<float*>(out));
-  else
-    colsum_finish_kernel<__nv_bfloat16>
-        <<<grid, 256, 0, s>>>(partial, row_blocks, N, static_cast<__nv_bfloat16*>(out));
-  return cudaGetLastError();
+    return launch_kernel(colsum_finish_kernel<float>, dim3(grid), dim3(256), 0, s, partial,
+                         row_blocks, N, static_cast<float*>(out));
+  return launch_kernel(colsum_finish_kernel<__nv_bfloat16>, dim3(grid), dim3(256), 0, s, partial,
+                       row_blocks, N, static_cast<__nv_bfloat16*>(out));
 }
 
 cudaError_t launch_pad_copy(const void* src, int64_t lds, int64_t rows, int64_t cols, void* dst,
                             int64_t ldd, cudaStream_t s) {
-  pad_copy_kernel<<<blocks_for(rows * ldd), 256, 0, s>>>(static_cast<const unsigned short*>(src), lds,
-                                                         rows, cols,
-                                                         static_cast<unsigned short*>(dst), ldd);
-  return cudaGetLastError();
+  const unsigned blocks = static_cast<unsigned>(rows < 148 * 16 ? rows : 148 * 16);
+  return launch_kernel(pad_copy_kernel, dim3(blocks), dim3(256), 0, s,
+                       static_cast<const unsigned short*>(src), lds, rows, cols,
+                       static_cast<unsigned short*>(dst), ldd);
 }
 
 }  // namespace vmoe

@@ -9,11 +9,9 @@
 // lane t of a row takes k = 8t..8t+7 and hands them to two MMAs as their (2t, 2t+1, 2t+8,
 // 2t+9) pairs, the same permutation for weights and tokens.  No shared memory or barrier
 // stands between a load and its use; four 32-wide chunks of two weight rows per lane are in
-// flight.  A block owns 16 weight rows, its 8 warps take every eighth chunk and add their
-// sums through shared memory in warp order.  The gated form takes 8 gate rows and 8 up rows
+// flight.  A block owns 16 weight rows, its 8 to 32 warps take its chunks in turn and add
+// their sums through shared memory in warp order.  The gated form takes 8 gate rows and 8 up rows
 // of the same features as the 16, so one thread ends up with both.
-#include <stdlib.h>
-
 #include "common.cuh"
 #include "dense.h"
 #include "dense_act.cuh"
@@ -133,13 +131,16 @@ dense_small_kernel(const SmallGemm g) {
   out[t * ep.ldo + col] = __float2bfloat16_rn(z);
 }
 
+// Warps per block: about four 32-wide chunks each (one batch of loads), so that all of a
+// block's weights are in flight at once; 32 only where the blocks are too few to fill the SMs
+// twice.  One row, cold weights, K x N: 2048 x 2048 7.4 / 4.1 / 4.2 us with 8 / 16 / 32 warps,
+// 8192 x 2048 24.4 / 14.5 / 10.8 us, 2048 x 8192 9.4 / 8.9 / 13.4 us.
 template <int EPI, bool VEC, int NT>
 cudaError_t launch_warps(const SmallGemm& g, unsigned blocks, cudaStream_t s) {
-  static const int forced = getenv("SMALL_WARPS") ? atoi(getenv("SMALL_WARPS")) : 0;
-  int w = forced ? forced : 8;
-  if (w >= 32)
+  const int64_t chunks = (g.K + 31) / 32;
+  if (chunks > 64 && blocks < 2u * static_cast<unsigned>(g.num_sms))
     return launch_kernel(dense_small_kernel<EPI, VEC, NT, 32>, dim3(blocks), dim3(1024), 0, s, g);
-  if (w >= 16)
+  if (chunks > 32)
     return launch_kernel(dense_small_kernel<EPI, VEC, NT, 16>, dim3(blocks), dim3(512), 0, s, g);
   return launch_kernel(dense_small_kernel<EPI, VEC, NT, 8>, dim3(blocks), dim3(256), 0, s, g);
 }
@@ -149,10 +150,105 @@ cudaError_t launch_nt(const SmallGemm& g, unsigned blocks, cudaStream_t s) {
   return g.T <= 8 ? launch_warps<EPI, VEC, 1>(g, blocks, s) : launch_warps<EPI, VEC, 2>(g, blocks, s);
 }
 
+// The fp32 form on the CUDA cores: a block owns 4 output features (gated: 2 gate and 2 up rows),
+// its 8 warps take the k range in turn, a lane 4 consecutive k.  A weight is loaded once and
+// used for all TT tokens, a token's x (from L1) for the 4 rows.
+template <int EPI, bool VEC, int TT>
+__global__ void __launch_bounds__(256)
+dense_small_f32_kernel(const SmallGemm g) {
+  constexpr bool kGate = EPI == kEpiGated;
+  constexpr int FEATURES = kGate ? 2 : 4;
+  __shared__ float red[8][4][TT];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * FEATURES;
+  pdl_wait_and_trigger();
+  const auto* w = static_cast<const float*>(g.w);
+  const auto* w2 = static_cast<const float*>(g.w2);
+  const auto* x = static_cast<const float*>(g.x);
+  const float* row[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t n = n0 + (kGate ? (i & 1) : i);
+    row[i] = n < g.N ? (kGate && i >= 2 ? w2 + n * g.ldw2 : w + n * g.ldw) : nullptr;
+  }
+  auto load4 = [&](const float* p, int64_t k) {
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (!p) return v;
+    if constexpr (VEC) {  // K % 4 == 0 and 16-byte aligned rows
+      if (k < g.K) v = __ldg(reinterpret_cast<const float4*>(p + k));
+    } else {
+      if (k < g.K) v.x = __ldg(p + k);
+      if (k + 1 < g.K) v.y = __ldg(p + k + 1);
+      if (k + 2 < g.K) v.z = __ldg(p + k + 2);
+      if (k + 3 < g.K) v.w = __ldg(p + k + 3);
+    }
+    return v;
+  };
+  float acc[4][TT] = {};
+  for (int64_t k = (warp * 32 + lane) * 4; k < g.K; k += 8 * 128) {
+    float4 a[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = load4(row[i], k);
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
+      const float4 b = load4(t < g.T ? x + t * g.ldx : nullptr, k);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        acc[i][t] += a[i].x * b.x + a[i].y * b.y + a[i].z * b.z + a[i].w * b.w;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
+      float s = acc[i][t];
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+      if (lane == 0) red[warp][i][t] = s;
+    }
+  __syncthreads();
+  const int f = threadIdx.x % FEATURES, t = threadIdx.x / FEATURES;
+  const int64_t col = n0 + f;
+  if (t >= g.T || t >= TT || col >= g.N) return;
+  const DenseEpi& ep = g.epi;
+  auto total = [&](int i, const void* bias) {
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) s += red[k][i][t];
+    return s + (bias ? static_cast<const float*>(bias)[col] : 0.f);
+  };
+  float z = total(f, ep.bias);
+  if (ep.z) static_cast<float*>(ep.z)[t * ep.ldz + col] = z;
+  if constexpr (kGate) {
+    const float up = total(f + 2, ep.bias2);
+    if (ep.z) static_cast<float*>(ep.z2)[t * ep.ldz + col] = up;
+    act_switch(ep.act, [&](auto A) { z = act_value1<decltype(A)::value>(z, ep.gamma) * up; });
+  } else {
+    act_switch(ep.act, [&](auto A) { z = act_value1<decltype(A)::value>(z, ep.gamma); });
+    if (ep.res) z += static_cast<const float*>(ep.res)[t * ep.ldr + col];
+  }
+  static_cast<float*>(ep.out)[t * ep.ldo + col] = z;
+}
+
+template <int EPI, bool VEC>
+cudaError_t launch_f32(const SmallGemm& g, cudaStream_t s) {
+  const int features = EPI == kEpiGated ? 2 : 4;
+  const dim3 grid(static_cast<unsigned>((g.N + features - 1) / features));
+  if (g.T <= 2) return launch_kernel(dense_small_f32_kernel<EPI, VEC, 2>, grid, dim3(256), 0, s, g);
+  if (g.T <= 8) return launch_kernel(dense_small_f32_kernel<EPI, VEC, 8>, grid, dim3(256), 0, s, g);
+  return launch_kernel(dense_small_f32_kernel<EPI, VEC, 16>, grid, dim3(256), 0, s, g);
+}
+
 }  // namespace
 
-cudaError_t launch_dense_small(int epi, const SmallGemm& g, cudaStream_t s) {
-  if (g.T < 1 || g.T > kSmallTokens || g.epi.out_f32) return cudaErrorInvalidValue;
+cudaError_t launch_dense_small(int dtype, int epi, const SmallGemm& g, cudaStream_t s) {
+  if (g.T < 1 || g.T > kSmallTokens) return cudaErrorInvalidValue;
+  if (dtype == kF32) {
+    if (epi == kEpiGated)
+      return g.vec_in ? launch_f32<kEpiGated, true>(g, s) : launch_f32<kEpiGated, false>(g, s);
+    return g.vec_in ? launch_f32<kEpiLinear, true>(g, s) : launch_f32<kEpiLinear, false>(g, s);
+  }
+  if (g.epi.out_f32) return cudaErrorInvalidValue;
   const int rows = epi == kEpiGated ? 8 : 16;
   const unsigned blocks = static_cast<unsigned>((g.N + rows - 1) / rows);
   cudaError_t e;

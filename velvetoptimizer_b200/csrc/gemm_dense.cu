@@ -14,8 +14,9 @@
 // 64-column chunks, stride offset 1 KB between 8-row groups).
 //
 // Extra forms of the k loop and of B:
-//   * two operand pairs (kb1 > 0): dx = dg Wg + du Wu runs as one product whose k blocks come
-//     from (dg, Wg) and then from (du, Wu), in one accumulator;
+//   * several operand pairs (segs): dx = dg Wg + du Wu runs as one product whose k blocks come
+//     from (dg, Wg) and then from (du, Wu), in one accumulator; an fp32 product as six pairs of
+//     its operands' bf16 planes (dense_f32.cu);
 //   * kEpiGated: the leader's half of B is 128 gate rows and the follower's 128 up rows of the
 //     same features, so a row's gate and up values meet in the epilogue;
 //   * groups: two A operands against one B (the gate's and the up's weight gradients);
@@ -123,7 +124,7 @@ __device__ __forceinline__ Item item_of(const DenseGemm& a, int item) {
     w.n = full * a.band + r % width;
   }
   w.kb = split * a.kb_per_split;
-  w.ke = min(w.kb + a.kb_per_split, a.kb0 + a.kb1);
+  w.ke = min(w.kb + a.kb_per_split, a.segs * a.kbs);
   return w;
 }
 
@@ -324,8 +325,8 @@ gemm_dense_kernel(const __grid_constant__ DenseMaps maps, const __grid_constant_
     mbar_init(smem_u32(&sh->done), 1);
     sh->abort = 0;
     fence_mbar_init();
-    prefetch_tmap(&maps.a0);
-    prefetch_tmap(&maps.b0);
+    prefetch_tmap(&maps.a[0]);
+    prefetch_tmap(&maps.b[0]);
   }
   cluster_sync_all();  // both CTAs' barriers exist before any cross-CTA arrive or copy
   if (warp == 1) tmem_alloc_pair(smem_u32(&sh->tmem_base), TMEM_COLS);
@@ -333,6 +334,7 @@ gemm_dense_kernel(const __grid_constant__ DenseMaps maps, const __grid_constant_
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sh->tmem_base;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // nothing above touches global memory
   const int total = args.groups * args.m_tiles * args.n_tiles * args.splits;
   const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
 
@@ -345,6 +347,11 @@ gemm_dense_kernel(const __grid_constant__ DenseMaps maps, const __grid_constant_
         const int a_at = w.m * PAIR_M + static_cast<int>(rank) * 128;
         // gated: this CTA's 128 rows are gate (leader) or up (follower) rows of one weight each
         const int b_at = EPI == kEpiGated ? w.n * 128 : w.n * BN + static_cast<int>(rank) * 128;
+        // one row of tiles: every pair reads other weights, and pairs that went through k in
+        // step would ask for the same columns of far rows at the same time
+        int at = w.kb;
+        if (args.m_tiles == 1) at += (w.n * 5) % (w.ke - w.kb);
+        int seg = at / args.kbs, kk = at - seg * args.kbs;
         bool ok = true;
         for (int kb = w.kb; kb < w.ke; ++kb, ++it) {
           const int s = it % STAGES;
@@ -355,11 +362,17 @@ gemm_dense_kernel(const __grid_constant__ DenseMaps maps, const __grid_constant_
             break;
           }
           if (aborted(sh)) { ok = false; break; }
-          const bool second = kb >= args.kb0;
-          const int k0 = (second ? kb - args.kb0 : kb) * BK;
-          const CUtensorMap* am = (second || w.g) ? &maps.a1 : &maps.a0;
-          const CUtensorMap* bm =
-              (second || (EPI == kEpiGated && !leader)) ? &maps.b1 : &maps.b0;
+          const int k0 = kk * BK;
+          const CUtensorMap* am = &maps.a[args.seg_a[seg] + w.g * args.group_a];
+          const CUtensorMap* bm = &maps.b[args.seg_b[seg] + (leader ? 0 : args.follower_b)];
+          if (++at == w.ke) {
+            at = w.kb;
+            seg = at / args.kbs;
+            kk = at - seg * args.kbs;
+          } else if (++kk == args.kbs) {
+            kk = 0;
+            ++seg;
+          }
           const uint32_t fb = smem_u32(&sh->full[s]);
           if (leader) mbar_arrive_expect_tx(fb, 2 * STAGE_BYTES);
           const uint32_t fb_leader = mapa_shared(fb, 0);
@@ -379,6 +392,8 @@ gemm_dense_kernel(const __grid_constant__ DenseMaps maps, const __grid_constant_
         }
         if (!ok) break;
       }
+      // the kernel after this one may come up while the last tiles are multiplied and stored
+      asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     }
   } else if (warp == 1) {
     // ---------------- MMA issuer (leader only) ----------------
@@ -632,10 +647,13 @@ cudaError_t launch(const DenseMaps& maps, const DenseGemm& g, int num_sms, cudaS
                                          static_cast<int>(SMEM_BYTES));
   if (err != cudaSuccess) return err;
   const int64_t work = static_cast<int64_t>(g.groups) * g.m_tiles * g.n_tiles * g.splits;
-  if (work < 1 || work > 0x7fffffff || g.band < 1 || g.kb_per_split < 1)
+  if (work < 1 || work > 0x7fffffff || g.band < 1 || g.kb_per_split < 1 || g.kbs < 1 ||
+      g.segs < 1 || g.segs > 12)
     return cudaErrorInvalidValue;
   cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2;
   attr[0].val.clusterDim.y = 1;
@@ -662,6 +680,7 @@ cudaError_t launch(const DenseMaps& maps, const DenseGemm& g, int num_sms, cudaS
   if (pairs > max_pairs) pairs = max_pairs;
   if (pairs > work) pairs = work;
   cfg.gridDim = dim3(static_cast<unsigned>(2 * pairs), 1, 1);
+  cfg.numAttrs = g_launch_pdl ? 2 : 1;
   err = cudaLaunchKernelEx(&cfg, kern, maps, g);
   return err != cudaSuccess ? err : cudaGetLastError();
 }
@@ -670,8 +689,9 @@ cudaError_t launch(const DenseMaps& maps, const DenseGemm& g, int num_sms, cudaS
 
 cudaError_t launch_gemm_dense(bool a_mn, bool b_mn, int epi, const DenseMaps& maps,
                               const DenseGemm& g, int num_sms, cudaStream_t s) {
-  if (g.splits > 1) {
-    if (!g.partial || g.ldp % 4) return cudaErrorInvalidValue;
+  if (g.splits > 1 && !g.partial) return cudaErrorInvalidValue;
+  if (g.partial) {
+    if (g.ldp % 4) return cudaErrorInvalidValue;
     if (!a_mn && !b_mn)
       return epi == kEpiGated ? launch<false, false, kEpiGated, true>(maps, g, num_sms, s)
                               : launch<false, false, kEpiLinear, true>(maps, g, num_sms, s);
