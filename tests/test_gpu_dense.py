@@ -517,6 +517,19 @@ def test_changed_input_is_noticed():
         y.sum().backward()
 
 
+def test_backward_twice():
+    import velvetoptimizer_b200 as vb
+    x = torch.randn(20, 16, device="cuda", dtype=BF16).requires_grad_()
+    ws = [torch.randn(s, device="cuda", dtype=BF16).requires_grad_() for s in ((24, 16), (24, 16), (16, 24))]
+    for y, ps in ((vb.linear(x, ws[0], activation="silu"), (x, ws[0])), (vb.gated_ffn(x, *ws), (x, *ws))):
+        dy = torch.randn_like(y)
+        a = torch.autograd.grad(y, ps, dy, retain_graph=True)
+        b = torch.autograd.grad(y, ps, dy)
+        assert all(torch.equal(u, v) for u, v in zip(a, b))
+        with pytest.raises(RuntimeError, match="second time"):
+            torch.autograd.grad(y, ps, dy)
+
+
 def test_first_call_of_a_thread_inside_a_capture():
     """A new thread's first call makes its context: nothing in that may disturb a capture."""
     import threading

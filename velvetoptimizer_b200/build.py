@@ -93,7 +93,7 @@ def build_host_module(name: str, force: bool = False, verbose: bool = False) -> 
            src, "-o", out + ".tmp", "-L", os.path.join(tdir, "lib"),
            "-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_python"]
     if name == "dense_ops":  # calls the C ABI library beside it
-        cmd += ["-lc10_cuda", LIB, "-Wl,-rpath,$ORIGIN"]
+        cmd += ["-lc10_cuda", "-ltorch_cuda", LIB, "-Wl,-rpath,$ORIGIN"]
     cmd += [f"-Wl,-rpath,{os.path.join(tdir, 'lib')}"]
     os.makedirs(LIB_DIR, exist_ok=True)
     if verbose:

@@ -6,7 +6,11 @@
 
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <ATen/cuda/EmptyTensor.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 
 #include <array>
 
@@ -15,7 +19,6 @@
 namespace {
 
 using at::Tensor;
-using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 using OptTensor = std::optional<Tensor>;
 
@@ -88,13 +91,18 @@ Tensor packed(const Tensor& t) {
 
 const void* ptr(const OptTensor& t) { return t && t->defined() ? t->data_ptr() : nullptr; }
 
+// An uninitialised CUDA tensor, past the dispatcher
+Tensor fresh(at::IntArrayRef shape, const at::TensorOptions& like) {
+  return at::detail::empty_cuda(shape, like);
+}
+
 struct Workspace {
   Tensor t;
   void* p = nullptr;
   size_t n = 0;
   Workspace(size_t bytes, const Tensor& like) {
     if (bytes == 0) return;
-    t = at::empty({static_cast<int64_t>(bytes)}, like.options().dtype(at::kByte));
+    t = fresh({static_cast<int64_t>(bytes)}, like.options().dtype(at::kByte));
     p = t.data_ptr();
     n = bytes;
   }
@@ -126,8 +134,8 @@ std::tuple<Tensor, Tensor> linear_forward(const Tensor& x_in, const Tensor& w_in
   d.dtype = d.grad_dtype = dtype_of(x.scalar_type());
   d.activation = static_cast<int32_t>(act);
   d.gamma = static_cast<float>(gamma);
-  Tensor y = at::empty({d.tokens, d.out_features}, x.options());
-  Tensor z = keep ? at::empty({d.tokens, d.out_features}, x.options()) : at::empty({0}, x.options());
+  Tensor y = fresh({d.tokens, d.out_features}, x.options());
+  Tensor z = keep ? fresh({d.tokens, d.out_features}, x.options()) : fresh({0}, x.options());
   size_t need = 0;
   check(o, vmoe_linear_workspace_size(o, &d, 0, &need), "vmoe_linear_workspace_size");
   const Workspace ws(need, x);
@@ -158,9 +166,9 @@ std::tuple<Tensor, Tensor, Tensor> linear_backward(const Tensor& x_in, const Ten
   d.grad_dtype = grad_f32 ? VMOE_F32 : d.dtype;
   const auto xo = x.options();
   const auto go = grad_f32 ? xo.dtype(at::kFloat) : xo;
-  Tensor dx = want[0] ? at::empty({d.tokens, d.in_features}, xo) : at::empty({0}, xo);
-  Tensor dw = want[1] ? at::empty({d.out_features, d.in_features}, go) : at::empty({0}, go);
-  Tensor db = want[2] ? at::empty({d.out_features}, go) : at::empty({0}, go);
+  Tensor dx = want[0] ? fresh({d.tokens, d.in_features}, xo) : fresh({0}, xo);
+  Tensor dw = want[1] ? fresh({d.out_features, d.in_features}, go) : fresh({0}, go);
+  Tensor db = want[2] ? fresh({d.out_features}, go) : fresh({0}, go);
   size_t need = 0;
   check(o, vmoe_linear_workspace_size(o, &d, 1, &need), "vmoe_linear_workspace_size");
   const Workspace ws(need, x);
@@ -203,9 +211,9 @@ std::tuple<Tensor, Tensor> gated_ffn_forward(const Tensor& x_in, const Tensor& g
   size_t need = 0, saved_bytes = 0;
   check(o, vmoe_gated_ffn_workspace_size(o, &d, 0, &need, &saved_bytes),
         "vmoe_gated_ffn_workspace_size");
-  Tensor y = at::empty({d.tokens, d.hidden}, x.options());
-  Tensor saved = at::empty({keep ? static_cast<int64_t>(saved_bytes) : 0},
-                           x.options().dtype(at::kByte));
+  Tensor y = fresh({d.tokens, d.hidden}, x.options());
+  Tensor saved = fresh({keep ? static_cast<int64_t>(saved_bytes) : 0},
+                       x.options().dtype(at::kByte));
   const Workspace ws(need, x);
   const bool kept = saved.numel() > 0;
   check(o,
@@ -237,7 +245,7 @@ std::array<Tensor, 7> gated_ffn_backward_array(const Tensor& x_in, const Tensor&
   const auto xo = x.options();
   const auto go = grad_f32 ? xo.dtype(at::kFloat) : xo;
   for (size_t i = 0; i < 7; ++i) {
-    out[i] = want[i] ? at::empty(shapes[i], i ? go : xo) : at::empty({0}, i ? go : xo);
+    out[i] = want[i] ? fresh(shapes[i], i ? go : xo) : fresh({0}, i ? go : xo);
     p[i] = want[i] ? out[i].data_ptr() : nullptr;
   }
   const vmoe_ffn_grads g{p[1], p[2], p[3], p[4], p[5], p[6]};
@@ -261,16 +269,11 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> gated_ffn_bac
 }
 
 // ---- autograd -----------------------------------------------------------------------------
+using torch::autograd::SavedVariable;
+
 OptTensor cast(const OptTensor& p, const Tensor& x) {
   return p && p->defined() ? OptTensor(p->to(x.scalar_type())) : std::nullopt;
 }
-
-// Which of `n` optional inputs the running backward needs (absent ones have no edge).
-struct Needs {
-  AutogradContext* ctx;
-  size_t edge = 0;
-  bool next(bool present) { return present && ctx->needs_input_grad(edge++); }
-};
 
 // The gradients have no gradient: differentiating through them raises.
 variable_list once(variable_list grads) {
@@ -289,45 +292,48 @@ variable_list once(variable_list grads) {
   return grads;
 }
 
-Tensor to_param(const Tensor& g, int64_t type) {
-  return g.to(static_cast<at::ScalarType>(type));
+Tensor to_param(const Tensor& g, at::ScalarType type) {
+  return g.scalar_type() == type ? g : g.to(type);
 }
 
-struct LinearFn : public torch::autograd::Function<LinearFn> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight,
-                        const OptTensor& bias, const OptTensor& residual, int64_t act,
-                        double gamma) {
-    const Tensor w = weight.to(x.scalar_type());
-    const bool has_b = bias && bias->defined(), has_r = residual && residual->defined();
-    const bool keep = act != VMOE_ACT_NONE && (x.requires_grad() || weight.requires_grad() ||
-                                               (has_b && bias->requires_grad()));
-    auto [y, z] = linear_forward(x, w, cast(bias, x), residual, act, gamma, keep);
-    ctx->save_for_backward({x, w, z});
-    ctx->saved_data["args"] = std::tuple<int64_t, double>(act, gamma);
-    ctx->saved_data["types"] = std::vector<int64_t>{
-        static_cast<int64_t>(weight.scalar_type()),
-        static_cast<int64_t>(has_b ? bias->scalar_type() : weight.scalar_type()), has_b, has_r};
-    return y;
-  }
+// A node with its inputs' edges in the order of `inputs` (absent ones have an empty edge).
+template <typename N>
+std::shared_ptr<N> make_node(std::initializer_list<const OptTensor*> inputs) {
+  std::shared_ptr<N> node(new N(), torch::autograd::deleteNode);
+  torch::autograd::edge_list edges;
+  edges.reserve(inputs.size());
+  for (const OptTensor* t : inputs)
+    edges.push_back(*t && (*t)->defined() ? torch::autograd::impl::gradient_edge(**t)
+                                          : torch::autograd::Edge());
+  node->set_next_edges(std::move(edges));
+  return node;
+}
 
-  static variable_list backward(AutogradContext* ctx, variable_list dys) {
-    const auto saved = ctx->get_saved_variables();
-    const auto types = ctx->saved_data["types"].toIntVector();
-    const auto args = ctx->saved_data["args"].toTuple();
-    Needs needs{ctx};
-    const bool nx = needs.next(true), nw = needs.next(true), nb = needs.next(types[2]),
-               nr = needs.next(types[3]);
-    variable_list out(6);
+struct LinearBackward : public torch::autograd::Node {
+  SavedVariable x, w, z;
+  int64_t act = 0;
+  double gamma = 0;
+  at::ScalarType w_type = at::kFloat, b_type = at::kFloat;
+
+  std::string name() const override { return "VesperLinearBackward"; }
+  void release_variables() override {
+    x.reset_data();
+    w.reset_data();
+    z.reset_data();
+  }
+  variable_list apply(variable_list&& dys) override {
+    variable_list out(4);
+    if (!dys[0].defined()) return out;
+    const bool nx = task_should_compute_output(0), nw = task_should_compute_output(1),
+               nb = task_should_compute_output(2), nr = task_should_compute_output(3);
     if (nx || nw || nb) {
-      at::NoGradGuard no_grad;
-      const bool f32 = types[0] == static_cast<int64_t>(at::kFloat) ||
-                       types[1] == static_cast<int64_t>(at::kFloat);
-      auto [dx, dw, db] = linear_backward(
-          saved[0], saved[1], saved[2], dys[0], args->elements()[0].toInt(),
-          args->elements()[1].toDouble(), {nx, nw, nb}, f32);
+      const Tensor xs = x.unpack(), ws = w.unpack(), zs = z.unpack();
+      at::AutoGradMode no_grad(false);
+      auto [dx, dw, db] = linear_backward(xs, ws, zs, dys[0], act, gamma, {nx, nw, nb},
+                                          w_type == at::kFloat || b_type == at::kFloat);
       if (nx) out[0] = dx;
-      if (nw) out[1] = to_param(dw, types[0]);
-      if (nb) out[2] = to_param(db, types[1]);
+      if (nw) out[1] = to_param(dw, w_type);
+      if (nb) out[2] = to_param(db, b_type);
     }
     out = once(std::move(out));
     if (nr) out[3] = dys[0];
@@ -335,48 +341,29 @@ struct LinearFn : public torch::autograd::Function<LinearFn> {
   }
 };
 
-struct GatedFfnFn : public torch::autograd::Function<GatedFfnFn> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& gate_w,
-                        const Tensor& up_w, const Tensor& down_w, const OptTensor& gate_b,
-                        const OptTensor& up_b, const OptTensor& down_b, const OptTensor& residual,
-                        int64_t act, double gamma) {
-    const std::array<OptTensor, 6> params{gate_w, up_w, down_w, gate_b, up_b, down_b};
-    bool keep = x.requires_grad(), f32 = false;
-    std::vector<int64_t> types;
-    for (const auto& p : params) {
-      const bool has = p && p->defined();
-      keep = keep || (has && p->requires_grad());
-      f32 = f32 || (has && p->scalar_type() == at::kFloat);
-      types.push_back(has ? static_cast<int64_t>(p->scalar_type()) : -1);
-    }
-    types.push_back(residual && residual->defined());
-    types.push_back(f32);
-    const Tensor wg = gate_w.to(x.scalar_type()), wu = up_w.to(x.scalar_type()),
-                 wd = down_w.to(x.scalar_type());
-    auto [y, saved] = gated_ffn_forward(x, wg, wu, wd, cast(gate_b, x), cast(up_b, x),
-                                        cast(down_b, x), residual, act, gamma, keep);
-    ctx->save_for_backward({x, wg, wu, wd, saved});
-    ctx->saved_data["args"] = std::tuple<int64_t, double>(act, gamma);
-    ctx->saved_data["types"] = types;
-    return y;
-  }
+struct GatedFfnBackward : public torch::autograd::Node {
+  SavedVariable x, wg, wu, wd, saved;
+  int64_t act = 0;
+  double gamma = 0;
+  std::array<at::ScalarType, 6> types{};
+  bool f32 = false;
 
-  static variable_list backward(AutogradContext* ctx, variable_list dys) {
-    const auto saved = ctx->get_saved_variables();
-    const auto types = ctx->saved_data["types"].toIntVector();
-    const auto args = ctx->saved_data["args"].toTuple();
-    Needs needs{ctx};
-    std::vector<bool> want{needs.next(true)};
-    for (size_t i = 0; i < 6; ++i) want.push_back(needs.next(types[i] >= 0));
-    const bool nr = needs.next(types[6]);
-    variable_list out(10);
+  std::string name() const override { return "VesperGatedFfnBackward"; }
+  void release_variables() override {
+    for (SavedVariable* v : {&x, &wg, &wu, &wd, &saved}) v->reset_data();
+  }
+  variable_list apply(variable_list&& dys) override {
+    variable_list out(8);
+    if (!dys[0].defined()) return out;
+    std::vector<bool> want(7);
     bool any = false;
-    for (const bool b : want) any = any || b;
+    for (size_t i = 0; i < 7; ++i) any |= (want[i] = task_should_compute_output(i));
+    const bool nr = task_should_compute_output(7);
     if (any) {
-      at::NoGradGuard no_grad;
-      auto got = gated_ffn_backward_array(saved[0], saved[1], saved[2], saved[3], saved[4], dys[0],
-                                          args->elements()[0].toInt(),
-                                          args->elements()[1].toDouble(), want, types[7]);
+      const Tensor xs = x.unpack(), g = wg.unpack(), u = wu.unpack(), d = wd.unpack(),
+                   s = saved.unpack();
+      at::AutoGradMode no_grad(false);
+      auto got = gated_ffn_backward_array(xs, g, u, d, s, dys[0], act, gamma, want, f32);
       for (size_t i = 0; i < 7; ++i)
         if (want[i]) out[i] = i ? to_param(got[i], types[i - 1]) : got[i];
     }
@@ -385,6 +372,65 @@ struct GatedFfnFn : public torch::autograd::Function<GatedFfnFn> {
     return out;
   }
 };
+
+bool wants(const OptTensor& t) { return t && t->defined() && t->requires_grad(); }
+
+Tensor linear_autograd(const Tensor& x, const Tensor& weight, const OptTensor& bias,
+                       const OptTensor& residual, int64_t act, double gamma) {
+  const OptTensor ox(x), ow(weight);
+  auto node = make_node<LinearBackward>({&ox, &ow, &bias, &residual});
+  Tensor y;
+  {
+    at::AutoGradMode no_grad(false);
+    const Tensor w = weight.to(x.scalar_type());
+    const bool keep = act != VMOE_ACT_NONE && (wants(ox) || wants(ow) || wants(bias));
+    auto [out, z] = linear_forward(x, w, cast(bias, x), residual, act, gamma, keep);
+    y = out;
+    node->x = SavedVariable(x, false);
+    node->w = SavedVariable(w, false);
+    node->z = SavedVariable(z, false);
+  }
+  node->act = act;
+  node->gamma = gamma;
+  node->w_type = weight.scalar_type();
+  node->b_type = bias && bias->defined() ? bias->scalar_type() : weight.scalar_type();
+  torch::autograd::set_history(y, node);
+  return y;
+}
+
+Tensor gated_ffn_autograd(const Tensor& x, const Tensor& gate_w, const Tensor& up_w,
+                          const Tensor& down_w, const OptTensor& gate_b, const OptTensor& up_b,
+                          const OptTensor& down_b, const OptTensor& residual, int64_t act,
+                          double gamma) {
+  const OptTensor ox(x), og(gate_w), ou(up_w), od(down_w);
+  auto node = make_node<GatedFfnBackward>({&ox, &og, &ou, &od, &gate_b, &up_b, &down_b, &residual});
+  bool keep = wants(ox);
+  size_t i = 0;
+  for (const OptTensor* p : {&og, &ou, &od, &gate_b, &up_b, &down_b}) {
+    const bool has = *p && (*p)->defined();
+    keep = keep || wants(*p);
+    node->f32 = node->f32 || (has && (*p)->scalar_type() == at::kFloat);
+    node->types[i++] = has ? (*p)->scalar_type() : x.scalar_type();
+  }
+  Tensor y;
+  {
+    at::AutoGradMode no_grad(false);
+    const auto t = x.scalar_type();
+    const Tensor wg = gate_w.to(t), wu = up_w.to(t), wd = down_w.to(t);
+    auto [out, saved] = gated_ffn_forward(x, wg, wu, wd, cast(gate_b, x), cast(up_b, x),
+                                          cast(down_b, x), residual, act, gamma, keep);
+    y = out;
+    node->x = SavedVariable(x, false);
+    node->wg = SavedVariable(wg, false);
+    node->wu = SavedVariable(wu, false);
+    node->wd = SavedVariable(wd, false);
+    node->saved = SavedVariable(saved, false);
+  }
+  node->act = act;
+  node->gamma = gamma;
+  torch::autograd::set_history(y, node);
+  return y;
+}
 
 // ---- the operators ------------------------------------------------------------------------
 void check_x(const char* name, const Tensor& x) {
@@ -420,8 +466,6 @@ Tensor flat(const Tensor& t) {
   return t.dim() == 2 ? t : t.reshape({t.numel() / t.size(-1), t.size(-1)});
 }
 
-bool wants(const OptTensor& t) { return t && t->defined() && t->requires_grad(); }
-
 Tensor linear(const Tensor& x, const Tensor& weight, const OptTensor& bias,
               const OptTensor& residual, int64_t act, double gamma) {
   check_x("linear", x);
@@ -438,7 +482,7 @@ Tensor linear(const Tensor& x, const Tensor& weight, const OptTensor& bias,
   const Tensor x2 = flat(x);
   Tensor y;
   if (at::GradMode::is_enabled() && (wants(x) || wants(weight) || wants(bias) || wants(residual))) {
-    y = LinearFn::apply(x2, weight, bias, r, act, gamma);
+    y = linear_autograd(x2, weight, bias, r, act, gamma);
   } else {
     at::NoGradGuard no_grad;
     y = std::get<0>(linear_forward(x2, weight.to(x.scalar_type()), cast(bias, x), r, act, gamma, false));
@@ -469,7 +513,7 @@ Tensor gated_ffn(const Tensor& x, const Tensor& gate_w, const Tensor& up_w, cons
   if (at::GradMode::is_enabled() &&
       (wants(x) || wants(gate_w) || wants(up_w) || wants(down_w) || wants(gate_b) || wants(up_b) ||
        wants(down_b) || wants(residual))) {
-    y = GatedFfnFn::apply(x2, gate_w, up_w, down_w, gate_b, up_b, down_b, r, act, gamma);
+    y = gated_ffn_autograd(x2, gate_w, up_w, down_w, gate_b, up_b, down_b, r, act, gamma);
   } else {
     at::NoGradGuard no_grad;
     const auto t = x.scalar_type();
