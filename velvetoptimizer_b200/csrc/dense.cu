@@ -440,6 +440,7 @@ int linear_forward(Call& c, const vmoe_linear& d, const LinearPtrs& p) {
     g.K = K;
     g.epi = e;
     g.num_sms = c.o->num_sms;
+    g.status = c.o->status;
     g.vec_in = K * elt % 16 == 0 && pitch16(p.x, d.ldx, elt) && pitch16(p.w, d.ldw, elt);
     return c.run([&] { return launch_dense_small(d.dtype, kEpiLinear, g, c.s); }, "linear");
   }
@@ -595,6 +596,7 @@ int ffn_forward(Call& c, const vmoe_gated_ffn& d, const FfnPtrs& p) {
     g.K = H;
     g.epi = e1;
     g.num_sms = c.o->num_sms;
+    g.status = c.o->status;
     g.vec_in = H * elt % 16 == 0 && pitch16(p.x, d.ldx, elt) && aligned16(p.w.gate_w) &&
                aligned16(p.w.up_w);
     TRY(c.run([&] { return launch_dense_small(d.dtype, kEpiGated, g, c.s); }, "gate|up"));
@@ -608,6 +610,8 @@ int ffn_forward(Call& c, const vmoe_gated_ffn& d, const FfnPtrs& p) {
     q.K = I;
     q.epi = e2;
     q.num_sms = c.o->num_sms;
+    q.status = c.o->status;
+    q.early_weights = 1;
     q.vec_in = I * elt % 16 == 0 && aligned16(p.w.down_w);
     return c.run([&] { return launch_dense_small(d.dtype, kEpiLinear, q, c.s); }, "down");
   }

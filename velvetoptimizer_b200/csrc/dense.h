@@ -115,7 +115,10 @@ struct SmallGemm {
   DenseEpi epi;
   int vec_in;  // x and the weights allow 16-byte loads
   int num_sms;
+  int* status;
+  int early_weights;  // the weights may be read before the kernel ahead has ended
 };
+cudaError_t launch_dense_stream(int epi, const SmallGemm& g, cudaStream_t s);  // dense_stream.cu
 cudaError_t launch_dense_small(int dtype, int epi, const SmallGemm& g, cudaStream_t s);
 
 // A decode batch (at most kSkinnyTokens rows): weights as the MMA's M operand, k divided over a

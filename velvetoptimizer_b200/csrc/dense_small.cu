@@ -250,6 +250,13 @@ cudaError_t launch_dense_small(int dtype, int epi, const SmallGemm& g, cudaStrea
   }
   if (g.epi.out_f32) return cudaErrorInvalidValue;
   const int rows = epi == kEpiGated ? 8 : 16;
+  // Persistent blocks that copy ahead (dense_stream.cu) pay where a block has several tiles or
+  // several slices of k to hide the waits between, and where two token groups make the
+  // register form's loads too few.  One row, cold weights, register / stream form: 8192 x 2048
+  // 10.9 / 9.9 us, gate|up of 2048 x 8192 14.8 / 13.3 us, but 2048 x 8192 8.9 / 9.6 us and
+  // 2048 x 2048 4.1 / 4.8 us; 16 rows: 2048 x 8192 13.0 / 11.3 us, 2048 x 2048 6.4 / 5.4 us.
+  if (g.vec_in && (g.K > 2048 || (g.N + rows - 1) / rows >= 6 * g.num_sms || (g.T > 8 && g.K > 1024)))
+    return launch_dense_stream(epi, g, s);
   const unsigned blocks = static_cast<unsigned>((g.N + rows - 1) / rows);
   cudaError_t e;
   if (epi == kEpiGated)
