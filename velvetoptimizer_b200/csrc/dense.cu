@@ -181,7 +181,10 @@ int run_product(Call& c, const Product& p) {
 }
 
 // The same for a decode batch's forward: x [T, K] and weights [N, K] (gated: two of them).
-int run_skinny(Call& c, int epi, Mat x, Mat w, Mat w2, const DenseEpi& e, const char* what) {
+int run_skinny(Call& c, int epi, Mat x, Mat w, Mat w2, const DenseEpi& e, const char* what,
+               bool second = false) {
+  // a second product's weights may be asked for early, unless they are copied just before
+  const bool early = second && w.ld % 8 == 0;
   TRY(c.tma_ready(x, what));
   TRY(c.tma_ready(w, what));
   if (epi == kEpiGated) TRY(c.tma_ready(w2, what));
@@ -203,6 +206,7 @@ int run_skinny(Call& c, int epi, Mat x, Mat w, Mat w2, const DenseEpi& e, const 
   g.kbs = static_cast<int>((x.cols + 63) / 64);
   g.epi = e;
   g.status = c.o->status;
+  g.early_weights = early;
   return c.run([&] { return launch_dense_skinny(epi, mw, mw2, mx, g, c.s); }, what);
 }
 
@@ -618,7 +622,7 @@ int ffn_forward(Call& c, const vmoe_gated_ffn& d, const FfnPtrs& p) {
   if (d.dtype == VMOE_BF16 && T <= kSkinnyTokens) {
     TRY(run_skinny(c, kEpiGated, {p.x, T, H, d.ldx}, {p.w.gate_w, I, H, H}, {p.w.up_w, I, H, H}, e1,
                    "gate|up"));
-    return run_skinny(c, kEpiLinear, {h, T, I, sv.ld}, {p.w.down_w, H, I, I}, {}, e2, "down");
+    return run_skinny(c, kEpiLinear, {h, T, I, sv.ld}, {p.w.down_w, H, I, I}, {}, e2, "down", true);
   }
   c.overlap = d.dtype == VMOE_F32;
   Product g, q;

@@ -130,6 +130,7 @@ struct SkinnyGemm {
   int kbs;  // 64-wide k blocks
   DenseEpi epi;
   int* status;
+  int early_weights;  // as SmallGemm's
   // set by the launcher
   int t_pad, parts, kb_per_part, stages;
   uint32_t tmem_cols, ring_bytes, exchange_bytes;

@@ -87,29 +87,40 @@ dense_skinny_kernel(const __grid_constant__ CUtensorMap w_map,
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sh->tmem_base;
-  pdl_wait_and_trigger();
+  // in a call's second kernel the weights were there before its first began: the producer asks
+  // for them, as far as the ring goes, before it waits for the tokens
+  const bool early = g.early_weights && warp == 0;
+  if (!early) pdl_wait_and_trigger();
   // the others' stores into this CTA's exchange wait for this (at the end of the main loop)
   if (parts > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 
   if (warp == 0) {
     if (lane == 0) {
-      int it = 0;
-      for (int kb = kb0; kb < kb1; ++kb, ++it) {
-        const int s = it % g.stages;
-        const uint32_t ph = (it / g.stages) & 1;
-        if (!mbar_wait(smem_u32(&sh->empty[s]), ph ^ 1)) {
-          set_abort(sh, g.status, kStatusTimeoutProducer);
-          break;
-        }
-        if (aborted(sh)) break;
-        const uint32_t fb = smem_u32(&sh->full[s]);
-        const uint32_t dst = base + s * stage_bytes;
+      auto weights = [&](int kb, uint32_t fb, uint32_t dst) {
         mbar_arrive_expect_tx(fb, stage_bytes);
         if constexpr (kGate) {
           tma_load_2d(dst, &w_map, fb, kb * BK, tile * 64);
           tma_load_2d(dst + W_BYTES / 2, &w2_map, fb, kb * BK, tile * 64);
         } else {
           tma_load_2d(dst, &w_map, fb, kb * BK, tile * 128);
+        }
+      };
+      const int ahead = early ? min(g.stages, kb1 - kb0) : 0;
+      for (int i = 0; i < ahead; ++i)
+        weights(kb0 + i, smem_u32(&sh->full[i]), base + i * stage_bytes);
+      if (early) pdl_wait_and_trigger();
+      int it = 0;
+      for (int kb = kb0; kb < kb1; ++kb, ++it) {
+        const int s = it % g.stages;
+        const uint32_t fb = smem_u32(&sh->full[s]), dst = base + s * stage_bytes;
+        if (it >= ahead) {
+          const uint32_t ph = (it / g.stages) & 1;
+          if (!mbar_wait(smem_u32(&sh->empty[s]), ph ^ 1)) {
+            set_abort(sh, g.status, kStatusTimeoutProducer);
+            break;
+          }
+          if (aborted(sh)) break;
+          weights(kb, fb, dst);
         }
         tma_load_2d(dst + W_BYTES, &x_map, fb, kb * BK, 0);
       }
@@ -144,6 +155,17 @@ dense_skinny_kernel(const __grid_constant__ CUtensorMap w_map,
     }
     __syncwarp();
   }
+  // an epilogue thread's feature, and its biases before the product is done
+  const int f = static_cast<int>(threadIdx.x - 64) % FEATURES;
+  const int group = static_cast<int>(threadIdx.x - 64) / FEATURES;
+  const int64_t col = static_cast<int64_t>(tile) * FEATURES + f;
+  const DenseEpi& ep = g.epi;
+  auto bias = [&](const void* p) {
+    return warp >= 2 && p && col < g.N
+               ? __bfloat162float(static_cast<const __nv_bfloat16*>(p)[col])
+               : 0.f;
+  };
+  const float b0 = bias(ep.bias), b1 = kGate ? bias(ep.bias2) : 0.f;
   // every thread: the product is complete (all copies landed, all stages read)
   if (!mbar_wait(smem_u32(&sh->done), 0)) set_abort(sh, g.status, kStatusTimeoutDrain);
   __syncwarp();
@@ -179,13 +201,6 @@ dense_skinny_kernel(const __grid_constant__ CUtensorMap w_map,
   if (warp >= 2) {
     // a thread per feature: PER of a chunk's 16 tokens, GROUPS apart
     constexpr int GROUPS = 32 * EPI_WARPS / FEATURES, PER = 16 / GROUPS;
-    const int f = (threadIdx.x - 64) % FEATURES, group = (threadIdx.x - 64) / FEATURES;
-    const int64_t col = static_cast<int64_t>(tile) * FEATURES + f;
-    const DenseEpi& ep = g.epi;
-    auto bias = [&](const void* p) {
-      return p && col < g.N ? __bfloat162float(static_cast<const __nv_bfloat16*>(p)[col]) : 0.f;
-    };
-    const float b0 = bias(ep.bias), b1 = kGate ? bias(ep.bias2) : 0.f;
     act_switch(ep.act, [&](auto A) {
 #pragma unroll 1
       for (int c = rank, slot = 0; c < chunks; c += parts, ++slot) {

@@ -73,6 +73,17 @@ dense_small_kernel(const SmallGemm g) {
 #pragma unroll
   for (int n = 0; n < NT; ++n) xr[n] = n * 8 + gid < g.T ? x + (n * 8 + gid) * g.ldx : nullptr;
 
+  // this thread's output, and what its epilogue reads, asked for with the weights
+  const DenseEpi& ep = g.epi;
+  const int f = threadIdx.x % ROWS, t = threadIdx.x / ROWS;
+  const int64_t col = n0 + f;
+  const bool mine = t < g.T && t < NT * 8 && col < g.N;
+  auto read = [&](const void* p, int64_t i) {
+    return p && mine ? __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]) : 0.f;
+  };
+  const float b0 = read(ep.bias, col), b1 = kGate ? read(ep.bias2, col) : 0.f;
+  const float res = kGate ? 0.f : read(ep.res, t * ep.ldr + col);
+
   float acc[NT][4] = {};
   const int64_t chunks = (g.K + 31) / 32;
   for (int64_t c = warp; c < chunks; c += WARPS * UNROLL) {
@@ -106,18 +117,12 @@ dense_small_kernel(const SmallGemm g) {
     sum[n][(l >> 2) + 8 * (i >> 1)][(l & 3) * 2 + (i & 1)] = s;
   }
   __syncthreads();
-  const int f = threadIdx.x % ROWS, t = threadIdx.x / ROWS;
-  const int64_t col = n0 + f;
-  if (t >= g.T || t >= NT * 8 || col >= g.N) return;
-  const DenseEpi& ep = g.epi;
-  auto bias = [&](const void* p) {
-    return p ? __bfloat162float(static_cast<const __nv_bfloat16*>(p)[col]) : 0.f;
-  };
-  float z = sum[t >> 3][f][t & 7] + bias(ep.bias);
+  if (!mine) return;
+  float z = sum[t >> 3][f][t & 7] + b0;
   auto* zp = static_cast<__nv_bfloat16*>(ep.z);
   auto* out = static_cast<__nv_bfloat16*>(ep.out);
   if constexpr (kGate) {
-    const float up = sum[t >> 3][f + 8][t & 7] + bias(ep.bias2);
+    const float up = sum[t >> 3][f + 8][t & 7] + b1;
     if (zp) {
       zp[t * ep.ldz + col] = __float2bfloat16_rn(z);
       static_cast<__nv_bfloat16*>(ep.z2)[t * ep.ldz + col] = __float2bfloat16_rn(up);
@@ -126,7 +131,7 @@ dense_small_kernel(const SmallGemm g) {
   } else {
     if (zp) zp[t * ep.ldz + col] = __float2bfloat16_rn(z);
     act_switch(ep.act, [&](auto A) { z = act_value2<decltype(A)::value>(both(z), ep.gamma).x; });
-    if (ep.res) z += __bfloat162float(static_cast<const __nv_bfloat16*>(ep.res)[t * ep.ldr + col]);
+    z += res;
   }
   out[t * ep.ldo + col] = __float2bfloat16_rn(z);
 }

@@ -128,6 +128,16 @@ dense_stream_kernel(const __grid_constant__ SmallGemm g, const int stages, const
     bool ok = true;
     for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, buf ^= 1) {
       float acc[NT][4] = {};
+      // this thread's output, and what its epilogue reads, asked for before the weights' wait
+      const DenseEpi& ep = g.epi;
+      const int f = threadIdx.x % ROWS, t = threadIdx.x / ROWS;
+      const int64_t col = static_cast<int64_t>(tile) * ROWS + f;
+      const bool mine = t < g.T && t < NT * 8 && col < g.N;
+      auto read = [&](const void* p, int64_t i) {
+        return p && mine ? __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]) : 0.f;
+      };
+      const float b0 = read(ep.bias, col), b1 = kGate ? read(ep.bias2, col) : 0.f;
+      const float res = kGate ? 0.f : read(ep.res, t * ep.ldr + col);
       for (int sl = 0; sl < slices; ++sl, ++it) {
         const int64_t k0 = static_cast<int64_t>(sl) * SLICE + tig * 8;
         if (slices > 1 || it == 0) {  // one slice: the same tokens for every tile
@@ -180,23 +190,17 @@ dense_stream_kernel(const __grid_constant__ SmallGemm g, const int stages, const
         sh->sum[buf][n][(l >> 2) + 8 * (i >> 1)][(l & 3) * 2 + (i & 1)] = s;
       }
       sync_multipliers();
-      const int f = threadIdx.x % ROWS, t = threadIdx.x / ROWS;
-      const int64_t col = static_cast<int64_t>(tile) * ROWS + f;
-      if (ok && t < g.T && t < NT * 8 && col < g.N) {
-        const DenseEpi& ep = g.epi;
-        auto bias = [&](const void* p) {
-          return p ? __bfloat162float(static_cast<const __nv_bfloat16*>(p)[col]) : 0.f;
-        };
-        float z = sh->sum[buf][t >> 3][f][t & 7] + bias(ep.bias);
+      if (ok && mine) {
+        float z = sh->sum[buf][t >> 3][f][t & 7] + b0;
         auto* zp = static_cast<__nv_bfloat16*>(ep.z);
         if (zp) zp[t * ep.ldz + col] = __float2bfloat16_rn(z);
         if constexpr (kGate) {
-          const float up = sh->sum[buf][t >> 3][f + 8][t & 7] + bias(ep.bias2);
+          const float up = sh->sum[buf][t >> 3][f + 8][t & 7] + b1;
           if (zp) static_cast<__nv_bfloat16*>(ep.z2)[t * ep.ldz + col] = __float2bfloat16_rn(up);
           act_switch(ep.act, [&](auto A) { z = act_value2<decltype(A)::value>(both(z), ep.gamma).x * up; });
         } else {
           act_switch(ep.act, [&](auto A) { z = act_value2<decltype(A)::value>(both(z), ep.gamma).x; });
-          if (ep.res) z += __bfloat162float(static_cast<const __nv_bfloat16*>(ep.res)[t * ep.ldr + col]);
+          z += res;
         }
         static_cast<__nv_bfloat16*>(ep.out)[t * ep.ldo + col] = __float2bfloat16_rn(z);
       }
