@@ -224,6 +224,17 @@ def test_captured_and_same_bits():
         assert float(step()) == n and all(torch.equal(g, q.grad) for g, q in zip(got, ps))
 
 
+def test_scaling_counts_as_a_change():
+    import velvetoptimizer_b200 as vb
+    p = torch.nn.Parameter(torch.zeros(8, device="cuda"))
+    p.grad = torch.ones(8, device="cuda")
+    v = p.grad._version
+    vb.grad_norm([p.grad])
+    assert p.grad._version == v
+    vb.clip_grad_norm_([p], 0.5)
+    assert p.grad._version > v
+
+
 def test_refusals():
     import velvetoptimizer_b200 as vb
     p = torch.nn.Parameter(torch.zeros(3, device="cuda"))

@@ -295,6 +295,8 @@ int run_f32(Call& c, Product p, const F32Planes& planes, std::initializer_list<c
   return c.run([&] { return launch_dense_finish(kF32, p.epi, g, c.s); }, p.what);
 }
 
+constexpr int kDzBlocksPerSm = 6;
+
 // dz = dy act'(z) (written when `dz` is given) and the column sums into `db`.
 int run_dz(Call& c, const void* dy, int64_t lddy, const void* z, int64_t ldz, void* dz,
            int64_t lddz, int64_t T, int64_t N, int act, float gamma, void* db, bool db_f32) {
@@ -312,7 +314,7 @@ int run_dz(Call& c, const void* dy, int64_t lddy, const void* z, int64_t ldz, vo
   a.gamma = gamma;
   const int64_t width = 32 * (c.dtype == kF32 ? 4 : 8);
   const int64_t strips = (N + width - 1) / width;
-  int64_t rb = (6 * static_cast<int64_t>(c.o->num_sms) + strips - 1) / strips;
+  int64_t rb = (kDzBlocksPerSm * static_cast<int64_t>(c.o->num_sms) + strips - 1) / strips;
   if (rb > (T + 31) / 32) rb = (T + 31) / 32;
   if (rb > 128) rb = 128;
   if (rb < 1) rb = 1;

@@ -99,11 +99,13 @@ dense_finish_kernel(const DenseGemm g) {
   }
 }
 
+// Four rows per thread in flight: with one, 201 MB (16,384 x 2048, silu) took 61 us.
 template <typename T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 3)
 dense_dz_kernel(const DzArgs a, bool vec_dy, bool vec_z, bool vec_dz) {
   constexpr int W = Vec16<T>::N;
   constexpr bool kFast = sizeof(T) == 2;
+  constexpr int ROWS = 4;
   __shared__ float red[8][32 * W];
   pdl_wait_and_trigger();
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
@@ -113,23 +115,54 @@ dense_dz_kernel(const DzArgs a, bool vec_dy, bool vec_z, bool vec_dz) {
   const int64_t r1 = min(a.T, r0 + a.rows_per_block);
   float sum[W] = {};
   if (valid > 0) {
-    for (int64_t r = r0 + ty; r < r1; r += 8) {
-      float v[W];
-      load_row<W>(static_cast<const T*>(a.dy) + r * a.lddy + col, v, valid, vec_dy);
-      if (a.act != kActNone) {
-        float z[W];
-        load_row<W>(static_cast<const T*>(a.z) + r * a.ldz + col, z, valid, vec_z);
-        act_switch(a.act, [&](auto A) {
-          float d[W];
-          act_grads<kFast, decltype(A)::value>(z, d, a.gamma);
+    const T* dy = static_cast<const T*>(a.dy) + col;
+    const T* z = static_cast<const T*>(a.z) + col;
+    T* dz = static_cast<T*>(a.dz) + col;
+    auto scale = [&](float (&v)[W], float (&g)[W]) {
+      act_switch(a.act, [&](auto A) {
+        float d[W];
+        act_grads<kFast, decltype(A)::value>(g, d, a.gamma);
 #pragma unroll
-          for (int j = 0; j < W; ++j) v[j] *= d[j];
-        });
-      }
-      if (a.dz)
-        store_row<W>(static_cast<T*>(a.dz) + r * a.lddz + col, v, valid, vec_dz);
+        for (int j = 0; j < W; ++j) v[j] *= d[j];
+      });
+    };
+    auto finish = [&](float (&v)[W], int64_t r) {
+      if (a.dz) store_row<W>(dz + r * a.lddz, v, valid, vec_dz);
 #pragma unroll
       for (int j = 0; j < W; ++j) sum[j] += v[j];
+    };
+    int64_t r = r0 + ty;
+    if (vec_dy && (vec_z || a.act == kActNone) && valid >= W) {
+      for (; r + 8 * (ROWS - 1) < r1; r += 8 * ROWS) {
+        uint4 pv[ROWS], pz[ROWS];
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i)
+          pv[i] = __ldg(reinterpret_cast<const uint4*>(dy + (r + 8 * i) * a.lddy));
+        if (a.act != kActNone) {
+#pragma unroll
+          for (int i = 0; i < ROWS; ++i)
+            pz[i] = __ldg(reinterpret_cast<const uint4*>(z + (r + 8 * i) * a.ldz));
+        }
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) {
+          float v[W], g[W];
+          load16_to_f(reinterpret_cast<const T*>(&pv[i]), v);
+          if (a.act != kActNone) {
+            load16_to_f(reinterpret_cast<const T*>(&pz[i]), g);
+            scale(v, g);
+          }
+          finish(v, r + 8 * i);
+        }
+      }
+    }
+    for (; r < r1; r += 8) {
+      float v[W], g[W];
+      load_row<W>(dy + r * a.lddy, v, valid, vec_dy);
+      if (a.act != kActNone) {
+        load_row<W>(z + r * a.ldz, g, valid, vec_z);
+        scale(v, g);
+      }
+      finish(v, r);
     }
   }
   if (!a.colsum) return;

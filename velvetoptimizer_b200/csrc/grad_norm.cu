@@ -3,10 +3,11 @@
 //   norm = (sum over all elements |g|^p)^(1/p),  p = 1, 2 or infinity
 //   c = min(1, max_norm / (norm + 1e-6));  g *= c
 //
-// Two launches whatever the number of tensors: their addresses and sizes travel in the kernel's
-// parameters, so nothing is copied to the device first and a captured call replays as it is.
-// Tensors are cut into 16 KB pieces, and every warp takes pieces at a fixed stride, so many
-// small tensors and a few large ones load the SMs alike and the order of every sum is fixed.
+// Two launches for up to 1024 tensors (two more for every further 1024): their addresses and
+// sizes travel in the kernel's parameters, so nothing is copied to the device first and a captured call replays as it is.
+// Tensors are cut into pieces of 1 to 16 KB (as many as give every warp one), and every warp
+// takes pieces at a fixed stride, so many small tensors and a few large ones load the SMs alike
+// and the order of every sum is fixed.
 // Bound by HBM: N bytes are read for the norm; where c < 1 they are read again and written, in
 // reverse order, so that what the norm read last is still in L2.  Where c is 1 nothing is
 // written (x * 1 has the same bits).  Sums are held in fp64: fp32 squares leave its range
@@ -21,7 +22,7 @@ namespace {
 
 constexpr int kWarps = 8;
 constexpr int kBlocksPerSm = 4;
-constexpr int kPieceBytes = 16384;
+constexpr int kMinPiece = 1024, kMaxPiece = 16384;  // bytes
 constexpr int kBatch = 1024;     // tensors per launch: 20 KB of kernel parameters
 constexpr int kSmallBatch = 64;
 
@@ -32,43 +33,49 @@ struct GradTable {
   int32_t end_piece[N];  // pieces of tensors 0..i
   int n = 0;
   int first_partial = 0;
+  int piece = kMaxPiece;
 };
 
-// Elements [first, last) of a tensor that its piece k covers.  Pieces are cut at 16 KB from the
+// Elements [first, last) of a tensor that its piece k covers.  Pieces are counted from the
 // first 16-byte boundary, so all but the ends are whole aligned vectors.
 template <typename T>
-__device__ __forceinline__ void piece_range(const T* p, int64_t count, int64_t k, int64_t& first,
-                                            int64_t& last) {
-  constexpr int64_t E = kPieceBytes / sizeof(T);
+__device__ __forceinline__ void piece_range(const T* p, int64_t count, int64_t k, int piece,
+                                            int64_t& first, int64_t& last) {
+  const int64_t E = piece / static_cast<int>(sizeof(T));
   const int64_t head = ((16 - (reinterpret_cast<uintptr_t>(p) & 15u)) & 15u) / sizeof(T);
   first = k == 0 ? 0 : head + k * E;
   last = min(count, head + (k + 1) * E);
 }
 
-// f(value) over a piece: scalars up to the first 16-byte boundary, vectors, scalars
+// f(value) over the n elements at p (one piece): scalars up to the first 16-byte boundary,
+// vectors, scalars
 template <typename T, typename S, typename V>
-__device__ __forceinline__ void walk(T* p, int64_t first, int64_t last, int lane, S&& scalar,
-                                     V&& vector) {
+__device__ __forceinline__ void walk(T* p, int n, int lane, S&& scalar, V&& vector) {
   constexpr int W = 16 / sizeof(T);
-  const int64_t head = ((16 - (reinterpret_cast<uintptr_t>(p + first) & 15u)) & 15u) / sizeof(T);
-  const int64_t body = min(last, first + head);
-  if (first + lane < body) scalar(p + first + lane);
-  const int64_t nvec = (last - body) / W;
-  constexpr int U = 8;
-  int64_t i = lane;
-  for (; i + 32 * (U - 1) < nvec; i += 32 * U) {
+  constexpr int U = 8;  // loads in flight per lane
+  const int head = min(n, static_cast<int>(((16 - (reinterpret_cast<uintptr_t>(p) & 15u)) & 15u) /
+                                           sizeof(T)));
+  if (lane < head) scalar(p + lane);
+  uint4* q = reinterpret_cast<uint4*>(p + head) + lane;
+  int left = (n - head) / W - lane;  // vectors from this lane's on
+  const int tail = (n - head) % W;
+  if (lane < tail) scalar(p + n - tail + lane);
+  for (; left > 32 * (U - 1); left -= 32 * U, q += 32 * U) {
     uint4 v[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) v[u] = *reinterpret_cast<const uint4*>(p + body + (i + 32 * u) * W);
+    for (int u = 0; u < U; ++u) v[u] = q[32 * u];
 #pragma unroll
-    for (int u = 0; u < U; ++u) vector(p + body + (i + 32 * u) * W, v[u]);
+    for (int u = 0; u < U; ++u) vector(reinterpret_cast<T*>(q + 32 * u), v[u]);
   }
-  for (; i < nvec; i += 32) {
-    const uint4 v = *reinterpret_cast<const uint4*>(p + body + i * W);
-    vector(p + body + i * W, v);
+  for (; left > 0; left -= 32 * 4, q += 32 * 4) {  // what does not fill a round
+    uint4 v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (left > 32 * u) v[u] = q[32 * u];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (left > 32 * u) vector(reinterpret_cast<T*>(q + 32 * u), v[u]);
   }
-  const int64_t tail = body + nvec * W;
-  if (tail + lane < last) scalar(p + tail + lane);
 }
 
 template <typename T>
@@ -120,7 +127,7 @@ __device__ __forceinline__ int tensor_of(const GradTable<N>& t, int k) {
 }
 
 template <int N, int P>
-__global__ void __launch_bounds__(32 * kWarps)
+__global__ void __launch_bounds__(32 * kWarps, kBlocksPerSm)
 grad_norm_kernel(const __grid_constant__ GradTable<N> t, double* partial) {
   __shared__ double red[kWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -133,8 +140,8 @@ grad_norm_kernel(const __grid_constant__ GradTable<N> t, double* partial) {
     auto run = [&](auto* p, int64_t count) {
       using T = std::remove_reference_t<decltype(*p)>;
       int64_t first, last;
-      piece_range(p, count, at, first, last);
-      walk(p, first, last, lane, [&](T* q) { add_value<P>(acc, Elt<T>::to_f(*q)); },
+      piece_range(p, count, at, t.piece, first, last);
+      walk(p + first, static_cast<int>(last - first), lane, [&](T* q) { add_value<P>(acc, Elt<T>::to_f(*q)); },
            [&](T*, uint4 v) {
              float f[16 / sizeof(T)];
              unpack<T>(v, f);
@@ -159,7 +166,7 @@ grad_norm_kernel(const __grid_constant__ GradTable<N> t, double* partial) {
 
 // Every block forms the same norm from the partials, then scales its pieces (N = 0: none).
 template <int N, int P>
-__global__ void __launch_bounds__(32 * kWarps)
+__global__ void __launch_bounds__(32 * kWarps, kBlocksPerSm)
 grad_scale_kernel(const __grid_constant__ GradTable<N> t, const double* partial, int partials,
                   float max_norm, int clip, float* norm_out) {
   __shared__ double red[kWarps];
@@ -192,8 +199,8 @@ grad_scale_kernel(const __grid_constant__ GradTable<N> t, const double* partial,
     auto run = [&](auto* p, int64_t count) {
       using T = std::remove_reference_t<decltype(*p)>;
       int64_t first, last;
-      piece_range(p, count, at, first, last);
-      walk(p, first, last, lane, [&](T* q) { *q = Elt<T>::from_f(Elt<T>::to_f(*q) * coef); },
+      piece_range(p, count, at, t.piece, first, last);
+      walk(p + first, static_cast<int>(last - first), lane, [&](T* q) { *q = Elt<T>::from_f(Elt<T>::to_f(*q) * coef); },
            [&](T* q, uint4 v) {
              float f[16 / sizeof(T)];
              unpack<T>(v, f);
@@ -207,10 +214,10 @@ grad_scale_kernel(const __grid_constant__ GradTable<N> t, const double* partial,
   }
 }
 
-int64_t pieces_of(const void* p, int64_t count, int dtype) {
+int64_t pieces_of(const void* p, int64_t count, int dtype, int piece) {
   const int64_t elt = dtype == kF32 ? 4 : 2;
   const int64_t head = ((16 - static_cast<int64_t>(reinterpret_cast<uintptr_t>(p) & 15u)) & 15) / elt;
-  const int64_t per = kPieceBytes / elt;
+  const int64_t per = piece / elt;
   const int64_t rest = count - head;
   return rest <= 0 ? 1 : (rest + per - 1) / per;
 }
@@ -226,6 +233,10 @@ template <int N, int P>
 cudaError_t run_list(const GradList& l, float max_norm, bool clip, float* norm, double* partial,
                      int num_sms, cudaStream_t s) {
   const int max_blocks = num_sms * kBlocksPerSm;
+  int64_t bytes = 0;
+  for (int i = 0; i < l.n; ++i) bytes += l.counts[i] * static_cast<int64_t>(dtype_bytes(l.dtypes[i]));
+  int piece = kMaxPiece;
+  while (piece > kMinPiece && bytes / piece < static_cast<int64_t>(max_blocks) * kWarps) piece /= 2;
   int partials = 0;
   bool first = true;
   for (int pass = 0; pass < (clip ? 2 : 1); ++pass) {
@@ -234,9 +245,10 @@ cudaError_t run_list(const GradList& l, float max_norm, bool clip, float* norm, 
       GradTable<N> t;
       int64_t total = 0;
       t.n = 0;
+      t.piece = piece;
       for (; at < l.n && t.n < N; ++at) {
         if (l.counts[at] == 0) continue;
-        const int64_t more = pieces_of(l.ptrs[at], l.counts[at], l.dtypes[at]);
+        const int64_t more = pieces_of(l.ptrs[at], l.counts[at], l.dtypes[at], piece);
         if (total + more > 0x3fffffff) {
           if (t.n == 0) return cudaErrorInvalidValue;
           break;

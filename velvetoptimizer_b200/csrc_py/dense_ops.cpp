@@ -1,5 +1,6 @@
-// Host path of velvetoptimizer_b200.linear and .gated_ffn for eager calls: argument checks,
-// output and workspace tensors, the C-ABI call and the autograd node, in C++.  The same work
+// Host path of velvetoptimizer_b200.linear, .gated_ffn, .grad_norm and .clip_grad_norm_ for
+// eager calls: argument checks, output and workspace tensors, the C-ABI call and the autograd
+// node, in C++.  The same work
 // done in Python and ctypes takes 30 us a forward and 100 us a backward, several times what
 // the kernels of a one-token call take.
 #include <torch/extension.h>
@@ -11,7 +12,11 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/autograd/variable.h>
 
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <algorithm>
 #include <array>
 
 #include "vesper_moe.h"
@@ -135,7 +140,8 @@ std::tuple<Tensor, Tensor> linear_forward(const Tensor& x_in, const Tensor& w_in
   d.activation = static_cast<int32_t>(act);
   d.gamma = static_cast<float>(gamma);
   Tensor y = fresh({d.tokens, d.out_features}, x.options());
-  Tensor z = keep ? fresh({d.tokens, d.out_features}, x.options()) : fresh({0}, x.options());
+  Tensor z;
+  if (keep) z = fresh({d.tokens, d.out_features}, x.options());
   size_t need = 0;
   check(o, vmoe_linear_workspace_size(o, &d, 0, &need), "vmoe_linear_workspace_size");
   const Workspace ws(need, x);
@@ -174,7 +180,7 @@ std::tuple<Tensor, Tensor, Tensor> linear_backward(const Tensor& x_in, const Ten
   const Workspace ws(need, x);
   check(o,
         vmoe_linear_backward(o, &d, x.data_ptr(), w.data_ptr(),
-                             z.numel() ? z.data_ptr() : nullptr, dy.data_ptr(), lddy,
+                             z.defined() && z.numel() ? z.data_ptr() : nullptr, dy.data_ptr(), lddy,
                              want[0] ? dx.data_ptr() : nullptr, want[1] ? dw.data_ptr() : nullptr,
                              want[2] ? db.data_ptr() : nullptr, ws.p, ws.n, stream_of(x)),
         "vmoe_linear_backward");
@@ -212,10 +218,10 @@ std::tuple<Tensor, Tensor> gated_ffn_forward(const Tensor& x_in, const Tensor& g
   check(o, vmoe_gated_ffn_workspace_size(o, &d, 0, &need, &saved_bytes),
         "vmoe_gated_ffn_workspace_size");
   Tensor y = fresh({d.tokens, d.hidden}, x.options());
-  Tensor saved = fresh({keep ? static_cast<int64_t>(saved_bytes) : 0},
-                       x.options().dtype(at::kByte));
+  Tensor saved;
+  if (keep) saved = fresh({static_cast<int64_t>(saved_bytes)}, x.options().dtype(at::kByte));
   const Workspace ws(need, x);
-  const bool kept = saved.numel() > 0;
+  const bool kept = keep && saved.numel() > 0;
   check(o,
         vmoe_gated_ffn_forward(o, &d, x.data_ptr(), &w, r.defined() ? r.data_ptr() : nullptr,
                                y.data_ptr(), kept ? saved.data_ptr() : nullptr,
@@ -523,6 +529,108 @@ Tensor gated_ffn(const Tensor& x, const Tensor& gate_w, const Tensor& up_w, cons
   return x.dim() == 2 ? y : y.reshape(x.sizes());
 }
 
+// ---- gradient norm and clipping -----------------------------------------------------------
+struct GradTable {
+  std::vector<void*> ptrs;
+  std::vector<int64_t> counts, bytes;
+  std::vector<int32_t> dtypes;
+
+  void add(const Tensor& t) {
+    if (t.numel() == 0) return;
+    ptrs.push_back(t.data_ptr());
+    counts.push_back(t.numel());
+    dtypes.push_back(dtype_of(t.scalar_type()));
+    bytes.push_back(t.numel() * static_cast<int64_t>(t.element_size()));
+  }
+
+  // A tensor given twice is taken once; any other overlap raises (two warps would scale the
+  // same element).
+  void check_overlap() {
+    const size_t n = ptrs.size();
+    std::vector<size_t> order(n);
+    for (size_t i = 0; i < n; ++i) order[i] = i;
+    auto at = [&](size_t i) { return reinterpret_cast<uintptr_t>(ptrs[i]); };
+    std::sort(order.begin(), order.end(),
+              [&](size_t a, size_t b) { return at(a) != at(b) ? at(a) < at(b) : a < b; });
+    std::vector<char> drop;
+    size_t last = 0;
+    uintptr_t end = 0;
+    for (size_t k = 0; k < n; ++k) {
+      const size_t i = order[k];
+      if (k > 0 && at(i) < end) {
+        TORCH_CHECK_VALUE(
+            at(i) == at(last) && bytes[i] == bytes[last] && dtypes[i] == dtypes[last],
+            "gradients overlap in memory");
+        drop.resize(n);
+        drop[i] = 1;
+        continue;
+      }
+      end = at(i) + static_cast<uintptr_t>(bytes[i]);
+      last = i;
+    }
+    if (drop.empty()) return;
+    size_t m = 0;
+    for (size_t i = 0; i < n; ++i) {
+      if (drop[i]) continue;
+      ptrs[m] = ptrs[i];
+      counts[m] = counts[i];
+      dtypes[m++] = dtypes[i];
+    }
+    ptrs.resize(m);
+    counts.resize(m);
+    dtypes.resize(m);
+  }
+};
+
+// The norm of the tensors of a list or tuple, or of their .grad where present (none: nothing),
+// scaled in place when max_norm >= 0.
+std::optional<Tensor> grad_norm(const py::object& items, bool use_grad, double max_norm, int norm) {
+  TORCH_CHECK_TYPE(PyList_Check(items.ptr()) || PyTuple_Check(items.ptr()), "expected a list or tuple");
+  PyObject** p = PySequence_Fast_ITEMS(items.ptr());
+  const Py_ssize_t n = PySequence_Fast_GET_SIZE(items.ptr());
+  GradTable table;
+  std::vector<std::pair<Tensor, Tensor>> copies;  // not dense: a dense copy each
+  Tensor like;
+  at::NoGradGuard no_grad;
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    TORCH_CHECK_TYPE(THPVariable_Check(p[i]), "expected tensors");
+    const Tensor& own = THPVariable_Unpack(p[i]);
+    const Tensor& t = use_grad ? own.grad() : own;
+    if (!t.defined()) continue;
+    TORCH_CHECK_TYPE(t.layout() == at::kStrided, "sparse gradients are not supported");
+    TORCH_CHECK_TYPE(supported(t.scalar_type()), "gradients must be float32 or bfloat16");
+    TORCH_CHECK(t.is_cuda(), "gradients must be CUDA tensors (there is no CPU path)");
+    if (!like.defined()) like = t;
+    TORCH_CHECK_VALUE(t.device() == like.device(), "gradients must lie on one device");
+    if (t.is_non_overlapping_and_dense()) {
+      table.add(t);
+      if (max_norm >= 0 && !t.is_inference()) torch::autograd::impl::bump_version(t);
+      continue;
+    }
+    for (int64_t k = 0; max_norm >= 0 && k < t.dim(); ++k)
+      TORCH_CHECK_VALUE(t.stride(k) != 0 || t.size(k) <= 1,
+                        "a gradient whose elements share memory cannot be scaled in place");
+    copies.emplace_back(t, t.contiguous());
+  }
+  if (!like.defined()) return std::nullopt;
+  for (const auto& c : copies) table.add(c.second);
+  table.check_overlap();
+  vmoe_ops* o = context(like);
+  const int count = static_cast<int>(table.ptrs.size());
+  size_t need = 0;
+  check(o, vmoe_grad_norm_workspace_size(o, count, &need), "vmoe_grad_norm_workspace_size");
+  const Workspace ws(need, like);
+  Tensor out = fresh({}, like.options().dtype(at::kFloat));
+  check(o,
+        vmoe_grad_norm(o, table.ptrs.data(), table.counts.data(), table.dtypes.data(), count, norm,
+                       static_cast<float>(max_norm), out.mutable_data_ptr<float>(), ws.p, ws.n,
+                       stream_of(like)),
+        "vmoe_grad_norm");
+  if (max_norm >= 0)
+    for (auto& c : copies) c.first.copy_(c.second);
+  return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_dense_ops, m) {
@@ -538,10 +646,21 @@ PYBIND11_MODULE(_dense_ops, m) {
   using Release = py::call_guard<py::gil_scoped_release>;
   m.def("linear", &linear, Release());
   m.def("gated_ffn", &gated_ffn, Release());
-  m.def("linear_forward", &linear_forward, Release());
+  // the tracers' ops return a tensor in every place
+  m.def("linear_forward", [](const Tensor& x, const Tensor& w, const OptTensor& b, const OptTensor& r,
+                             int64_t act, double gamma, bool keep) {
+    auto [y, z] = linear_forward(x, w, b, r, act, gamma, keep);
+    return std::make_tuple(y, keep ? z : fresh({0}, x.options()));
+  }, Release());
   m.def("linear_backward", &linear_backward, Release());
-  m.def("gated_ffn_forward", &gated_ffn_forward, Release());
+  m.def("gated_ffn_forward", [](const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& wd,
+                                const OptTensor& bg, const OptTensor& bu, const OptTensor& bd,
+                                const OptTensor& r, int64_t act, double gamma, bool keep) {
+    auto [y, saved] = gated_ffn_forward(x, wg, wu, wd, bg, bu, bd, r, act, gamma, keep);
+    return std::make_tuple(y, keep ? saved : fresh({0}, x.options().dtype(at::kByte)));
+  }, Release());
   m.def("gated_ffn_backward", &gated_ffn_backward, Release());
+  m.def("grad_norm", &grad_norm);
   m.def("device_status", [](const Tensor& x) {
     int32_t code = 0;
     vmoe_ops* o = context(x);

@@ -7,21 +7,19 @@ the GPU unless ``error_if_nonfinite`` asks for it.
 """
 from __future__ import annotations
 
-import ctypes
 import math
 
 import torch
 
-from . import _lib
-from .dense import ops_for
+from .dense import _native
 
 _NORMS = {math.inf: 0, 1.0: 1, 2.0: 2}  # VMOE_NORM_*
 
 
-def _tensors(tensors) -> list:
-    if isinstance(tensors, torch.Tensor):
-        return [tensors]
-    return tensors if isinstance(tensors, (list, tuple)) else list(tensors)
+def _tensors(tensors):
+    if type(tensors) in (list, tuple):
+        return tensors
+    return [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
 
 
 def _norm_code(norm_type) -> int:
@@ -31,40 +29,11 @@ def _norm_code(norm_type) -> int:
     return code
 
 
-def _run(items: list, use_grad: bool, max_norm: float, code: int) -> torch.Tensor:
-    from .lib._param_key import grad_table  # built beside the library
-    table = grad_table(items, use_grad)
-    if table is None:
-        return torch.tensor(0.0)
-    ptrs, counts, dtypes, index, odd = table
-    device = torch.device("cuda", index)
-    copies = []
-    if odd:  # slices with gaps and the like: a dense copy each, written back after the scaling
-        ours = [items[i].grad if use_grad else items[i] for i in odd]
-        for t in ours:
-            if max_norm >= 0 and any(st == 0 and n > 1 for n, st in zip(t.shape, t.stride())):
-                raise ValueError("a gradient whose elements share memory cannot be scaled in place")
-        copies = [(t, t.contiguous()) for t in ours]
-        more = grad_table([c for _, c in copies], False)
-        ptrs, counts, dtypes = ptrs + more[0], counts + more[1], dtypes + more[2]
-    o = ops_for(device)
-    n = len(counts) // 8
-    size = ctypes.c_size_t()
-    o.check(o.lib.vmoe_grad_norm_workspace_size(o.ptr, n, size), "vmoe_grad_norm_workspace_size")
-    # the norm takes the workspace's last bytes: one allocation
-    ws = torch.empty(size.value + 4, dtype=torch.uint8, device=device)
-    norm = ws[size.value:].view(torch.float32)[0]
-    stream = torch.cuda.current_stream(device).cuda_stream
-    o.check(o.lib.vmoe_grad_norm(o.ptr, ptrs, counts, dtypes, n, code, max_norm, norm.data_ptr(),
-                                 ws.data_ptr(), size.value, ctypes.c_void_p(stream)),
-            "vmoe_grad_norm")
-    if max_norm >= 0:
-        for t, c in copies:
-            t.copy_(c)
-    return norm
+def _run(items, use_grad: bool, max_norm: float, code: int) -> torch.Tensor:
+    norm = _native().grad_norm(items, use_grad, max_norm, code)
+    return torch.tensor(0.0) if norm is None else norm
 
 
-@torch.no_grad()
 def grad_norm(tensors, norm_type: float = 2.0) -> torch.Tensor:
     """The norm of all elements of ``tensors`` (a tensor or an iterable of float32 and bfloat16
     CUDA tensors on one device) as a float32 scalar on their device.
@@ -75,7 +44,6 @@ def grad_norm(tensors, norm_type: float = 2.0) -> torch.Tensor:
     return _run(_tensors(tensors), False, -1.0, _norm_code(norm_type))
 
 
-@torch.no_grad()
 def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0,
                     error_if_nonfinite: bool = False) -> torch.Tensor:
     """Scale the gradients of ``parameters`` in place by ``min(1, max_norm / (norm + 1e-6))`` and
