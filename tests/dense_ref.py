@@ -125,9 +125,7 @@ def gated_ffn(x, wg, wu, wd, bg, bu, bd, r, dy, kind, gamma, dtype, grad_dtype=N
     if dy is None:
         return out
     dh, edh = product(dy, wd)
-    # g and u (v here) are kept rounded
-    eg = eg + u * (g.abs() + eg)
-    ev = ev + u * (v.abs() + ev)
+    # g and u (v here) are kept in fp32
     d = act_grad(g, kind, gamma)
     ed = CURVE * (eg / g.abs().clamp(min=1e-30)).clamp(max=1.0) + 8 * f
     if kind == "relu":

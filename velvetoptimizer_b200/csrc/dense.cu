@@ -550,17 +550,19 @@ struct FfnPtrs {
   char* saved;  // training: g | u | h
 };
 
+// g and u [T, ld] in fp32, then h [T, ld]; ld keeps every row in whole 16-byte units
 struct FfnSaved {
   int64_t ld;
-  size_t part, total;
+  size_t part, total;  // bytes of g (and of u), and of all
 };
 
 FfnSaved ffn_saved(const vmoe_gated_ffn& d) {
   FfnSaved s;
   s.ld = round_up(d.inter, 8);
-  s.part = (static_cast<size_t>(d.tokens) * s.ld * dtype_bytes(d.dtype) + 255) &
-           ~static_cast<size_t>(255);
-  s.total = 3 * s.part;
+  auto round256 = [](size_t n) { return (n + 255) & ~static_cast<size_t>(255); };
+  const size_t n = static_cast<size_t>(d.tokens) * s.ld;
+  s.part = round256(n * 4);
+  s.total = 2 * s.part + round256(n * dtype_bytes(d.dtype));
   return s;
 }
 

@@ -33,7 +33,11 @@ struct DenseEpi {
   void* out = nullptr;
   void* out2 = nullptr;  // kEpiGluBwd: du; second group of a grouped launch: its output
   int64_t ldo = 0;
-  void* z = nullptr;   // kept pre-activations (linear: z, gated: g; glu backward reads g)
+  // kept pre-activations.  The linear's z has the operands' type: its rounding reaches the
+  // gradient only through act'.  The gated block's g and u are fp32: both scale the gradient
+  // directly, and rounded to bf16 they would add as much error again as rounding dg and du for
+  // the products does (relative error of dx 0.0030 against 0.0024; 3 % more time).
+  void* z = nullptr;   // linear: z; gated, and its gradient: g
   void* z2 = nullptr;  // u
   int64_t ldz = 0;
   int out_f32 = 0;  // out is fp32 (gradients of fp32 parameters)

@@ -43,8 +43,8 @@ dense_finish_kernel(const DenseGemm g) {
     }
     if constexpr (EPI == kEpiGluBwd) {
       float gg[V];
-      load_row<V>(static_cast<const T*>(ep.z) + row * ep.ldz + col, gg, valid, ep.vec & kVecZ);
-      load_row<V>(static_cast<const T*>(ep.z2) + row * ep.ldz + col, u, valid, ep.vec & kVecZ);
+      load_row<V>(static_cast<const float*>(ep.z) + row * ep.ldz + col, gg, valid, ep.vec & kVecZ);
+      load_row<V>(static_cast<const float*>(ep.z2) + row * ep.ldz + col, u, valid, ep.vec & kVecZ);
       act_switch(ep.act, [&](auto A) {
         float d[V];
         act_grads<kFast, decltype(A)::value>(gg, d, ep.gamma);
@@ -73,8 +73,8 @@ dense_finish_kernel(const DenseGemm g) {
         for (int j = 0; j < V; ++j) u[j] += b[j];
       }
       if (ep.z) {
-        store_row<V>(static_cast<T*>(ep.z) + row * ep.ldz + col, v, valid, ep.vec & kVecZ);
-        store_row<V>(static_cast<T*>(ep.z2) + row * ep.ldz + col, u, valid, ep.vec & kVecZ);
+        store_row<V>(static_cast<float*>(ep.z) + row * ep.ldz + col, v, valid, ep.vec & kVecZ);
+        store_row<V>(static_cast<float*>(ep.z2) + row * ep.ldz + col, u, valid, ep.vec & kVecZ);
       }
       act_switch(ep.act, [&](auto A) {
         act_values<kFast, decltype(A)::value>(v, ep.gamma);

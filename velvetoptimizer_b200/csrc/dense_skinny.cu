@@ -49,6 +49,14 @@ __device__ __forceinline__ void st_cluster(uint32_t addr, float v) {
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
 
+// the first n of a thread's values, GROUPS rows apart
+template <int GROUPS, typename T, int PER>
+__device__ __forceinline__ void store_rows(T* p, int64_t ld, const float (&v)[PER], int n) {
+#pragma unroll
+  for (int i = 0; i < PER; ++i, p += GROUPS * ld)
+    if (i < n) *p = Elt<T>::from_f(v[i]);
+}
+
 template <int EPI>
 __global__ void __launch_bounds__(THREADS, 1)
 dense_skinny_kernel(const __grid_constant__ CUtensorMap w_map,
@@ -232,20 +240,18 @@ dense_skinny_kernel(const __grid_constant__ CUtensorMap w_map,
             if constexpr (kGate) up[i] += sums[i * GROUPS * 128 + 64];
           }
         }
-        auto store = [&](void* to, int64_t ld, const float (&v)[PER]) {
-          auto* p = static_cast<__nv_bfloat16*>(to) + t0 * ld + col;
-#pragma unroll
-          for (int i = 0; i < PER; ++i, p += GROUPS * ld)
-            if (i < n) *p = __float2bfloat16_rn(v[i]);
-        };
         if (ep.z) {
-          store(ep.z, ep.ldz, z);
-          if constexpr (kGate) store(ep.z2, ep.ldz, up);
+          if constexpr (kGate) {
+            store_rows<GROUPS>(static_cast<float*>(ep.z) + t0 * ep.ldz + col, ep.ldz, z, n);
+            store_rows<GROUPS>(static_cast<float*>(ep.z2) + t0 * ep.ldz + col, ep.ldz, up, n);
+          } else {
+            store_rows<GROUPS>(static_cast<__nv_bfloat16*>(ep.z) + t0 * ep.ldz + col, ep.ldz, z, n);
+          }
         }
         act_values<true, decltype(A)::value>(z, ep.gamma);
 #pragma unroll
         for (int i = 0; i < PER; ++i) z[i] = kGate ? z[i] * up[i] : z[i] + r[i];
-        store(ep.out, ep.ldo, z);
+        store_rows<GROUPS>(static_cast<__nv_bfloat16*>(ep.out) + t0 * ep.ldo + col, ep.ldo, z, n);
       }
     });
   }

@@ -119,17 +119,16 @@ dense_small_kernel(const SmallGemm g) {
   __syncthreads();
   if (!mine) return;
   float z = sum[t >> 3][f][t & 7] + b0;
-  auto* zp = static_cast<__nv_bfloat16*>(ep.z);
   auto* out = static_cast<__nv_bfloat16*>(ep.out);
   if constexpr (kGate) {
     const float up = sum[t >> 3][f + 8][t & 7] + b1;
-    if (zp) {
-      zp[t * ep.ldz + col] = __float2bfloat16_rn(z);
-      static_cast<__nv_bfloat16*>(ep.z2)[t * ep.ldz + col] = __float2bfloat16_rn(up);
+    if (ep.z) {
+      static_cast<float*>(ep.z)[t * ep.ldz + col] = z;
+      static_cast<float*>(ep.z2)[t * ep.ldz + col] = up;
     }
     act_switch(ep.act, [&](auto A) { z = act_value2<decltype(A)::value>(both(z), ep.gamma).x * up; });
   } else {
-    if (zp) zp[t * ep.ldz + col] = __float2bfloat16_rn(z);
+    if (ep.z) static_cast<__nv_bfloat16*>(ep.z)[t * ep.ldz + col] = __float2bfloat16_rn(z);
     act_switch(ep.act, [&](auto A) { z = act_value2<decltype(A)::value>(both(z), ep.gamma).x; });
     z += res;
   }

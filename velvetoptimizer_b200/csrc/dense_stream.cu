@@ -192,13 +192,15 @@ dense_stream_kernel(const __grid_constant__ SmallGemm g, const int stages, const
       sync_multipliers();
       if (ok && mine) {
         float z = sh->sum[buf][t >> 3][f][t & 7] + b0;
-        auto* zp = static_cast<__nv_bfloat16*>(ep.z);
-        if (zp) zp[t * ep.ldz + col] = __float2bfloat16_rn(z);
         if constexpr (kGate) {
           const float up = sh->sum[buf][t >> 3][f + 8][t & 7] + b1;
-          if (zp) static_cast<__nv_bfloat16*>(ep.z2)[t * ep.ldz + col] = __float2bfloat16_rn(up);
+          if (ep.z) {
+            static_cast<float*>(ep.z)[t * ep.ldz + col] = z;
+            static_cast<float*>(ep.z2)[t * ep.ldz + col] = up;
+          }
           act_switch(ep.act, [&](auto A) { z = act_value2<decltype(A)::value>(both(z), ep.gamma).x * up; });
         } else {
+          if (ep.z) static_cast<__nv_bfloat16*>(ep.z)[t * ep.ldz + col] = __float2bfloat16_rn(z);
           act_switch(ep.act, [&](auto A) { z = act_value2<decltype(A)::value>(both(z), ep.gamma).x; });
           z += res;
         }

@@ -214,6 +214,28 @@ __device__ __forceinline__ void land(const Block& b, const uint4 (&v)[4], uint8_
   }
 }
 
+// 32 rows x 16 columns of an fp32 matrix whose rows are whole aligned 16-byte units
+struct Kept {
+  const float* p;
+  int64_t ld;
+  int rows, cols;  // cols a multiple of 4
+};
+
+__device__ __forceinline__ void fetch16(const Kept& b, uint4 (&v)[4], int lane) {
+  const float* p = b.p + (lane >> 2) * b.ld + (lane & 3) * 4;
+#pragma unroll
+  for (int i = 0; i < 4; ++i, p += 8 * b.ld) {
+    v[i] = make_uint4(0, 0, 0, 0);
+    if (i * 8 + (lane >> 2) < b.rows && (lane & 3) * 4 < b.cols)
+      v[i] = __ldg(reinterpret_cast<const uint4*>(p));
+  }
+}
+
+__device__ __forceinline__ void land16(const uint4 (&v)[4], uint8_t* buf, int lane) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) *unit16(buf, i * 8 + (lane >> 2), lane & 3) = v[i];
+}
+
 __device__ __forceinline__ void get_row(uint8_t* buf, float (&v)[32], int lane) {
 #pragma unroll
   for (int c = 0; c < 4; ++c)
@@ -257,11 +279,12 @@ __device__ __forceinline__ void flush_f32(float* p, int64_t ld, int rows, int co
     *reinterpret_cast<float4*>(unit32(buf, lane, c)) =
         make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
   __syncwarp();
-  if (vec && cols == 32) {
+  if (vec && cols % 4 == 0) {
+    float* q = p + (lane >> 3) * ld + (lane & 7) * 4;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 8; ++i, q += 4 * ld) {
       const int r = i * 4 + (lane >> 3), c = lane & 7;
-      if (r < rows) *reinterpret_cast<uint4*>(p + r * ld + c * 4) = *unit32(buf, r, c);
+      if (r < rows && c * 4 < cols) *reinterpret_cast<uint4*>(q) = *unit32(buf, r, c);
     }
   } else {
 #pragma unroll 8
@@ -459,12 +482,18 @@ gemm_dense_kernel(const __grid_constant__ DenseMaps maps, const __grid_constant_
         return Block{static_cast<__nv_bfloat16*>(const_cast<void*>(p)) + row0 * ld + col0 + c, ld,
                      rows, vec ? (cols + 7) & ~7 : cols, vec};
       };
+      // 16 columns at offset c of g or u, which the forward kept in fp32 rows of whole units
+      auto kept = [&](const void* p, int c) {
+        const int64_t left = args.N - col0 - c;
+        return Kept{static_cast<const float*>(p) + row0 * ep.ldz + col0 + c, ep.ldz, rows,
+                    static_cast<int>(left < 16 ? (left > 0 ? (left + 3) & ~3 : 0) : 16)};
+      };
       // what the epilogue reads besides the accumulator is asked for before the product is done
       uint4 pre0[4], pre1[4];
       const bool has_res = !SPLIT && EPI == kEpiLinear && ep.res;
       if constexpr (!SPLIT && EPI == kEpiGluBwd) {
-        fetch(block(ep.z, ep.ldz, 0, kVecZ), pre0, lane);
-        fetch(block(ep.z2, ep.ldz, 0, kVecZ), pre1, lane);
+        fetch16(kept(ep.z, 0), pre0, lane);
+        fetch16(kept(ep.z2, 0), pre1, lane);
       } else if (has_res) {
         fetch(block(ep.res, ep.ldr, 0, kVecRes), pre0, lane);
       }
@@ -520,11 +549,10 @@ gemm_dense_kernel(const __grid_constant__ DenseMaps maps, const __grid_constant_
             add_bias(u, bias_s[1]);
           }
           if (ep.z) {
-            put_row(turn_a, g, lane);
-            put_row(turn_b, u, lane);
+            const int64_t at = row0 * ep.ldz + col0 + c;
+            flush_f32(static_cast<float*>(ep.z) + at, ep.ldz, rows, h.cols, true, g, turn_a, lane);
             __syncwarp();
-            flush(block(ep.z, ep.ldz, c, kVecZ), turn_a, lane);
-            flush(block(ep.z2, ep.ldz, c, kVecZ), turn_b, lane);
+            flush_f32(static_cast<float*>(ep.z2) + at, ep.ldz, rows, h.cols, true, u, turn_a, lane);
             __syncwarp();
           }
           act_switch(ep.act, [&](auto A) {
@@ -536,46 +564,56 @@ gemm_dense_kernel(const __grid_constant__ DenseMaps maps, const __grid_constant_
           __syncwarp();
           flush(h, turn_a, lane);
         } else if constexpr (EPI == kEpiGluBwd) {
-          const Block bg = block(ep.z, ep.ldz, c, kVecZ), bu = block(ep.z2, ep.ldz, c, kVecZ);
-          float dh[32];
-          tmem_ld32(t_row + c, dh);
-          release(c);
-          if (bg.cols == 0) continue;
-          land(bg, pre0, turn_a, lane);
-          land(bu, pre1, turn_b, lane);
-          __syncwarp();
-          if (c + 32 < COLS) {
-            fetch(block(ep.z, ep.ldz, c + 32, kVecZ), pre0, lane);
-            fetch(block(ep.z2, ep.ldz, c + 32, kVecZ), pre1, lane);
+          const Block bg = block(ep.out, ep.ldo, c, kVecOut), bu = block(ep.out2, ep.ldo, c, kVecOut);
+          if (bg.cols == 0) {
+            release(c);
+            continue;
           }
-          // a unit of 8 columns at a time, g and u replaced by dg and du where they lie: a row
-          // is read and rewritten by its own thread, the others' units meet at the sync
-          act_switch(ep.act, [&](auto A) {
+          // 16 columns of g and u at a time through the two halves of the buffer, 32 of dg and
+          // du out
+          uint4 dg[4], du[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              auto* ug = reinterpret_cast<__nv_bfloat16*>(unit16(turn_a, lane, k));
-              auto* uu = reinterpret_cast<__nv_bfloat16*>(unit16(turn_b, lane, k));
-              float g[8], u[8];
-              load16_to_f(ug, g);
-              load16_to_f(uu, u);
-#pragma unroll
-              for (int j = 0; j < 8; j += 2) {
-                const float2 p = make_float2(dh[8 * k + j], dh[8 * k + j + 1]);
-                float2 a, d;
-                act_grad2<decltype(A)::value>(make_float2(g[j], g[j + 1]), ep.gamma, a, d);
-                const float2 dg = mul2(mul2(p, make_float2(u[j], u[j + 1])), d), du = mul2(p, a);
-                g[j] = dg.x;
-                g[j + 1] = dg.y;
-                u[j] = du.x;
-                u[j + 1] = du.y;
-              }
-              store16_from_f(ug, g);
-              store16_from_f(uu, u);
+          for (int half = 0; half < 2; ++half) {
+            land16(pre0, turn_a, lane);
+            land16(pre1, turn_b, lane);
+            __syncwarp();
+            if (c + 16 * half + 16 < COLS) {
+              fetch16(kept(ep.z, c + 16 * half + 16), pre0, lane);
+              fetch16(kept(ep.z2, c + 16 * half + 16), pre1, lane);
             }
-          });
+            float dh[16];
+            tmem_ld16(t_row + c + 16 * half, dh);
+            if (half == 1) release(c);
+            act_switch(ep.act, [&](auto A) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {  // a unit of 4 columns
+                const float4 gv = *reinterpret_cast<const float4*>(unit16(turn_a, lane, k));
+                const float4 uv = *reinterpret_cast<const float4*>(unit16(turn_b, lane, k));
+                const float2 p0 = make_float2(dh[4 * k], dh[4 * k + 1]),
+                             p1 = make_float2(dh[4 * k + 2], dh[4 * k + 3]);
+                float2 a0, d0, a1, d1;
+                act_grad2<decltype(A)::value>(make_float2(gv.x, gv.y), ep.gamma, a0, d0);
+                act_grad2<decltype(A)::value>(make_float2(gv.z, gv.w), ep.gamma, a1, d1);
+                const float2 g0 = mul2(mul2(p0, make_float2(uv.x, uv.y)), d0), u0 = mul2(p0, a0);
+                const float2 g1 = mul2(mul2(p1, make_float2(uv.z, uv.w)), d1), u1 = mul2(p1, a1);
+                uint32_t* tg = reinterpret_cast<uint32_t*>(dg) + 8 * half + 2 * k;
+                uint32_t* tu = reinterpret_cast<uint32_t*>(du) + 8 * half + 2 * k;
+                tg[0] = pack_bf16x2(g0.x, g0.y);
+                tg[1] = pack_bf16x2(g1.x, g1.y);
+                tu[0] = pack_bf16x2(u0.x, u0.y);
+                tu[1] = pack_bf16x2(u1.x, u1.y);
+              }
+            });
+            __syncwarp();
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            *unit16(turn_a, lane, k) = dg[k];
+            *unit16(turn_b, lane, k) = du[k];
+          }
           __syncwarp();
-          flush(block(ep.out, ep.ldo, c, kVecOut), turn_a, lane);
-          flush(block(ep.out2, ep.ldo, c, kVecOut), turn_b, lane);
+          flush(bg, turn_a, lane);
+          flush(bu, turn_b, lane);
           if (ep.colsum) {
             float* dst = ep.colsum + row0 / 32 * args.N + col0 + c;
             const int cols = static_cast<int>(min(args.N - col0 - c, static_cast<int64_t>(32)));

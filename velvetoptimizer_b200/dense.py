@@ -115,8 +115,9 @@ def _(x, weight, z, dy, activation, gamma, want, grad_f32):
 @gated_ffn_forward_op.register_fake
 def _(x, gate_w, up_w, down_w, gate_b, up_b, down_b, residual, activation, gamma, keep):
     T, I = x.shape[0], gate_w.shape[0]
-    part = (T * ((I + 7) // 8 * 8) * x.element_size() + 255) // 256 * 256
-    return x.new_empty(x.shape), x.new_empty((3 * part if keep else 0,), dtype=torch.uint8)
+    n = T * ((I + 7) // 8 * 8)  # g and u in fp32, h
+    size = 2 * ((4 * n + 255) // 256 * 256) + (n * x.element_size() + 255) // 256 * 256
+    return x.new_empty(x.shape), x.new_empty((size if keep else 0,), dtype=torch.uint8)
 
 
 @gated_ffn_backward_op.register_fake
