@@ -626,13 +626,15 @@ def test_abi_pointer_refusals():
     assert f(o.ptr, d, p, p, None, None, None, None, ws, 1 << 19, None) == 1   # no y
     assert f(o.ptr, d, p + 2, p, None, None, p, None, ws, 1 << 19, None) == 1  # unaligned x
     assert f(o.ptr, d, p + 1, p, None, None, p, None, ws, 1 << 19, None) == 1
+    # 400 rows: the bias gradient's partial sums need a workspace (40 rows need none)
+    d = _lib.VmoeLinear(400, 64, 64, 64, 64, 64, bf, 0, 0.1, bf)
     assert o.lib.vmoe_linear_workspace_size(o.ptr, d, 1, n) == 0 and n.value > 0
     args = (p, p, None, p, 64, p, p, p)
     assert b(o.ptr, d, *args, None, 0, None) == _lib.VMOE_ERR_WORKSPACE
     assert b(o.ptr, d, *args, ws, n.value - 1, None) == _lib.VMOE_ERR_WORKSPACE
     assert b(o.ptr, d, *args, ws + 16, n.value, None) == _lib.VMOE_ERR_WORKSPACE
     assert b(o.ptr, d, p, p, None, p, 65, p, p, p, ws, n.value, None) == 1     # a pitch it cannot read
-    act = _lib.VmoeLinear(40, 64, 64, 64, 64, 64, bf, 2, 0.1, bf)
+    act = _lib.VmoeLinear(400, 64, 64, 64, 64, 64, bf, 2, 0.1, bf)
     assert o.lib.vmoe_linear_workspace_size(o.ptr, act, 1, n) == 0
     assert b(o.ptr, act, *args, ws, n.value, None) == 1                        # no z
     ffn = _lib.VmoeGatedFfn(40, 64, 64, 64, 64, bf, 4, 0.1, bf)

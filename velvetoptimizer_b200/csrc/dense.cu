@@ -296,6 +296,8 @@ int run_f32(Call& c, Product p, const F32Planes& planes, std::initializer_list<c
 }
 
 constexpr int kDzBlocksPerSm = 6;
+// so few rows are summed by one block per column strip, which spares the second launch
+constexpr int64_t kDzOneBlock = 256;
 
 // dz = dy act'(z) (written when `dz` is given) and the column sums into `db`.
 int run_dz(Call& c, const void* dy, int64_t lddy, const void* z, int64_t ldz, void* dz,
@@ -317,14 +319,19 @@ int run_dz(Call& c, const void* dy, int64_t lddy, const void* z, int64_t ldz, vo
   int64_t rb = (kDzBlocksPerSm * static_cast<int64_t>(c.o->num_sms) + strips - 1) / strips;
   if (rb > (T + 31) / 32) rb = (T + 31) / 32;
   if (rb > 128) rb = 128;
-  if (rb < 1) rb = 1;
+  if (rb < 1 || T <= kDzOneBlock) rb = 1;
   a.rows_per_block = (T + rb - 1) / rb;
   a.row_blocks = static_cast<int>((T + a.rows_per_block - 1) / a.rows_per_block);
-  if (db) a.colsum = c.ws.take<float>(static_cast<size_t>(a.row_blocks) * N * 4);
+  if (db && a.row_blocks == 1) {
+    a.db = db;
+    a.db_f32 = db_f32;
+  } else if (db) {
+    a.colsum = c.ws.take<float>(static_cast<size_t>(a.row_blocks) * N * 4);
+  }
   if (c.dry) return VMOE_OK;
   TRY(c.run([&] { return launch_dense_dz(c.dtype, a, c.s); }, "activation gradient"));
-  if (db)
-    return c.run([&] { return launch_colsum_finish(a.colsum, a.row_blocks, N, db, db_f32, c.s); }, "bias gradient");
+  if (a.colsum)
+    return c.run([&] { return launch_colsum_finish(a.colsum, a.row_blocks, N, db, nullptr, db_f32, c.s); }, "bias gradient");
   return VMOE_OK;
 }
 
@@ -818,10 +825,18 @@ int ffn_backward(Call& c, const vmoe_gated_ffn& d, const FfnPtrs& p) {
   }
   if (summed) {
     if (c.dry) return VMOE_OK;
-    if (gr.gate_b) TRY(c.run([&] { return launch_colsum_finish(colsum, row_blocks, I, gr.gate_b, gf32, c.s); }, "dbg"));
-    if (gr.up_b)
-      TRY(c.run([&] { return launch_colsum_finish(colsum + row_blocks * I, row_blocks, I, gr.up_b, gf32, c.s); }, "dbu"));
-    return VMOE_OK;
+    if (!gr.gate_b) {
+      if (!gr.up_b) return VMOE_OK;
+      return c.run(
+          [&] {
+            return launch_colsum_finish(colsum + row_blocks * I, row_blocks, I, gr.up_b, nullptr,
+                                        gf32, c.s);
+          },
+          "dbu");
+    }
+    return c.run(
+        [&] { return launch_colsum_finish(colsum, row_blocks, I, gr.gate_b, gr.up_b, gf32, c.s); },
+        "dbg");
   }
   TRY(run_dz(c, dg, sv.ld, nullptr, 0, nullptr, 0, T, I, kActNone, 0.f, c.dry ? any : gr.gate_b,
              gf32));

@@ -155,12 +155,15 @@ struct DzArgs {
   int act;
   float gamma;
   float* colsum;  // [row_blocks][N] partials, or null
+  void* db;       // one row block: the sums' own place instead
+  bool db_f32;
   int row_blocks;
   int64_t rows_per_block;
 };
 cudaError_t launch_dense_dz(int dtype, const DzArgs& a, cudaStream_t s);
 cudaError_t launch_colsum_finish(const float* partial, int64_t row_blocks, int64_t N, void* out,
-                                 bool out_f32, cudaStream_t s);
+                                 void* out2, bool out_f32, cudaStream_t s);
+// (out2: the sums of a second set of partials after the first)
 // rows of bf16 to a buffer whose pitch is a multiple of 8
 cudaError_t launch_pad_copy(const void* src, int64_t lds, int64_t rows, int64_t cols, void* dst,
                             int64_t ldd, cudaStream_t s);

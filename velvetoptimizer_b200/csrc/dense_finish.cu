@@ -165,7 +165,7 @@ dense_dz_kernel(const DzArgs a, bool vec_dy, bool vec_z, bool vec_dz) {
       finish(v, r);
     }
   }
-  if (!a.colsum) return;
+  if (!a.colsum && !a.db) return;
 #pragma unroll
   for (int j = 0; j < W; ++j) red[ty][tx * W + j] = sum[j];
   __syncthreads();
@@ -175,14 +175,20 @@ dense_dz_kernel(const DzArgs a, bool vec_dy, bool vec_z, bool vec_dz) {
     float s = 0.f;
 #pragma unroll
     for (int k = 0; k < 8; ++k) s += red[k][c];
-    a.colsum[blockIdx.y * a.N + n] = s;
+    if (!a.db) a.colsum[blockIdx.y * a.N + n] = s;
+    else if (a.db_f32) static_cast<float*>(a.db)[n] = s;
+    else static_cast<T*>(a.db)[n] = Elt<T>::from_f(s);
   }
 }
 
 template <typename T>
 __global__ void __launch_bounds__(256)
-colsum_finish_kernel(const float* partial, int64_t row_blocks, int64_t N, T* out) {
+colsum_finish_kernel(const float* partial, int64_t row_blocks, int64_t N, T* out, T* out2) {
   __shared__ float red[8][32];
+  if (blockIdx.y == 1) {
+    partial += row_blocks * N;
+    out = out2;
+  }
   pdl_wait_and_trigger();
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int64_t n = blockIdx.x * 32ll + tx;
@@ -260,13 +266,13 @@ cudaError_t launch_dense_dz(int dtype, const DzArgs& a, cudaStream_t s) {
 }
 
 cudaError_t launch_colsum_finish(const float* partial, int64_t row_blocks, int64_t N, void* out,
-                                 bool out_f32, cudaStream_t s) {
-  const unsigned grid = static_cast<unsigned>((N + 31) / 32);
+                                 void* out2, bool out_f32, cudaStream_t s) {
+  const dim3 grid(static_cast<unsigned>((N + 31) / 32), out2 ? 2 : 1);
   if (out_f32)
-    return launch_kernel(colsum_finish_kernel<float>, dim3(grid), dim3(256), 0, s, partial,
-                         row_blocks, N, static_cast<float*>(out));
-  return launch_kernel(colsum_finish_kernel<__nv_bfloat16>, dim3(grid), dim3(256), 0, s, partial,
-                       row_blocks, N, static_cast<__nv_bfloat16*>(out));
+    return launch_kernel(colsum_finish_kernel<float>, grid, dim3(256), 0, s, partial, row_blocks, N,
+                         static_cast<float*>(out), static_cast<float*>(out2));
+  return launch_kernel(colsum_finish_kernel<__nv_bfloat16>, grid, dim3(256), 0, s, partial, row_blocks,
+                       N, static_cast<__nv_bfloat16*>(out), static_cast<__nv_bfloat16*>(out2));
 }
 
 cudaError_t launch_pad_copy(const void* src, int64_t lds, int64_t rows, int64_t cols, void* dst,
