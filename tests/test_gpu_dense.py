@@ -282,6 +282,29 @@ def test_gated_ffn_partial_gradients():
         assert torch.allclose(one[0].float(), full[i].float(), rtol=2 ** -7, atol=1e-3), i
 
 
+@pytest.mark.parametrize("T", [6, 60, 200])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_gated_ffn_strides(T, dtype):
+    import velvetoptimizer_b200 as vb
+    H, I = 40, 56
+    gen = torch.Generator().manual_seed(0)
+    # a transposed weight, a slice with a long pitch, one that starts between 16-byte boundaries
+    wg = rand(gen, H, I, std=0.2, dtype=dtype).cuda().t()
+    wu = rand(gen, I, H + 24, std=0.2, dtype=dtype).cuda()[:, 8:8 + H]
+    wd = rand(gen, H * I + 3, std=0.2, dtype=dtype).cuda()[3:].view(H, I)
+    bs = [rand(gen, 2 * n, dtype=dtype).cuda()[::2] for n in (I, I, H)]
+    dys = list(views(gen, T, H, dtype))
+    for i, x in enumerate(views(gen, T, H, dtype)):
+        dy, r = dys[i], dys[(i + 2) % len(dys)]
+        leaves = [t.detach().requires_grad_() for t in (x, wg, wu, wd, *bs)]
+        y = vb.gated_ffn(*leaves, residual=r)
+        got = torch.autograd.grad(y, leaves, dy)
+        want = ref.gated_ffn(*(d64(t) for t in (x, wg, wu, wd, *bs)), d64(r), d64(dy), "era", GAMMA, dtype)
+        ref.check(f"y of view {i}", y, *want["y"], 2, dtype)
+        for n, g in zip(("dx", "dwg", "dwu", "dwd", "dbg", "dbu", "dbd"), got):
+            ref.check(f"{n} of view {i}", g, *want[n], 2, dtype)
+
+
 def test_far_values_stay_finite():
     """Pre-activations far out in the tails: the derivative's polynomial must not overflow."""
     import velvetoptimizer_b200 as vb
