@@ -85,6 +85,22 @@ def test_linear_f32(T, K, N, act):
     run_linear(T, K, N, act=act, dtype=F32, seed=T)
 
 
+@pytest.mark.parametrize("T,K,N", [(300, 8192, 256), (2000, 264, 40), (150, 40, 6000)])
+def test_linear_f32_long_sums(T, K, N):
+    """Sums of thousands of terms stay at fp32's own error, in every product: below 1e-6 by norm
+    (two thousand roundings to nearest of independent sign, sqrt(2000) 2^-24 = 2.7e-6, would
+    already be over; a truncating accumulator reaches 9e-6 at 8192 terms)."""
+    import velvetoptimizer_b200 as vb
+    gen = torch.Generator().manual_seed(T)
+    x, w, dy = (rand(gen, *s, dtype=F32) for s in ((T, K), (N, K), (T, N)))
+    lx, lw = leaf(x), leaf(w)
+    y = vb.linear(lx, lw)
+    dx, dw = torch.autograd.grad(y, (lx, lw), dy.cuda())
+    x, w, dy = x.double(), w.double(), dy.double()
+    for got, want in ((y, x @ w.t()), (dx, dy @ w), (dw, dy.t() @ x)):
+        assert float((d64(got) - want).norm() / want.norm()) < 1e-6
+
+
 @pytest.mark.parametrize("T", [5, 90])
 @pytest.mark.parametrize("dtype,wdtype", [(BF16, F32), (F32, BF16)])
 def test_linear_parameters_of_another_type(T, dtype, wdtype):

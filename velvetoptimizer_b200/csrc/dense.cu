@@ -242,6 +242,10 @@ struct F32Planes {
   }
 };
 
+// k blocks (64 products per output each) that an fp32 product's accumulator takes before it is
+// read out and added in registers.
+constexpr int kF32RunBlocks = 8;
+
 // C = sum over the pairs of A B, or with two groups (gated: two Bs) one product for each, then
 // the epilogue.  p.a / p.b and the pairs' lists are filled in here.
 int run_f32(Call& c, Product p, const F32Planes& planes, std::initializer_list<const F32Mat*> as,
@@ -264,7 +268,8 @@ int run_f32(Call& c, Product p, const F32Planes& planes, std::initializer_list<c
   }
   p.group_a = 3;
   p.follower_b = p.epi == kEpiGated ? 3 : 0;
-  const DenseGemm g = plan_product(c, p, true);
+  DenseGemm g = plan_product(c, p, true);
+  g.run_kb = kF32RunBlocks;
   if (c.dry) return VMOE_OK;
   TRY(launch_product(c, p, g));
   const int64_t area = p.M * g.ldp;

@@ -59,6 +59,7 @@ struct DenseGemm {
   int group_a = 0;
   int follower_b = 0;  // kEpiGated: the follower's B maps (the up weight)
   int splits = 1, kb_per_split = 0;
+  int run_kb = 1 << 30;  // partials: k blocks the tensor cores accumulate before a read-out
   int band = 0;          // n tiles per band of the tile order
   float* partial = nullptr;  // given: [splits][groups][M][ldp], and no epilogue
   int64_t ldp = 0;

@@ -98,6 +98,27 @@ __device__ __forceinline__ void arrive_remote(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
+// 8 accumulator columns of this warp's 32 lanes
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, float (&v)[8]) {
+  uint32_t r[8];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7])
+      : "r"(taddr)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// First accumulator column of the i-th 32-wide block of an epilogue warp's share (two shares;
+// gated: two blocks of gate columns, then the up columns of the same features).
+template <int EPI>
+__device__ __forceinline__ int column_of(int part, int i) {
+  return EPI == kEpiGated ? (i >> 1) * 128 + part * 64 + (i & 1) * 32 : part * 128 + i * 32;
+}
+
 struct Item {
   int g, m, n, kb, ke;
 };
@@ -422,36 +443,41 @@ gemm_dense_kernel(const __grid_constant__ DenseMaps maps, const __grid_constant_
     // ---------------- MMA issuer (leader only) ----------------
     if (leader && lane == 0) {
       int it = 0, local = 0;
-      for (int item = pair; item < total; item += num_pairs, ++local) {
+      for (int item = pair; item < total; item += num_pairs) {
         const Item w = item_of(args, item);
-        const int acc = local & 1;
-        const uint32_t aph = (local >> 1) & 1;
-        if (!mbar_wait_cluster(smem_u32(&sh->tempty[acc]), aph ^ 1)) {
-          set_abort(sh, args.status, kStatusTimeoutMma);
-          break;
-        }
-        tc_fence_after();
-        const uint32_t d_tmem = tmem + acc * BN;
         bool ok = true;
-        for (int kb = w.kb; kb < w.ke; ++kb, ++it) {
-          const int s = it % STAGES;
-          const uint32_t ph = (it / STAGES) & 1;
-          if (!mbar_wait(smem_u32(&sh->full[s]), ph)) {
+        // a split product may read its accumulator out in between (see the epilogue)
+        const int run = SPLIT ? args.run_kb : w.ke - w.kb;
+        for (int k0 = w.kb; ok && k0 < w.ke; k0 += run, ++local) {
+          const int acc = local & 1;
+          const uint32_t aph = (local >> 1) & 1;
+          if (!mbar_wait_cluster(smem_u32(&sh->tempty[acc]), aph ^ 1)) {
             set_abort(sh, args.status, kStatusTimeoutMma);
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t a_addr = a_s + s * HALF_BYTES, b_addr = b_s + s * HALF_BYTES;
+          const uint32_t d_tmem = tmem + acc * BN;
+          const int k1 = min(w.ke, k0 + run);
+          for (int kb = k0; kb < k1; ++kb, ++it) {
+            const int s = it % STAGES;
+            const uint32_t ph = (it / STAGES) & 1;
+            if (!mbar_wait(smem_u32(&sh->full[s]), ph)) {
+              set_abort(sh, args.status, kStatusTimeoutMma);
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t a_addr = a_s + s * HALF_BYTES, b_addr = b_s + s * HALF_BYTES;
 #pragma unroll
-          for (int k = 0; k < BK / 16; ++k)
-            umma_bf16_pair(d_tmem, op_desc<A_MN>(a_addr, k), op_desc<B_MN>(b_addr, k), IDESC,
-                           (kb > w.kb || k > 0) ? 1u : 0u);
-          umma_commit_pair(smem_u32(&sh->empty[s]), 0x3);  // frees the stage in both CTAs
+            for (int k = 0; k < BK / 16; ++k)
+              umma_bf16_pair(d_tmem, op_desc<A_MN>(a_addr, k), op_desc<B_MN>(b_addr, k), IDESC,
+                             (kb > k0 || k > 0) ? 1u : 0u);
+            umma_commit_pair(smem_u32(&sh->empty[s]), 0x3);  // frees the stage in both CTAs
+          }
+          if (ok) umma_commit_pair(smem_u32(&sh->tfull[acc]), 0x3);
         }
-        if (!ok) break;
-        umma_commit_pair(smem_u32(&sh->tfull[acc]), 0x3);
-        if (aborted(sh)) break;
+        if (!ok || aborted(sh)) break;
       }
       umma_commit_pair(smem_u32(&sh->done), 0x1);
       if (!mbar_wait(smem_u32(&sh->done), 0)) report(args.status, kStatusTimeoutDrain);
@@ -465,6 +491,55 @@ gemm_dense_kernel(const __grid_constant__ DenseMaps maps, const __grid_constant_
     uint8_t* turn_b = turn_a + BLOCK_BYTES;
     const DenseEpi& ep = args.epi;
     constexpr int COLS = EPI == kEpiGated ? 64 : 128;  // columns (features) of a warp's share
+    if constexpr (SPLIT) {
+      // fp32 partials in the accumulator's own column order (gated: gate | up per tile).  The
+      // tensor cores truncate when they add to the accumulator, an error that grows with the
+      // number of additions: an fp32 product is read out every run_kb k blocks and summed here,
+      // rounded to nearest (relative error of a sum over 8192: 9.1e-6 without, 4.8e-7 with; no measurable time).
+      int local = 0;
+      for (int item = pair; item < total; item += num_pairs) {
+        const Item w = item_of(args, item);
+        float v[4][32] = {};
+        bool ok = true;
+        for (int k0 = w.kb; k0 < w.ke; k0 += args.run_kb, ++local) {
+          const int acc = local & 1;
+          const bool got = mbar_wait(smem_u32(&sh->tfull[acc]), (local >> 1) & 1);
+          __syncwarp();
+          ok = __all_sync(0xffffffffu, got);
+          if (!ok) {
+            if (lane == 0) set_abort(sh, args.status, kStatusTimeoutEpilogue);
+            break;
+          }
+          tc_fence_after();
+          const uint32_t t_row = tmem + (static_cast<uint32_t>(q * 32) << 16) + acc * BN;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+#pragma unroll
+            for (int h = 0; h < 32; h += 8) {
+              float t[8];
+              tmem_ld8(t_row + column_of<EPI>(part, i) + h, t);
+#pragma unroll
+              for (int j = 0; j < 8; ++j) v[i][h + j] += t[j];
+            }
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) arrive_remote(mapa_shared(smem_u32(&sh->tempty[acc]), 0));
+        }
+        if (!ok) break;
+        const int64_t row0 = static_cast<int64_t>(w.m) * PAIR_M + rank * 128 + q * 32;
+        const int rows = static_cast<int>(args.M - row0 < 32 ? args.M - row0 : 32);
+        float* dst = args.partial +
+                     ((static_cast<int64_t>(item % args.splits) * args.groups + w.g) * args.M + row0) *
+                         args.ldp +
+                     static_cast<int64_t>(w.n) * BN;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          __syncwarp();
+          flush_f32(dst + column_of<EPI>(part, i), args.ldp, rows, 32, true, v[i], turn_a, lane);
+        }
+      }
+    } else {
     int local = 0;
     for (int item = pair; item < total; item += num_pairs, ++local) {
       const Item w = item_of(args, item);
@@ -490,8 +565,8 @@ gemm_dense_kernel(const __grid_constant__ DenseMaps maps, const __grid_constant_
       };
       // what the epilogue reads besides the accumulator is asked for before the product is done
       uint4 pre0[4], pre1[4];
-      const bool has_res = !SPLIT && EPI == kEpiLinear && ep.res;
-      if constexpr (!SPLIT && EPI == kEpiGluBwd) {
+      const bool has_res = EPI == kEpiLinear && ep.res;
+      if constexpr (EPI == kEpiGluBwd) {
         fetch16(kept(ep.z, 0), pre0, lane);
         fetch16(kept(ep.z2, 0), pre1, lane);
       } else if (has_res) {
@@ -516,25 +591,7 @@ gemm_dense_kernel(const __grid_constant__ DenseMaps maps, const __grid_constant_
 #pragma unroll 1
       for (int c = 0; c < COLS; c += 32) {
         __syncwarp();
-        if constexpr (SPLIT) {
-          // fp32 partials in the accumulator's own column order (gated: gate | up per tile)
-          const int split = item % args.splits;
-          float* dst = args.partial +
-                       ((static_cast<int64_t>(split) * args.groups + w.g) * args.M + row0) * args.ldp +
-                       static_cast<int64_t>(w.n) * BN + part * COLS + c;
-          float v[32];
-          tmem_ld32(t_row + c, v);
-          if constexpr (EPI == kEpiGated) {
-            flush_f32(dst, args.ldp, rows, 32, true, v, turn_a, lane);
-            tmem_ld32(t_row + 128 + c, v);
-            release(c);
-            __syncwarp();
-            flush_f32(dst + 128, args.ldp, rows, 32, true, v, turn_a, lane);
-          } else {
-            release(c);
-            flush_f32(dst, args.ldp, rows, 32, true, v, turn_a, lane);
-          }
-        } else if constexpr (EPI == kEpiGated) {
+        if constexpr (EPI == kEpiGated) {
           float g[32], u[32];
           tmem_ld32(t_row + c, g);
           tmem_ld32(t_row + 128 + c, u);
@@ -659,6 +716,7 @@ gemm_dense_kernel(const __grid_constant__ DenseMaps maps, const __grid_constant_
           }
         }
       }
+    }
     }
   }
 
