@@ -412,7 +412,8 @@ typedef struct vmoe_ffn_weights {
 typedef struct vmoe_ffn_grads {       /* each may be null */
   void *gate_w, *up_w, *down_w, *gate_b, *up_b, *down_b;
 } vmoe_ffn_grads;
-/* workspace of a forward or a backward, and what a training forward keeps (g, u and h) */
+/* workspace of a forward or a backward, and what a training forward keeps (g and u
+ * in fp32, h) */
 VMOE_API int vmoe_gated_ffn_workspace_size(vmoe_ops* ops, const vmoe_gated_ffn* d, int backward,
                                            size_t* bytes, size_t* saved_bytes);
 /* `saved` (256-byte aligned): null for inference, else vmoe_gated_ffn_workspace_size's

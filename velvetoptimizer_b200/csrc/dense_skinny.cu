@@ -11,6 +11,8 @@
 // adds its own tokens' parts in rank order and runs the epilogue for them.  One launch, no
 // partial sums in global memory, no atomics.  TMEM lanes are features, so a warp's stores of
 // one token are 32 consecutive features without a transpose.
+// 64 rows, cold weights, K x N: 2048 x 8192 12.8 us, 4096 x 8192 19.3 (5.2 TB/s between the two),
+// 64 x 8192 5.3, which is what launch, ring fill and exchange cost; 8192 x 2048 14.9.
 // Every mbarrier wait is bounded; a CTA that gives up still takes both cluster barriers.
 #include <atomic>
 
