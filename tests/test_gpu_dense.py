@@ -321,6 +321,82 @@ def test_gated_ffn_strides(T, dtype):
             ref.check(f"{n} of view {i}", g, *want[n], 2, dtype)
 
 
+# More than 2^31 elements in an operand.  Only the last rows (or features) have a gradient, so the
+# sums over all rows are those of the last ones: a form of their size is the whole reference.
+def last_rows(T, N, R, gen):
+    dy = torch.zeros(T, N, device="cuda", dtype=BF16)
+    dy[-R:] = rand(gen, R, N).cuda()
+    return dy
+
+
+def test_linear_rows_past_32_bits():
+    import velvetoptimizer_b200 as vb
+    T, K, N, R = 270_000, 64, 8192, 40
+    gen = torch.Generator().manual_seed(0)
+    x = rand(gen, T, K).cuda().requires_grad_()
+    w = rand(gen, N, K, std=K ** -0.5).cuda().requires_grad_()
+    b = rand(gen, N, std=0.1).cuda().requires_grad_()
+    y = vb.linear(x, w, b, activation="silu")
+    assert y.numel() > 2 ** 31
+    dy = last_rows(T, N, R, gen)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    want = ref.linear(d64(x[-R:]), d64(w), d64(b), None, d64(dy[-R:]), "silu", GAMMA, BF16)
+    ref.check("y", y[-R:], *want["y"], 1, BF16)
+    ref.check("dx", dx[-R:], *want["dx"], 3, BF16)
+    ref.check("dw", dw, *want["dw"], 3, BF16)
+    ref.check("db", db, *want["db"], 3, BF16)
+    assert not dx[:-R].any()
+    del y, dy, dx
+    torch.cuda.empty_cache()
+
+
+def test_gated_ffn_rows_past_32_bits():
+    import velvetoptimizer_b200 as vb
+    T, H, I, R = 270_000, 64, 8192, 40
+    gen = torch.Generator().manual_seed(0)
+    leaves = [t.cuda().requires_grad_() for t in (
+        rand(gen, T, H), rand(gen, I, H, std=H ** -0.5), rand(gen, I, H, std=H ** -0.5),
+        rand(gen, H, I, std=I ** -0.5), rand(gen, I, std=0.1), rand(gen, I, std=0.1),
+        rand(gen, H, std=0.1))]
+    y = vb.gated_ffn(*leaves, activation="silu")
+    dy = last_rows(T, H, R, gen)
+    got = torch.autograd.grad(y, leaves, dy)
+    want = ref.gated_ffn(d64(leaves[0][-R:]), *(d64(t) for t in leaves[1:]), None, d64(dy[-R:]), "silu",
+                         GAMMA, BF16)
+    ref.check("y", y[-R:], *want["y"], 2, BF16)
+    assert not got[0][:-R].any()
+    ref.check("dx", got[0][-R:], *want["dx"], 2, BF16)
+    for n, g in zip(("dwg", "dwu", "dwd", "dbg", "dbu", "dbd"), got[1:]):
+        ref.check(n, g, *want[n], 2, BF16)
+    del y, dy, got
+    torch.cuda.empty_cache()
+
+
+# the streaming form, the decode form and the pair form on a weight whose last rows lie that far
+@pytest.mark.parametrize("T", [1, 40, 200])
+def test_linear_weight_past_32_bits(T):
+    import velvetoptimizer_b200 as vb
+    K, N, R = 65_544, 32_840, 72
+    gen = torch.Generator().manual_seed(0)
+    x = rand(gen, T, K).cuda().requires_grad_()
+    w = torch.zeros(N, K, device="cuda", dtype=BF16)
+    w[-R:] = rand(gen, R, K, std=K ** -0.5).cuda()
+    w.requires_grad_()
+    assert w.numel() > 2 ** 31
+    y = vb.linear(x, w)
+    assert not y[:, :-R].any()
+    dy = torch.zeros(T, N, device="cuda", dtype=BF16)
+    dy[:, -R:] = rand(gen, T, R).cuda()
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    want = ref.linear(d64(x), d64(w[-R:]), None, None, d64(dy[:, -R:]), "none", GAMMA, BF16)
+    ref.check("y", y[:, -R:], *want["y"], 1, BF16)
+    ref.check("dx", dx, *want["dx"], 3, BF16)
+    ref.check("dw", dw[-R:], *want["dw"], 3, BF16)
+    assert not dw[:-R].any()
+    del w, dw
+    torch.cuda.empty_cache()
+
+
 def test_far_values_stay_finite():
     """Pre-activations far out in the tails: the derivative's polynomial must not overflow."""
     import velvetoptimizer_b200 as vb

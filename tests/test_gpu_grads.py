@@ -106,6 +106,22 @@ def test_large():
     check_clip(params(gen, [(5000, 1999), (3, 1000003), (129,)], [F32, BF16, F32]), 10.0)
 
 
+def test_tensor_past_32_bits():
+    """Ones at the ends of a tensor of more than 2^31 elements: the norm and the factor are exact."""
+    import velvetoptimizer_b200 as vb
+    n = 2 ** 31 + 4099
+    p = torch.nn.Parameter(torch.empty(n, device="cuda", dtype=BF16))
+    p.grad = torch.zeros(n, device="cuda", dtype=BF16)
+    p.grad[:2] = 1
+    p.grad[-2:] = 1
+    assert float(vb.clip_grad_norm_([p], 1.0)) == 2.0
+    # 1 / (2 + 1e-6) rounds to 0.5 as bf16
+    assert p.grad[:2].tolist() == [0.5, 0.5] and p.grad[-2:].tolist() == [0.5, 0.5]
+    assert not p.grad[2:-2].any()
+    del p
+    torch.cuda.empty_cache()
+
+
 def test_no_fp32_overflow_or_loss():
     import velvetoptimizer_b200 as vb
     for dtype, v in ((F32, 1e30), (BF16, 1e30), (F32, 1e-30)):
