@@ -1,0 +1,107 @@
+"""GPU: linear, gated_ffn and the gradient norm at the edges: row ends, non-finite values, tangents,
+tracers, status words, refusals of the C ABI."""
+import ctypes
+
+import pytest
+import torch
+
+from tests import dense_ref as ref
+from tests.test_gpu_dense import BF16, F32, GAMMA, d64, leaf, rand, run_ffn, run_linear
+
+pytestmark = pytest.mark.gpu
+
+
+# fp32 gradients of a bf16 call, at row lengths that end inside 8 columns: multiples of 4, and not
+@pytest.mark.parametrize("T", [5, 90, 300])
+@pytest.mark.parametrize("K,N", [(4, 24), (12, 40), (100, 36), (1004, 260), (260, 1004), (10, 6),
+                                 (101, 7)])
+def test_linear_f32_gradients_at_row_ends(T, K, N):
+    run_linear(T, K, N, act="silu", dtype=BF16, wdtype=F32, seed=T + K)
+
+
+@pytest.mark.parametrize("T", [5, 90, 300])
+@pytest.mark.parametrize("H,I", [(12, 40), (40, 12), (100, 36), (1004, 260), (260, 1004), (10, 6)])
+def test_gated_ffn_f32_gradients_at_row_ends(T, H, I):
+    run_ffn(T, H, I, dtype=BF16, wdtype=F32, seed=T + H)
+
+
+def ops():
+    from velvetoptimizer_b200 import _lib
+    return _lib, _lib.Ops(torch.cuda.current_device())
+
+
+GUARD = 64
+
+
+class Guarded:
+    """A buffer of n elements with words after it that must stay as they are."""
+
+    def __init__(self, shape, dtype):
+        self.n = 1
+        for s in shape:
+            self.n *= s
+        self.buf = torch.full((self.n + GUARD,), 7.0, device="cuda", dtype=dtype)
+        self.t = self.buf[:self.n].view(shape)
+
+    def ptr(self):
+        return self.buf.data_ptr()
+
+    def check(self):
+        assert (self.buf[self.n:] == 7.0).all()
+
+
+@pytest.mark.parametrize("T", [5, 90, 300])
+@pytest.mark.parametrize("K,N", [(100, 36), (4, 260), (1004, 12), (9, 5)])
+def test_nothing_is_written_past_the_gradients(T, K, N):
+    """What lies behind dW, db and dx keeps its value (linear through the C ABI)."""
+    _lib, o = ops()
+    gen = torch.Generator().manual_seed(T)
+    bf = _lib.VMOE_BF16
+    x, w, dy = rand(gen, T, K).cuda(), rand(gen, N, K).cuda(), rand(gen, T, N).cuda()
+    d = _lib.VmoeLinear(T, K, N, K, K, N, bf, 0, 0.1, _lib.VMOE_F32)
+    n = ctypes.c_size_t()
+    o.check(o.lib.vmoe_linear_workspace_size(o.ptr, d, 1, n), "size")
+    ws = torch.empty(n.value + 256, device="cuda", dtype=torch.uint8)
+    dx, dw, db = Guarded((T, K), BF16), Guarded((N, K), F32), Guarded((N,), F32)
+    stream = torch.cuda.current_stream().cuda_stream
+    o.check(o.lib.vmoe_linear_backward(o.ptr, d, x.data_ptr(), w.data_ptr(), None, dy.data_ptr(), N,
+                                       dx.ptr(), dw.ptr(), db.ptr(), ws.data_ptr(), n.value,
+                                       stream), "backward")
+    torch.cuda.synchronize()
+    want = ref.linear(d64(x), d64(w), None, None, d64(dy), "none", GAMMA, BF16, F32)
+    for name, g in (("dx", dx), ("dw", dw), ("db", db)):
+        g.check()
+        ref.check(name, g.t, *want[name], 3, BF16)
+
+
+@pytest.mark.parametrize("T", [5, 90, 300])
+@pytest.mark.parametrize("H,I", [(100, 36), (36, 100), (12, 260)])
+def test_nothing_is_written_past_the_blocks_gradients(T, H, I):
+    _lib, o = ops()
+    gen = torch.Generator().manual_seed(T)
+    bf = _lib.VMOE_BF16
+    x, dy = rand(gen, T, H).cuda(), rand(gen, T, H).cuda()
+    w = [rand(gen, *s, std=s[1] ** -0.5).cuda() for s in ((I, H), (I, H), (H, I))]
+    d = _lib.VmoeGatedFfn(T, H, I, H, H, bf, 2, 0.1, _lib.VMOE_F32)
+    n, s = ctypes.c_size_t(), ctypes.c_size_t()
+    o.check(o.lib.vmoe_gated_ffn_workspace_size(o.ptr, d, 1, n, s), "size")
+    m = ctypes.c_size_t()
+    o.check(o.lib.vmoe_gated_ffn_workspace_size(o.ptr, d, 0, m, None), "size")
+    ws = torch.empty(max(n.value, m.value) + 256, device="cuda", dtype=torch.uint8)
+    saved = torch.empty(s.value, device="cuda", dtype=torch.uint8)
+    y = Guarded((T, H), BF16)
+    shapes = dict(dx=(T, H), dwg=(I, H), dwu=(I, H), dwd=(H, I), dbg=(I,), dbu=(I,), dbd=(H,))
+    g = {k: Guarded(v, BF16 if k == "dx" else F32) for k, v in shapes.items()}
+    stream = torch.cuda.current_stream().cuda_stream
+    vw = _lib.VmoeFfnWeights(*[t.data_ptr() for t in w])
+    vg = _lib.VmoeFfnGrads(*[g[k].ptr() for k in ("dwg", "dwu", "dwd", "dbg", "dbu", "dbd")])
+    o.check(o.lib.vmoe_gated_ffn_forward(o.ptr, d, x.data_ptr(), vw, None, y.ptr(), saved.data_ptr(),
+                                         s.value, ws.data_ptr(), m.value, stream), "forward")
+    o.check(o.lib.vmoe_gated_ffn_backward(o.ptr, d, x.data_ptr(), vw, dy.data_ptr(), H, g["dx"].ptr(),
+                                          vg, saved.data_ptr(), s.value, ws.data_ptr(), n.value,
+                                          stream), "backward")
+    torch.cuda.synchronize()
+    want = ref.gated_ffn(d64(x), *map(d64, w), None, None, None, None, d64(dy), "silu", GAMMA, BF16, F32)
+    for name, t in (("y", y), *g.items()):
+        t.check()
+        ref.check(name, t.t, *want[name], 2, BF16)

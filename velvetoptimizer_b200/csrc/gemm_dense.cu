@@ -712,8 +712,11 @@ gemm_dense_kernel(const __grid_constant__ DenseMaps maps, const __grid_constant_
           }
           if (ep.out_f32) {
             __syncwarp();
+            // the columns that exist: an fp32 row is whole 16-byte units from a multiple of 4
+            // columns on, so `out`, rounded up to 8 for bf16's, may reach into the next row
+            const int cols = static_cast<int>(min(args.N - col0 - c, static_cast<int64_t>(32)));
             flush_f32(static_cast<float*>(w.g ? ep.out2 : ep.out) + row0 * ep.ldo + col0 + c, ep.ldo,
-                      rows, out.cols, out.vec, v, turn_a, lane);
+                      rows, cols, out.vec, v, turn_a, lane);
           } else {
             put_row(turn_a, v, lane);
             __syncwarp();
