@@ -380,7 +380,8 @@ VMOE_API int vmoe_linear_workspace_size(vmoe_ops* ops, const vmoe_linear* d, int
                                         size_t* bytes);
 /* y [T, N] contiguous.  z [T, N] contiguous, optional: the pre-activations x W^T + b, which
  * the backward of an activation other than VMOE_ACT_NONE reads.  bf16 x and W whose pitch is
- * a multiple of 8 must start on a 16-byte boundary (other pitches may start anywhere). */
+ * a multiple of 8 must start on a 16-byte boundary; everything else, and x and W of other
+ * pitches, may start on any element. */
 VMOE_API int vmoe_linear_forward(vmoe_ops* ops, const vmoe_linear* d, const void* x,
                                  const void* weight, const void* bias, const void* residual,
                                  void* y, void* z, void* workspace, size_t workspace_bytes,

@@ -105,3 +105,51 @@ def test_nothing_is_written_past_the_blocks_gradients(T, H, I):
     for name, t in (("y", y), *g.items()):
         t.check()
         ref.check(name, t.t, *want[name], 2, BF16)
+
+
+def test_abi_refuses_addresses_between_elements():
+    """Every operand that is read or written by elements is refused when it starts between two."""
+    _lib, o = ops()
+    buf = torch.zeros(1 << 20, device="cuda", dtype=torch.uint8)
+    p, ws, n = buf.data_ptr(), buf.data_ptr() + (1 << 19), 1 << 19
+    bad = _lib.VMOE_ERR_INVALID_ARG
+    for dtype, elt, gdtype in ((_lib.VMOE_BF16, 2, _lib.VMOE_F32), (_lib.VMOE_F32, 4, _lib.VMOE_F32)):
+        for T in (0, 4, 40):
+            d = _lib.VmoeLinear(T, 64, 64, 64, 64, 64, dtype, 2, 0.1, gdtype)
+            f = [p, p, p, p, p, p]                       # x, w, bias, residual, y, z
+            for i in range(2, 6):
+                a = list(f)
+                a[i] += elt // 2
+                if T:
+                    assert o.lib.vmoe_linear_forward(o.ptr, d, *a, ws, n, None) == bad, (dtype, i)
+            for i in range(6):                           # x, w, z, dy | lddy | dx, dw, db
+                a = [p, p, p, p, 64, p, p, p]
+                at = (2, 3, 5, 6, 7, 0)[i]
+                a[at] += 2 if at in (6, 7) else elt // 2
+                if T or at > 4:
+                    assert o.lib.vmoe_linear_backward(o.ptr, d, *a, ws, n, None) == bad, (dtype, at)
+            e = _lib.VmoeGatedFfn(T, 64, 64, 64, 64, dtype, 2, 0.1, gdtype)
+            w = [p] * 6
+            for i in (3, 4, 5, 6, 7):                    # biases, residual, y
+                a, q = list(w), [p, p]
+                if i < 6:
+                    a[i] += elt // 2
+                else:
+                    q[i - 6] += elt // 2
+                if T:
+                    assert o.lib.vmoe_gated_ffn_forward(o.ptr, e, p, _lib.VmoeFfnWeights(*a), q[0], q[1],
+                                                        None, 0, ws, n, None) == bad, (dtype, i)
+            for i in range(7):                           # gradients, dx
+                a, dx = list(w), p
+                if i < 6:
+                    a[i] += 2
+                else:
+                    dx += elt // 2
+                assert o.lib.vmoe_gated_ffn_backward(
+                    o.ptr, e, p, _lib.VmoeFfnWeights(*w), p, 64, dx, _lib.VmoeFfnGrads(*a), p, n, ws, n,
+                    None) == bad, (dtype, i)
+    ptrs, counts = (ctypes.c_void_p * 1)(p), (ctypes.c_int64 * 1)(8)
+    types = (ctypes.c_int32 * 1)(_lib.VMOE_F32)
+    assert o.lib.vmoe_grad_norm(o.ptr, ptrs, counts, types, 1, 2, 1.0, p + 2, ws, n, None) == bad
+    torch.cuda.synchronize()
+    assert not buf.any()  # nothing ran

@@ -386,6 +386,13 @@ int check_ptr(vmoe_ops* o, const char* name, const void* p, int64_t ld, int dtyp
   return VMOE_OK;
 }
 
+// an operand that is read or written element by element, or none
+int check_elt(vmoe_ops* o, const char* name, const void* p, size_t elt) {
+  if (reinterpret_cast<uintptr_t>(p) % elt)
+    return ops_fail(o, VMOE_ERR_INVALID_ARG, "%s is not aligned to its elements", name);
+  return VMOE_OK;
+}
+
 // dy [T, cols]: contiguous, or (bf16) a pitch the TMA reads in place, so that the workspace
 // size needs no pitch
 int check_dy(vmoe_ops* o, const void* dy, int64_t lddy, int64_t cols, int dtype) {
@@ -939,6 +946,11 @@ int vmoe_linear_forward(vmoe_ops* o, const vmoe_linear* d, const void* x, const 
   TRY(check_ptr(o, "weight", weight, d->ldw, d->dtype));
   if (residual) TRY(check_ld(o, "ldr", d->ldr, d->out_features));
   if (!y) return ops_fail(o, VMOE_ERR_INVALID_ARG, "y is required");
+  const size_t elt = dtype_bytes(d->dtype);
+  TRY(check_elt(o, "bias", bias, elt));
+  TRY(check_elt(o, "residual", residual, elt));
+  TRY(check_elt(o, "y", y, elt));
+  TRY(check_elt(o, "z", z, elt));
   TRY(check_workspace(o, workspace, workspace_bytes, need));
   DeviceGuard g(o->device);
   Call c{o, {static_cast<char*>(workspace), 0}, static_cast<cudaStream_t>(stream), false, d->dtype};
@@ -959,10 +971,13 @@ int vmoe_linear_backward(vmoe_ops* o, const vmoe_linear* d, const void* x, const
   if (!d) return ops_fail(o, VMOE_ERR_INVALID_ARG, "d is required");
   size_t need = 0;
   TRY(vmoe_linear_workspace_size(o, d, 1, &need));
+  const size_t gelt = dtype_bytes(d->grad_dtype);
+  TRY(check_elt(o, "dx", dx, dtype_bytes(d->dtype)));
+  TRY(check_elt(o, "dweight", dweight, gelt));
+  TRY(check_elt(o, "dbias", dbias, gelt));
   DeviceGuard g(o->device);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (d->tokens == 0) {  // sums over no rows
-    const size_t gelt = dtype_bytes(d->grad_dtype);
     cudaError_t e = cudaSuccess;
     if (dweight) e = cudaMemsetAsync(dweight, 0, d->in_features * d->out_features * gelt, s);
     if (e == cudaSuccess && dbias) e = cudaMemsetAsync(dbias, 0, d->out_features * gelt, s);
@@ -973,6 +988,7 @@ int vmoe_linear_backward(vmoe_ops* o, const vmoe_linear* d, const void* x, const
   TRY(check_dy(o, dy, lddy, d->out_features, d->dtype));
   if (d->activation != VMOE_ACT_NONE && !z)
     return ops_fail(o, VMOE_ERR_INVALID_ARG, "the activation's gradient needs z");
+  TRY(check_elt(o, "z", z, dtype_bytes(d->dtype)));
   TRY(check_workspace(o, workspace, workspace_bytes, need));
   Call c{o, {static_cast<char*>(workspace), 0}, s, false, d->dtype};
   LinearPtrs p{};
@@ -1035,6 +1051,12 @@ int vmoe_gated_ffn_forward(vmoe_ops* o, const vmoe_gated_ffn* d, const void* x,
   TRY(check_ffn_call(o, d, x, w));
   if (residual) TRY(check_ld(o, "ldr", d->ldr, d->hidden));
   if (!y) return ops_fail(o, VMOE_ERR_INVALID_ARG, "y is required");
+  const size_t elt = dtype_bytes(d->dtype);
+  TRY(check_elt(o, "gate_b", w->gate_b, elt));
+  TRY(check_elt(o, "up_b", w->up_b, elt));
+  TRY(check_elt(o, "down_b", w->down_b, elt));
+  TRY(check_elt(o, "residual", residual, elt));
+  TRY(check_elt(o, "y", y, elt));
   if (saved) TRY(check_saved(o, d, saved, saved_bytes));
   TRY(check_workspace(o, workspace, workspace_bytes, need));
   DeviceGuard g(o->device);
@@ -1056,13 +1078,16 @@ int vmoe_gated_ffn_backward(vmoe_ops* o, const vmoe_gated_ffn* d, const void* x,
   if (!d || !grads) return ops_fail(o, VMOE_ERR_INVALID_ARG, "d and grads are required");
   size_t need = 0;
   TRY(vmoe_gated_ffn_workspace_size(o, d, 1, &need, nullptr));
+  const size_t e = dtype_bytes(d->grad_dtype), m = d->hidden * d->inter * e;
+  const struct { const char* name; void* p; size_t n; } out[6] = {
+      {"d gate_w", grads->gate_w, m}, {"d up_w", grads->up_w, m}, {"d down_w", grads->down_w, m},
+      {"d gate_b", grads->gate_b, d->inter * e}, {"d up_b", grads->up_b, d->inter * e},
+      {"d down_b", grads->down_b, d->hidden * e}};
+  for (const auto& q : out) TRY(check_elt(o, q.name, q.p, e));
+  TRY(check_elt(o, "dx", dx, dtype_bytes(d->dtype)));
   DeviceGuard g(o->device);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (d->tokens == 0) {
-    const size_t e = dtype_bytes(d->grad_dtype), m = d->hidden * d->inter * e;
-    const struct { void* p; size_t n; } out[6] = {
-        {grads->gate_w, m}, {grads->up_w, m}, {grads->down_w, m}, {grads->gate_b, d->inter * e},
-        {grads->up_b, d->inter * e}, {grads->down_b, d->hidden * e}};
     for (const auto& q : out) {
       const cudaError_t rc = q.p ? cudaMemsetAsync(q.p, 0, q.n, s) : cudaSuccess;
       if (rc != cudaSuccess) return ops_cuda_fail(o, rc, "zero gradients");

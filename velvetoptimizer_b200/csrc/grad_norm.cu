@@ -335,6 +335,8 @@ int vmoe_grad_norm(vmoe_ops* o, void* const* tensors, const int64_t* counts, con
     if (!tensors[i] || reinterpret_cast<uintptr_t>(tensors[i]) % dtype_bytes(dtypes[i]))
       return ops_fail(o, VMOE_ERR_INVALID_ARG, "tensor %d is null or not aligned to its elements", i);
   }
+  if (reinterpret_cast<uintptr_t>(total_norm) % sizeof(float))
+    return ops_fail(o, VMOE_ERR_INVALID_ARG, "total_norm is not aligned to its element");
   const size_t need = norm_workspace(o, n);
   if (!workspace || workspace_bytes < need)
     return ops_fail(o, VMOE_ERR_WORKSPACE, "workspace needs %zu bytes (got %zu)", need,
