@@ -153,3 +153,21 @@ def test_abi_refuses_addresses_between_elements():
     assert o.lib.vmoe_grad_norm(o.ptr, ptrs, counts, types, 1, 2, 1.0, p + 2, ws, n, None) == bad
     torch.cuda.synchronize()
     assert not buf.any()  # nothing ran
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+def test_sizes_past_64_bits_are_refused(dtype):
+    """Sizes whose workspace would not fit 64 bits: refused, never a small number."""
+    _lib, o = ops()
+    n, s, big = ctypes.c_size_t(), ctypes.c_size_t(), (1 << 31) - 1
+    for T, K, N in ((big, big, 8), (big, 8, big), (8, big, big), (big, big, big), (1 << 20, (1 << 20) + 1, 8)):
+        d = _lib.VmoeLinear(T, K, N, K, K, N, dtype, 2, 0.1, dtype)
+        e = _lib.VmoeGatedFfn(T, K, N, K, K, dtype, 2, 0.1, dtype)
+        for backward in (0, 1):
+            assert o.lib.vmoe_linear_workspace_size(o.ptr, d, backward, n) == _lib.VMOE_ERR_UNSUPPORTED_SHAPE
+            assert o.lib.vmoe_gated_ffn_workspace_size(o.ptr, e, backward, n, s) == _lib.VMOE_ERR_UNSUPPORTED_SHAPE
+    T, I = 1 << 20, 1 << 20  # the largest: its sizes are what the formulas give
+    e = _lib.VmoeGatedFfn(T, 8, I, 8, 8, dtype, 2, 0.1, dtype)
+    assert o.lib.vmoe_gated_ffn_workspace_size(o.ptr, e, 1, n, s) == 0
+    elt = 2 if dtype == _lib.VMOE_BF16 else 4
+    assert s.value == T * I * (8 + elt) and n.value > 2 * T * I * elt

@@ -368,6 +368,15 @@ int check_dim(vmoe_ops* o, const char* name, int64_t v) {
   return VMOE_OK;
 }
 
+// A matrix of the call: below 2^40 elements, so that no size or offset derived from it (its
+// bytes, three planes, two groups of 16 splits) leaves 64 bits.
+int check_area(vmoe_ops* o, const char* name, int64_t rows, int64_t cols) {
+  if (rows > 0 && cols > (static_cast<int64_t>(1) << 40) / rows)
+    return ops_fail(o, VMOE_ERR_UNSUPPORTED_SHAPE, "%s of %lld x %lld is more than 2^40 elements",
+                    name, static_cast<long long>(rows), static_cast<long long>(cols));
+  return VMOE_OK;
+}
+
 int check_ld(vmoe_ops* o, const char* name, int64_t ld, int64_t cols) {
   if (ld < cols || ld > (static_cast<int64_t>(1) << 36))
     return ops_fail(o, VMOE_ERR_INVALID_ARG, "%s must be at least the row length %lld (got %lld)",
@@ -408,6 +417,9 @@ int check_linear(vmoe_ops* o, const vmoe_linear* d) {
   TRY(check_common(o, d->tokens, d->dtype, d->activation, d->grad_dtype, d->gamma));
   TRY(check_dim(o, "in_features", d->in_features));
   TRY(check_dim(o, "out_features", d->out_features));
+  TRY(check_area(o, "x", d->tokens, d->in_features));
+  TRY(check_area(o, "y", d->tokens, d->out_features));
+  TRY(check_area(o, "weight", d->out_features, d->in_features));
   TRY(check_ld(o, "ldx", d->ldx, d->in_features));
   return check_ld(o, "ldw", d->ldw, d->in_features);
 }
@@ -418,6 +430,9 @@ int check_ffn(vmoe_ops* o, const vmoe_gated_ffn* d) {
     return ops_fail(o, VMOE_ERR_INVALID_ARG, "the gated block needs an activation");
   TRY(check_dim(o, "hidden", d->hidden));
   TRY(check_dim(o, "inter", d->inter));
+  TRY(check_area(o, "x", d->tokens, d->hidden));
+  TRY(check_area(o, "h", d->tokens, d->inter));
+  TRY(check_area(o, "weight", d->inter, d->hidden));
   return check_ld(o, "ldx", d->ldx, d->hidden);
 }
 
