@@ -171,3 +171,23 @@ def test_sizes_past_64_bits_are_refused(dtype):
     assert o.lib.vmoe_gated_ffn_workspace_size(o.ptr, e, 1, n, s) == 0
     elt = 2 if dtype == _lib.VMOE_BF16 else 4
     assert s.value == T * I * (8 + elt) and n.value > 2 * T * I * elt
+
+
+@pytest.mark.parametrize("T", [5, 33, 300, 4001])
+@pytest.mark.parametrize("bad", [float("inf"), -float("inf")])
+def test_bias_sums_take_in_real_rows_alone(T, bad):
+    """An infinite down weight makes dh infinite, not NaN, where dy has one sign: so are the gate's
+    and the up's bias gradients, whatever the number of rows is in the last block of 32."""
+    import velvetoptimizer_b200 as vb
+    H, I = 40, 72
+    x = torch.full((T, H), 0.5, device="cuda", dtype=BF16)
+    wg, wu = (torch.full((I, H), 0.125, device="cuda", dtype=BF16) for _ in range(2))
+    wd = torch.full((H, I), 0.25, device="cuda", dtype=BF16)
+    wd[3, 7] = bad
+    bg, bu = (torch.zeros(I, device="cuda", dtype=BF16).requires_grad_() for _ in range(2))
+    y = vb.gated_ffn(x, wg, wu, wd, bg, bu, activation="silu")
+    dbg, dbu = torch.autograd.grad(y, (bg, bu), torch.ones_like(y))
+    for g in (dbg, dbu):
+        assert g[7] == bad
+        rest = torch.cat([g[:7], g[8:]])
+        assert torch.isfinite(rest).all() and (rest > 0).all()

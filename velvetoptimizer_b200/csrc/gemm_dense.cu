@@ -668,10 +668,12 @@ gemm_dense_kernel(const __grid_constant__ DenseMaps maps, const __grid_constant_
             });
             __syncwarp();
           }
+          // a row outside has zeros for dy but not for its product: 0 x infinity in the weights
+          const uint4 zero = make_uint4(0, 0, 0, 0);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            *unit16(turn_a, lane, k) = dg[k];
-            *unit16(turn_b, lane, k) = du[k];
+            *unit16(turn_a, lane, k) = lane < rows ? dg[k] : zero;
+            *unit16(turn_b, lane, k) = lane < rows ? du[k] : zero;
           }
           __syncwarp();
           flush(bg, turn_a, lane);
