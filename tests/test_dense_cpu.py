@@ -74,3 +74,39 @@ def test_context_without_gpu_is_a_clean_error():
     assert _lib.load().vmoe_ops_create(0, ctypes.byref(h)) == _lib.VMOE_ERR_CUDA and not h.value
     with pytest.raises(_lib.VmoeError):
         _lib.Ops(0)
+
+
+def elements(t):
+    """Byte offsets of a tensor's elements."""
+    at = [t.data_ptr()]
+    for n, s in zip(t.shape, t.stride()):
+        at = [a + i * s * t.element_size() for a in at for i in range(n)]
+    return {a + k for a in at for k in range(t.element_size())}
+
+
+def test_shared_memory_is_found_exactly():
+    """The overlap check of gradients that are not dense against sets of addresses."""
+    import random
+
+    from velvetoptimizer_b200.lib import _dense_ops
+    rng = random.Random(0)
+    buf = torch.zeros(4096)
+    seen = [0, 0]
+    for _ in range(4000):
+        two = []
+        for _ in range(2):
+            dims = rng.randint(1, 3)
+            shape = [rng.randint(1, 5) for _ in range(dims)]
+            stride = [rng.choice((0, 1, 2, 3, 4, 5, 8, 12, 20)) for _ in range(dims)]
+            t = torch.as_strided(buf, shape, stride, rng.randint(0, 40))
+            two.append(t.view(torch.bfloat16)[..., 1:] if stride[-1] == 1 and rng.random() < 0.3 else t)
+        a, b = two
+        want = bool(elements(a) & elements(b))
+        assert _dense_ops.share_memory(a, b) == want, (a.shape, a.stride(), b.shape, b.stride())
+        seen[want] += 1
+    assert min(seen) > 500
+    wide = torch.zeros(1000, 64)
+    assert not _dense_ops.share_memory(wide[:, :10], wide[:, 10:30])
+    assert _dense_ops.share_memory(wide[:, :11], wide[:, 10:30])
+    assert not _dense_ops.share_memory(wide[::2], wide[1::2])
+    assert _dense_ops.share_memory(wide[::2], wide[998:])

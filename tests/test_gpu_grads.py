@@ -277,3 +277,51 @@ def test_layer_step():
     (out.float().square().mean() + 0.01 * aux).backward()
     ps = list(layer.parameters())
     check_clip([q for q in ps if q.grad is not None], 1e-3)
+
+
+def test_shared_gradients_that_are_not_dense_count_once():
+    """Row-gapped, transposed and strided gradients that several parameters share."""
+    import velvetoptimizer_b200 as vb
+    gen = torch.Generator().manual_seed(0)
+    for dtype in (F32, BF16):
+        for cut in (lambda w: w[:, 10:30], lambda w: w[:, ::2], lambda w: w[::3, 1:]):
+            wide = torch.randn(40, 60, generator=gen).to(dtype).cuda()
+            was, g = wide.clone(), cut(wide)
+            want = norm64([g], 2.0)
+            assert float(vb.grad_norm([g, g])) == pytest.approx(want, rel=2.0 ** -22)
+            ps = [torch.nn.Parameter(torch.zeros_like(g)) for _ in range(3)]
+            for q in ps[:2]:
+                q.grad = g
+            ps[2] = torch.nn.Parameter(torch.zeros_like(g.t()))
+            ps[2].grad = g.t()
+            norm = vb.clip_grad_norm_([*ps, ps[0]], want / 2)
+            assert float(norm) == pytest.approx(want, rel=2.0 ** -22)
+            ref = cut(was).double() * (0.5 * want / (want + 1e-6))
+            assert ((g.double() - ref).abs() <= (U[dtype] + 2.0 ** -22) * ref.abs()).all()
+            outside = torch.ones_like(wide, dtype=torch.bool)
+            cut(outside)[:] = False
+            assert torch.equal(wide[outside], was[outside])
+
+
+def test_overlapping_gradients_that_are_not_dense_are_refused():
+    import velvetoptimizer_b200 as vb
+    wide = torch.ones(40, 60, device="cuda")
+    for a, b in ((wide, wide[:, 10:30]), (wide[:, :20], wide[:, 19:40]), (wide[::2], wide[30:]),
+                 (wide[:, ::2], wide[:, ::3]), (wide[:, 10:30], wide[5])):
+        for pair in ((a, b), (b, a)):
+            with pytest.raises(ValueError, match="overlap"):
+                vb.grad_norm(list(pair))
+            ps = [torch.nn.Parameter(torch.zeros_like(t)) for t in pair]
+            for q, t in zip(ps, pair):
+                q.grad = t
+            with pytest.raises(ValueError, match="overlap"):
+                vb.clip_grad_norm_(ps, 1.0)
+    assert (wide == 1).all()
+    # apart, however they interleave
+    parts = [wide[:, :10], wide[:, 10:30], wide[:, 30::2], wide[:, 31::2]]
+    assert float(vb.grad_norm(parts)) == pytest.approx(math.sqrt(2400))
+    ps = [torch.nn.Parameter(torch.zeros_like(t)) for t in parts]
+    for q, t in zip(ps, parts):
+        q.grad = t
+    vb.clip_grad_norm_(ps, 1.0)
+    assert torch.allclose(wide, torch.full_like(wide, 1 / math.sqrt(2400)))

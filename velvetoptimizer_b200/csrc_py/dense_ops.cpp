@@ -582,6 +582,105 @@ struct GradTable {
   }
 };
 
+// The bytes that a strided tensor covers: from `at` on, every sum of multiples of the strides,
+// outermost first; the last dimension is the run of consecutive bytes.
+struct Footprint {
+  uintptr_t at = 0, end = 0;
+  std::vector<std::pair<int64_t, int64_t>> dims;  // size, stride
+
+  explicit Footprint(const Tensor& t) : at(reinterpret_cast<uintptr_t>(t.data_ptr())) {
+    const int64_t elt = static_cast<int64_t>(t.element_size());
+    std::vector<std::pair<int64_t, int64_t>> d{{elt, 1}};
+    for (int64_t k = 0; k < t.dim(); ++k)
+      if (t.size(k) > 1 && t.stride(k) > 0) d.emplace_back(t.size(k), t.stride(k) * elt);
+    std::sort(d.begin(), d.end(), [](const auto& a, const auto& b) { return a.second > b.second; });
+    end = at + 1;
+    for (const auto& q : d) {
+      end += static_cast<uintptr_t>((q.first - 1) * q.second);
+      if (!dims.empty() && dims.back().second == q.first * q.second)
+        dims.back() = {dims.back().first * q.first, q.second};  // one run
+      else
+        dims.push_back(q);
+    }
+  }
+  bool operator==(const Footprint& o) const { return at == o.at && dims == o.dims; }
+};
+
+// Whether two footprints share a byte: is there a sum of a's multiples minus b's that equals the
+// distance of their starts?  Searched from the largest stride down; what the smaller strides can
+// reach leaves one or two multiples to try for each stride of nested layouts.  A search that gets
+// long (strides that interleave) counts as shared.
+bool share_memory(const Footprint& a, const Footprint& b) {
+  if (a.end <= b.at || b.end <= a.at) return false;
+  struct Term {
+    int64_t stride, lo, hi;  // multiples; then what the terms after this one reach
+    int64_t reach_lo = 0, reach_hi = 0;
+  };
+  std::vector<Term> terms;
+  for (const auto& q : a.dims) terms.push_back({q.second, 0, q.first - 1});
+  for (const auto& q : b.dims) {
+    auto same = std::find_if(terms.begin(), terms.end(), [&](const Term& t) { return t.stride == q.second; });
+    if (same != terms.end()) same->lo -= q.first - 1;
+    else terms.push_back({q.second, -(q.first - 1), 0});
+  }
+  std::sort(terms.begin(), terms.end(), [](const Term& x, const Term& y) { return x.stride > y.stride; });
+  for (size_t i = terms.size() - 1; i-- > 0;) {
+    const Term& n = terms[i + 1];
+    terms[i].reach_lo = n.reach_lo + n.lo * n.stride;
+    terms[i].reach_hi = n.reach_hi + n.hi * n.stride;
+  }
+  auto floor_div = [](int64_t x, int64_t y) { return x / y - (x % y < 0); };
+  int64_t steps = 0;
+  auto search = [&](auto&& self, size_t i, int64_t d) -> bool {
+    if (i == terms.size()) return d == 0;
+    if (++steps > 100000) return true;
+    const Term& t = terms[i];
+    const int64_t from = std::max(t.lo, -floor_div(t.reach_hi - d, t.stride));
+    const int64_t to = std::min(t.hi, floor_div(d - t.reach_lo, t.stride));
+    for (int64_t m = from; m <= to; ++m)
+      if (self(self, i + 1, d - m * t.stride)) return true;
+    return false;
+  };
+  return search(search, 0, static_cast<int64_t>(b.at - a.at));
+}
+
+// Of the tensors that are not dense, those whose memory no other one has; raises where one
+// shares some of its memory with another, dense ones among them.
+std::vector<Tensor> distinct(const std::vector<Tensor>& gapped, const std::vector<Tensor>& dense) {
+  struct Entry {
+    Footprint f;
+    size_t gapped;  // index, or -1
+  };
+  constexpr size_t kDense = static_cast<size_t>(-1);
+  std::vector<Entry> all;
+  all.reserve(gapped.size() + dense.size());
+  for (size_t i = 0; i < gapped.size(); ++i) all.push_back({Footprint(gapped[i]), i});
+  for (const Tensor& t : dense) all.push_back({Footprint(t), kDense});
+  std::stable_sort(all.begin(), all.end(), [](const Entry& x, const Entry& y) { return x.f.at < y.f.at; });
+  std::vector<char> keep(gapped.size(), 1);
+  std::vector<const Entry*> open;  // begun before and not ended
+  for (const Entry& e : all) {
+    open.erase(std::remove_if(open.begin(), open.end(), [&](const Entry* o) { return o->f.end <= e.f.at; }),
+               open.end());
+    bool again = false;
+    for (const Entry* o : open) {
+      if (o->gapped == kDense && e.gapped == kDense) continue;  // check_overlap's
+      if (o->gapped != kDense && e.gapped != kDense && o->f == e.f &&
+          gapped[o->gapped].scalar_type() == gapped[e.gapped].scalar_type()) {
+        again = true;
+        break;
+      }
+      TORCH_CHECK_VALUE(!share_memory(o->f, e.f), "gradients overlap in memory");
+    }
+    if (again) keep[e.gapped] = 0;
+    else open.push_back(&e);
+  }
+  std::vector<Tensor> out;
+  for (size_t i = 0; i < gapped.size(); ++i)
+    if (keep[i]) out.push_back(gapped[i]);
+  return out;
+}
+
 // The norm of the tensors of a list or tuple, or of their .grad where present (none: nothing),
 // scaled in place when max_norm >= 0.
 std::optional<Tensor> grad_norm(const py::object& items, bool use_grad, double max_norm, int norm) {
@@ -589,14 +688,18 @@ std::optional<Tensor> grad_norm(const py::object& items, bool use_grad, double m
   PyObject** p = PySequence_Fast_ITEMS(items.ptr());
   const Py_ssize_t n = PySequence_Fast_GET_SIZE(items.ptr());
   GradTable table;
-  std::vector<std::pair<Tensor, Tensor>> copies;  // not dense: a dense copy each
+  std::vector<Tensor> gapped;  // not dense
   Tensor like;
   at::NoGradGuard no_grad;
-  for (Py_ssize_t i = 0; i < n; ++i) {
-    TORCH_CHECK_TYPE(THPVariable_Check(p[i]), "expected tensors");
-    const Tensor& own = THPVariable_Unpack(p[i]);
-    const Tensor& t = use_grad ? own.grad() : own;
-    if (!t.defined()) continue;
+  auto each = [&](auto&& f) {
+    for (Py_ssize_t i = 0; i < n; ++i) {
+      TORCH_CHECK_TYPE(THPVariable_Check(p[i]), "expected tensors");
+      const Tensor& own = THPVariable_Unpack(p[i]);
+      const Tensor& t = use_grad ? own.grad() : own;
+      if (t.defined()) f(t);
+    }
+  };
+  each([&](const Tensor& t) {
     TORCH_CHECK_TYPE(t.layout() == at::kStrided, "sparse gradients are not supported");
     TORCH_CHECK_TYPE(supported(t.scalar_type()), "gradients must be float32 or bfloat16");
     TORCH_CHECK(t.is_cuda(), "gradients must be CUDA tensors (there is no CPU path)");
@@ -605,16 +708,27 @@ std::optional<Tensor> grad_norm(const py::object& items, bool use_grad, double m
     if (t.is_non_overlapping_and_dense()) {
       table.add(t);
       if (max_norm >= 0 && !t.is_inference()) torch::autograd::impl::bump_version(t);
-      continue;
+      return;
     }
+    if (t.numel() == 0) return;
     for (int64_t k = 0; max_norm >= 0 && k < t.dim(); ++k)
       TORCH_CHECK_VALUE(t.stride(k) != 0 || t.size(k) <= 1,
                         "a gradient whose elements share memory cannot be scaled in place");
-    copies.emplace_back(t, t.contiguous());
-  }
+    gapped.push_back(t);
+  });
   if (!like.defined()) return std::nullopt;
-  for (const auto& c : copies) table.add(c.second);
   table.check_overlap();
+  std::vector<std::pair<Tensor, Tensor>> copies;  // of those that are not dense: a dense copy each
+  if (!gapped.empty()) {
+    std::vector<Tensor> dense;
+    each([&](const Tensor& t) {
+      if (t.is_non_overlapping_and_dense() && t.numel() > 0) dense.push_back(t);
+    });
+    for (const Tensor& t : distinct(gapped, dense)) {
+      copies.emplace_back(t, t.contiguous());
+      table.add(copies.back().second);
+    }
+  }
   vmoe_ops* o = context(like);
   const int count = static_cast<int>(table.ptrs.size());
   size_t need = 0;
@@ -661,6 +775,9 @@ PYBIND11_MODULE(_dense_ops, m) {
   }, Release());
   m.def("gated_ffn_backward", &gated_ffn_backward, Release());
   m.def("grad_norm", &grad_norm);
+  m.def("share_memory", [](const Tensor& a, const Tensor& b) {
+    return share_memory(Footprint(a), Footprint(b));
+  });
   m.def("device_status", [](const Tensor& x) {
     int32_t code = 0;
     vmoe_ops* o = context(x);
