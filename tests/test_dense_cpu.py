@@ -110,3 +110,11 @@ def test_shared_memory_is_found_exactly():
     assert _dense_ops.share_memory(wide[:, :11], wide[:, 10:30])
     assert not _dense_ops.share_memory(wide[::2], wide[1::2])
     assert _dense_ops.share_memory(wide[::2], wide[998:])
+
+
+def test_tangents_are_refused_before_the_device():
+    import torch.autograd.forward_ad as fwd
+    with fwd.dual_level():
+        t = fwd.make_dual(torch.ones(3), torch.ones(3))
+        with pytest.raises(NotImplementedError, match="tangent"):
+            vb.grad_norm([t])

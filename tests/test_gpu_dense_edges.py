@@ -191,3 +191,38 @@ def test_bias_sums_take_in_real_rows_alone(T, bad):
         assert g[7] == bad
         rest = torch.cat([g[:7], g[8:]])
         assert torch.isfinite(rest).all() and (rest > 0).all()
+
+
+@pytest.mark.parametrize("grad", [True, False])
+@pytest.mark.parametrize("dtype,wdtype", [(BF16, BF16), (BF16, F32), (F32, F32)])
+def test_tangents_are_refused(grad, dtype, wdtype):
+    """A tangent in any argument raises; without one, calls inside a dual level run as ever."""
+    import torch.autograd.forward_ad as fwd
+
+    import velvetoptimizer_b200 as vb
+    gen = torch.Generator().manual_seed(0)
+    lin = [rand(gen, 2, 3, 16, dtype=dtype), rand(gen, 24, 16, dtype=wdtype), rand(gen, 24, dtype=wdtype),
+           rand(gen, 2, 3, 24, dtype=dtype)]
+    ffn = [rand(gen, 6, 16, dtype=dtype), rand(gen, 24, 16, dtype=wdtype), rand(gen, 24, 16, dtype=wdtype),
+           rand(gen, 16, 24, dtype=wdtype), rand(gen, 24, dtype=wdtype), rand(gen, 24, dtype=wdtype),
+           rand(gen, 16, dtype=wdtype), rand(gen, 6, 16, dtype=dtype)]
+    for fn, args in ((lambda a: vb.linear(*a[:3], residual=a[3], activation="silu"), lin),
+                     (lambda a: vb.gated_ffn(*a[:7], residual=a[7]), ffn)):
+        args = [t.cuda().requires_grad_(grad) for t in args]
+        want = fn(args)
+        with fwd.dual_level():
+            assert torch.equal(fn(args), want)
+            for i in range(len(args)):
+                a = list(args)
+                a[i] = fwd.make_dual(a[i], torch.ones_like(a[i]))
+                with pytest.raises(NotImplementedError, match="tangent"):
+                    fn(a)
+            if grad:
+                dy = fwd.make_dual(torch.ones_like(want), torch.ones_like(want))
+                with pytest.raises(NotImplementedError, match="tangent"):
+                    torch.autograd.grad(fn(args), args, dy)
+    g = torch.ones(8, device="cuda")
+    with fwd.dual_level():
+        assert float(vb.grad_norm([g])) == pytest.approx(8 ** 0.5)
+        with pytest.raises(NotImplementedError, match="tangent"):
+            vb.grad_norm([fwd.make_dual(g, g)])

@@ -94,6 +94,15 @@ Tensor packed(const Tensor& t) {
   return misaligned(m) ? m.clone(at::MemoryFormat::Contiguous) : m;
 }
 
+// Forward-mode derivatives are not computed: a tangent raises rather than being left out.
+template <typename... T>
+void no_tangents(const char* name, const T&... tensors) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  auto dual = [](const OptTensor& t) { return t && t->defined() && t->_fw_grad(/*level=*/0).defined(); };
+  TORCH_CHECK_NOT_IMPLEMENTED(!(dual(tensors) || ...), name,
+                              " has no forward-mode derivative: an argument carries a tangent");
+}
+
 const void* ptr(const OptTensor& t) { return t && t->defined() ? t->data_ptr() : nullptr; }
 
 // An uninitialised CUDA tensor, past the dispatcher
@@ -126,6 +135,7 @@ OptTensor contiguous(const OptTensor& b) {
 std::tuple<Tensor, Tensor> linear_forward(const Tensor& x_in, const Tensor& w_in,
                                           const OptTensor& bias, const OptTensor& residual,
                                           int64_t act, double gamma, bool keep) {
+  no_tangents("linear", x_in, w_in, bias, residual);
   vmoe_ops* o = context(x_in);
   vmoe_linear d{};
   d.tokens = x_in.size(0);
@@ -158,6 +168,7 @@ std::tuple<Tensor, Tensor, Tensor> linear_backward(const Tensor& x_in, const Ten
                                                    const Tensor& z, const Tensor& dy_in,
                                                    int64_t act, double gamma,
                                                    const std::vector<bool>& want, bool grad_f32) {
+  no_tangents("linear's backward", x_in, w_in, z, dy_in);
   vmoe_ops* o = context(x_in);
   vmoe_linear d{};
   d.tokens = x_in.size(0);
@@ -206,6 +217,7 @@ std::tuple<Tensor, Tensor> gated_ffn_forward(const Tensor& x_in, const Tensor& g
                                              const OptTensor& gate_b, const OptTensor& up_b,
                                              const OptTensor& down_b, const OptTensor& residual,
                                              int64_t act, double gamma, bool keep) {
+  no_tangents("gated_ffn", x_in, gate_w, up_w, down_w, gate_b, up_b, down_b, residual);
   vmoe_ops* o = context(x_in);
   vmoe_gated_ffn d = ffn_desc(x_in, gate_w.size(0), act, gamma);
   const Tensor x = rows(x_in, d.ldx);
@@ -236,6 +248,7 @@ std::array<Tensor, 7> gated_ffn_backward_array(const Tensor& x_in, const Tensor&
                                                const Tensor& saved, const Tensor& dy_in,
                                                int64_t act, double gamma,
                                                const std::vector<bool>& want, bool grad_f32) {
+  no_tangents("gated_ffn's backward", x_in, gate_w, up_w, down_w, saved, dy_in);
   vmoe_ops* o = context(x_in);
   const int64_t I = gate_w.size(0), H = x_in.size(1);
   vmoe_gated_ffn d = ffn_desc(x_in, I, act, gamma);
@@ -702,6 +715,7 @@ std::optional<Tensor> grad_norm(const py::object& items, bool use_grad, double m
   each([&](const Tensor& t) {
     TORCH_CHECK_TYPE(t.layout() == at::kStrided, "sparse gradients are not supported");
     TORCH_CHECK_TYPE(supported(t.scalar_type()), "gradients must be float32 or bfloat16");
+    no_tangents("grad_norm", t);
     TORCH_CHECK(t.is_cuda(), "gradients must be CUDA tensors (there is no CPU path)");
     if (!like.defined()) like = t;
     TORCH_CHECK_VALUE(t.device() == like.device(), "gradients must lie on one device");
