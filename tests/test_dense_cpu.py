@@ -118,3 +118,40 @@ def test_tangents_are_refused_before_the_device():
         t = fwd.make_dual(torch.ones(3), torch.ones(3))
         with pytest.raises(NotImplementedError, match="tangent"):
             vb.grad_norm([t])
+
+
+def test_the_eager_path_gives_way_to_tracers():
+    """Tracers and dispatch modes get the registered ops; subclasses in any place do too."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    from velvetoptimizer_b200.dense import _eager
+    t = torch.ones(2)
+    assert _eager(t, torch.nn.Parameter(t), None)
+    seen = []
+
+    def fn(x):
+        seen.append(_eager(t))
+        return x + 1
+
+    make_fx(fn)(t)
+    make_fx(fn, pre_dispatch=True)(t)
+    make_fx(fn, tracing_mode="fake")(t)
+    torch.jit.trace(fn, t, check_trace=False)
+
+    class Mode(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    with Mode():
+        fn(t)
+    assert seen == [False] * 5 and _eager(t)
+
+    class Sub(torch.Tensor):
+        pass
+
+    assert not _eager(t, t.as_subclass(Sub)) and not _eager(t.as_subclass(Sub), t)
+    for trace in (lambda f: make_fx(f)(t), lambda f: make_fx(f, pre_dispatch=True)(t),
+                  lambda f: torch.jit.trace(f, t, check_trace=False)):
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            trace(lambda x: vb.grad_norm([x]))

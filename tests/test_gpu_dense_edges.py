@@ -226,3 +226,50 @@ def test_tangents_are_refused(grad, dtype, wdtype):
         assert float(vb.grad_norm([g])) == pytest.approx(8 ** 0.5)
         with pytest.raises(NotImplementedError, match="tangent"):
             vb.grad_norm([fwd.make_dual(g, g)])
+
+
+def test_tracers_record_the_registered_ops():
+    """make_fx and torch.jit.trace on real tensors record the ops, not their results; a dispatch
+    mode sees them; results and gradients are the eager path's."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    import velvetoptimizer_b200 as vb
+    gen = torch.Generator().manual_seed(0)
+
+    def inputs():
+        return [rand(gen, 40, 64).cuda(), *(rand(gen, *s, std=0.1).cuda()
+                                            for s in ((72, 64), (72, 64), (64, 72), (72,)))]
+
+    def fn(x, wg, wu, wd, b):
+        return vb.linear(vb.gated_ffn(x, wg, wu, wd, b, residual=x), wg, b, activation="silu")
+
+    def step(*p):
+        p = [t.detach().requires_grad_() for t in p]
+        y = fn(*p)
+        return [y, *torch.autograd.grad(y.float().sum(), p)]
+
+    p, q = inputs(), inputs()
+    for kw in (dict(), dict(tracing_mode="fake")):
+        graph = make_fx(fn, **kw)(*p)
+        names = [str(n.target) for n in graph.graph.nodes if "vesper_moe" in str(n.target)]
+        assert [n.split(".")[1] for n in names] == ["gated_ffn_forward", "linear_forward"]
+        assert torch.equal(graph(*q), fn(*q))
+    graph = make_fx(step)(*p)
+    names = {str(n.target).split(".")[1] for n in graph.graph.nodes if "vesper_moe" in str(n.target)}
+    assert names == {f"{a}_{b}" for a in ("linear", "gated_ffn") for b in ("forward", "backward")}
+    assert all(torch.equal(a, b) for a, b in zip(graph(*q), step(*q)))
+    with torch.no_grad():
+        traced = torch.jit.trace(fn, tuple(p))
+        assert torch.equal(traced(*q), fn(*q))
+    seen = []
+
+    class Mode(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(func.__name__.split(".")[0])
+            return func(*args, **(kwargs or {}))
+
+    want = fn(*p)
+    with Mode():
+        assert torch.equal(fn(*p), want)
+    assert "linear_forward" in seen and "gated_ffn_forward" in seen

@@ -14,7 +14,10 @@
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/autograd/variable.h>
 
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <algorithm>
 #include <array>
@@ -698,6 +701,11 @@ std::vector<Tensor> distinct(const std::vector<Tensor>& gapped, const std::vecto
 // scaled in place when max_norm >= 0.
 std::optional<Tensor> grad_norm(const py::object& items, bool use_grad, double max_norm, int norm) {
   TORCH_CHECK_TYPE(PyList_Check(items.ptr()) || PyTuple_Check(items.ptr()), "expected a list or tuple");
+  // a tracer would take the norm for a constant and miss the scaling
+  TORCH_CHECK(!torch::jit::tracer::isTracing() &&
+                  !c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch) &&
+                  !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY),
+              "grad_norm and clip_grad_norm_ cannot be traced");
   PyObject** p = PySequence_Fast_ITEMS(items.ptr());
   const Py_ssize_t n = PySequence_Fast_GET_SIZE(items.ptr());
   GradTable table;
@@ -788,6 +796,13 @@ PYBIND11_MODULE(_dense_ops, m) {
     return std::make_tuple(y, keep ? saved : fresh({0}, x.options().dtype(at::kByte)));
   }, Release());
   m.def("gated_ffn_backward", &gated_ffn_backward, Release());
+  // Whether a call on plain tensors may come here past the dispatcher: no dispatch mode (make_fx,
+  // fake tensors, counters), no pre-dispatch tracing and no torch.jit.trace wants to see it.
+  m.def("eager", [] {
+    return !c10::impl::TorchDispatchModeTLS::any_modes_set() &&
+           !c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch) &&
+           !torch::jit::tracer::isTracing();
+  });
   m.def("grad_norm", &grad_norm);
   m.def("share_memory", [](const Tensor& a, const Tensor& b) {
     return share_memory(Footprint(a), Footprint(b));

@@ -48,8 +48,16 @@ def _native():
 _module = None
 
 
-def _eager(x: torch.Tensor) -> bool:
-    return type(x) in (torch.Tensor, torch.nn.Parameter) and not torch.compiler.is_compiling()
+_PLAIN = (torch.Tensor, torch.nn.Parameter, type(None))
+
+
+def _eager(*tensors: torch.Tensor | None) -> bool:
+    """Whether a call on these arguments may skip the registered ops: plain tensors all, and no
+    tracer or dispatch mode that would miss the call."""
+    for t in tensors:
+        if type(t) not in _PLAIN:
+            return False
+    return not torch.compiler.is_compiling() and _native().eager()
 
 
 # ------------------------------------------------------------------------------ the kernels
@@ -228,7 +236,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     if activation not in ACTIVATIONS:
         raise ValueError(f"linear: activation must be one of {', '.join(ACTIVATIONS)}, "
                          f"not {activation!r}")
-    if _eager(x):
+    if _eager(x, weight, bias, residual):
         return _native().linear(x, weight, bias, residual, ACTIVATIONS[activation], gamma)
     _check_x("linear", x)
     if weight.dim() != 2 or weight.shape[1] != x.shape[-1] or 0 in weight.shape:
@@ -268,7 +276,7 @@ def gated_ffn(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: torch.Tenso
     if activation == "none" or activation not in ACTIVATIONS:
         raise ValueError(f"gated_ffn: activation must be one of {', '.join(ACTIVATIONS)} but none, "
                          f"not {activation!r}")
-    if _eager(x):
+    if _eager(x, gate_weight, up_weight, down_weight, gate_bias, up_bias, down_bias, residual):
         return _native().gated_ffn(x, gate_weight, up_weight, down_weight, gate_bias, up_bias,
                                    down_bias, residual, ACTIVATIONS[activation], gamma)
     _check_x("gated_ffn", x)
