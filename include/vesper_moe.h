@@ -347,7 +347,8 @@ typedef struct vmoe_ops vmoe_ops;
 VMOE_API int vmoe_ops_create(int device, vmoe_ops** out);
 VMOE_API int vmoe_ops_destroy(vmoe_ops* ops);
 VMOE_API const char* vmoe_ops_last_error(const vmoe_ops* ops);
-/* As vmoe_device_status: reads and clears the status word, synchronises `stream`. */
+/* As vmoe_device_status: reads and clears the status word, synchronises `stream`.  The word is
+ * the device's: it tells of the kernels of every context on the context's device. */
 VMOE_API int vmoe_ops_device_status(vmoe_ops* ops, int32_t* code, void* stream);
 
 /* Activations.  gelu_tanh is GELU's tanh form; ERA = gelu_tanh + gamma * softplus

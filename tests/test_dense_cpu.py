@@ -155,3 +155,9 @@ def test_the_eager_path_gives_way_to_tracers():
                   lambda f: torch.jit.trace(f, t, check_trace=False)):
         with pytest.raises(RuntimeError, match="cannot be traced"):
             trace(lambda x: vb.grad_norm([x]))
+
+
+def test_device_status_wants_a_cuda_device():
+    for bad in ("cpu", torch.device("cpu")):
+        with pytest.raises(ValueError, match="CUDA"):
+            vb.device_status(bad)

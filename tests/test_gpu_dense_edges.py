@@ -273,3 +273,43 @@ def test_tracers_record_the_registered_ops():
     with Mode():
         assert torch.equal(fn(*p), want)
     assert "linear_forward" in seen and "gated_ffn_forward" in seen
+
+
+class OpsHead(ctypes.Structure):
+    """The beginning of struct vmoe_ops (csrc/ops_host.h)."""
+    _fields_ = [("device", ctypes.c_int), ("num_sms", ctypes.c_int), ("sm100", ctypes.c_bool),
+                ("status", ctypes.c_void_p)]
+
+
+def test_a_wait_that_gave_up_on_another_thread_is_reported():
+    """The status that a kernel of any thread's context leaves reaches every thread's question, is
+    cleared by it, and is not handed on to later contexts.  The status is written from the host."""
+    import threading
+
+    import velvetoptimizer_b200 as vb
+    from velvetoptimizer_b200.dense import _native
+    _lib = ops()[0]
+    cudart = ctypes.CDLL("libcudart.so.12")
+    index = torch.cuda.current_device()
+
+    def leave(code):
+        o = _lib.Ops(index)
+        head = ctypes.cast(o.ptr, ctypes.POINTER(OpsHead)).contents
+        assert head.device == index and head.num_sms > 0 and head.sm100
+        word = ctypes.c_int(code)
+        rc = cudart.cudaMemcpy(ctypes.c_void_p(head.status), ctypes.byref(word), ctypes.c_size_t(4), 1)
+        o.close()
+        assert rc == 0
+
+    x = torch.zeros(1, device="cuda")
+    for ask in (vb.device_status, lambda: vb.device_status(index), lambda: vb.device_status("cuda"),
+                lambda: _native().device_status(x), lambda: vb.device_status(x.device)):
+        assert ask() == 0
+        t = threading.Thread(target=leave, args=(0x103,))
+        t.start()
+        t.join()
+        with pytest.raises(_lib.VmoeError, match="0x103") as e:
+            ask()
+        assert e.value.code == _lib.VMOE_ERR_TIMEOUT
+        assert ask() == 0
+    assert _lib.Ops(index).device_status(torch.cuda.current_stream().cuda_stream) == 0

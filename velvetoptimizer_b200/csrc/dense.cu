@@ -3,7 +3,6 @@
 //
 // Every call first lays its workspace out (Arena), then launches; the size functions run the
 // same layout without a base.  Nothing is allocated and the host never waits.
-#include <atomic>
 #include <initializer_list>
 
 #include "dense.h"
@@ -11,10 +10,10 @@
 
 namespace {
 
-// Status words of the contexts, zero from the module's load on (contexts past this number
-// share them).
-constexpr int kStatusWords = 256;
-__device__ int g_ops_status[kStatusWords];
+// The status word of a device, zero from the module's load on.  One for all its contexts: a
+// gradient's kernels are launched from autograd's thread, through a context that the thread
+// which asks for the status never sees.
+__device__ int g_ops_status;
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 bool pitch16(const void* p, int64_t ld, size_t elt) {
@@ -893,20 +892,19 @@ int vmoe_ops_create(int device, vmoe_ops** out) {
   cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device);
   cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, device);
   o->sm100 = major == 10 && minor == 0;
-  // a status word of the library's own: a thread whose first call falls into a stream capture
-  // (a captured backward on autograd's thread) must allocate and clear nothing
-  static std::atomic<unsigned> next{0};
+  // the word is the library's own: a thread whose first call falls into a stream capture (a
+  // captured backward on autograd's thread) must allocate and clear nothing
   cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
   cudaThreadExchangeStreamCaptureMode(&mode);
-  void* words = nullptr;
-  const cudaError_t e = cudaGetSymbolAddress(&words, g_ops_status);
+  void* word = nullptr;
+  const cudaError_t e = cudaGetSymbolAddress(&word, g_ops_status);
   cudaThreadExchangeStreamCaptureMode(&mode);
   if (e != cudaSuccess) {
     fprintf(stderr, "vmoe_ops_create: %s\n", cudaGetErrorString(e));
     delete o;
     return VMOE_ERR_CUDA;
   }
-  o->status = static_cast<int*>(words) + next.fetch_add(1) % kStatusWords;
+  o->status = static_cast<int*>(word);
   *out = o;
   return VMOE_OK;
 }

@@ -35,6 +35,17 @@ def ops_for(device: torch.device) -> _lib.Ops:
     return o
 
 
+def device_status(device: torch.device | int | str | None = None) -> int:
+    """Whether a kernel of ``linear``, ``gated_ffn`` or their gradients on ``device`` (the current
+    one), launched from any thread, gave up a bounded wait since the last call: raises
+    ``VmoeError`` if so, and clears it.  Waits for the device's current stream.  Returns 0."""
+    if not isinstance(device, torch.device):
+        device = torch.device("cuda", device) if isinstance(device, int) else torch.device(device or "cuda")
+    if device.type != "cuda":
+        raise ValueError(f"device_status: {device} is not a CUDA device")
+    return ops_for(device).device_status(torch.cuda.current_stream(device).cuda_stream)
+
+
 def _native():
     """The host module of the eager path (csrc_py/dense_ops.cpp, built beside the library)."""
     global _module
