@@ -313,3 +313,84 @@ def test_a_wait_that_gave_up_on_another_thread_is_reported():
         assert e.value.code == _lib.VMOE_ERR_TIMEOUT
         assert ask() == 0
     assert _lib.Ops(index).device_status(torch.cuda.current_stream().cuda_stream) == 0
+
+
+def same_as_fp32(got, a, b):
+    """a @ b in fp32's infinities and NaNs, every other value within its sum's bound."""
+    got, want = got.detach().cpu(), a @ b
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isinf(), want.isinf())
+    assert torch.equal(got[want.isinf()], want[want.isinf()])
+    ok = want.isfinite()
+    a64, b64 = a.double(), b.double()
+    exact = (a64 @ b64)[ok]
+    bound = ((a64.abs() @ b64.abs()) * (a.shape[1] + 2) * 2.0 ** -23)[ok]
+    assert ((got[ok].double() - exact).abs() <= bound + 2.0 ** -24 * exact.abs()).all()
+
+
+@pytest.mark.parametrize("T,K,N", [(3, 72, 40), (40, 72, 40), (300, 72, 40), (150, 200, 130),
+                                   (40, 2048, 264), (17, 33, 300)])
+def test_f32_products_that_overflow(T, K, N):
+    """Finite operands whose products leave fp32's range: infinity, as fp32 arithmetic gives, in
+    every product and beside values as exact as ever.  All terms of such a sum have one sign, so
+    that it does not depend on their order."""
+    import velvetoptimizer_b200 as vb
+    gen = torch.Generator().manual_seed(T)
+    x, w, dy = (rand(gen, *s, dtype=F32) for s in ((T, K), (N, K), (T, N)))
+    x[2], w[5] = (x[2].abs() + 0.1) * 1.5e30, (w[5].abs() + 0.1) * 1.5e30
+    dy[1, 5], dy[2, 7] = 1.7e30, -1.7e30
+    lx, lw = leaf(x), leaf(w)
+    y = vb.linear(lx, lw)
+    dx, dw = torch.autograd.grad(y, (lx, lw), dy.cuda())
+    assert float(y[2, 5]) == float("inf") and (dx[1] == float("inf")).all() and (dw[7] == -float("inf")).all()
+    for got, a, b in ((y, x, w.t()), (dx, dy, w), (dw, dy.t(), x)):
+        same_as_fp32(got, a, b)
+
+
+@pytest.mark.parametrize("T", [3, 40, 300])
+def test_f32_products_that_just_fit(T):
+    """x y below fp32's largest number though the operands round, as bf16, to a product above it."""
+    import velvetoptimizer_b200 as vb
+    v = 2.0 ** 64 * (1 - 2.0 ** -10)
+    x, w = torch.zeros(T, 40), torch.zeros(24, 40)
+    x[1, 3], w[7, 3] = v, -v
+    y = vb.linear(x.cuda(), w.cuda(), residual=torch.ones(T, 24, device="cuda"))
+    want = torch.ones(T, 24, dtype=torch.float64)
+    want[1, 7] -= v * v
+    assert torch.isfinite(y).all()
+    assert ((y.double().cpu() - want).abs() <= 2.0 ** -23 * want.abs()).all()
+
+
+@pytest.mark.parametrize("T", [3, 40, 300])
+def test_f32_gated_products_that_overflow(T):
+    """An overflowing gate (one row), an overflowing dh (another) and overflowing weight gradients:
+    infinite where fp32 is, the other rows as ever."""
+    import velvetoptimizer_b200 as vb
+    gen = torch.Generator().manual_seed(T)
+    H, I = 40, 72
+    p = [rand(gen, *s, dtype=F32).abs() for s in ((T, H), (I, H), (I, H), (H, I))]
+    x, wg, wu, wd = p
+    dy = rand(gen, T, H, dtype=F32).abs()
+    x[2] = (x[2] + 0.1) * 1.3e30
+    wg[9] = (wg[9] + 0.1) * 1.5e30
+    wd[3] = (wd[3] + 0.1) * 1.7e20
+    dy[1, 3] = 1.9e30
+    leaves = [leaf(t) for t in p]
+    y = vb.gated_ffn(*leaves, activation="relu")
+    grads = torch.autograd.grad(y, leaves, dy.cuda())
+    ref64 = [t.double().requires_grad_() for t in p]
+    g, u = ref64[0] @ ref64[1].t(), ref64[0] @ ref64[2].t()
+    want = (torch.relu(g) * u) @ ref64[3].t()
+    exact = torch.autograd.grad(want, ref64, dy.double())
+    inf = float("inf")
+    assert (y[2] == inf).all() and (grads[0][1] == inf).all()
+    big = torch.finfo(F32).max
+    for name, a, b in zip(("y", "dx", "dwg", "dwu", "dwd"), (y, *grads), (want, *exact)):
+        a, b = a.detach().double().cpu(), b.detach()
+        over = b > big
+        assert not a.isnan().any(), name
+        assert (a[over] == inf).all(), name
+        # far from overflow in every intermediate: rows of x and dy without large values
+        rows = [i for i in range(T) if i not in (1, 2)]
+        if name in ("y", "dx"):
+            ok = b[rows] < 1e30
+            assert ((a[rows] - b[rows])[ok].abs() <= 1e-5 * b[rows][ok]).all(), name

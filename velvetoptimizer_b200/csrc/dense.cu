@@ -216,13 +216,15 @@ struct F32Mat {
   Mat plane[3];
 };
 
-// The planes of up to kMats matrices of one call, and their flags.
+// The planes of one call's matrices, and its products' redo words, which the first launch clears.
 struct F32Planes {
-  static constexpr int kMats = 8;
-  int* flags = nullptr;
-  int n = 0;
+  int* words = nullptr;
+  int used = 0;
+  bool cleared = false;
 
-  explicit F32Planes(Call& c) { flags = c.ws.take<int>(kMats * kSplitBlocks * 4); }
+  explicit F32Planes(Call& c) { words = c.ws.take<int>(kRedoWords * sizeof(int)); }
+
+  int* word() { return words ? words + used++ : nullptr; }
 
   int split(Call& c, std::initializer_list<F32Mat*> mats) {
     Split3 s[3];
@@ -234,10 +236,10 @@ struct F32Planes {
         m->plane[i] = {out ? out + i * plane : nullptr, m->rows, m->cols, ld};
       s[k++] = {m->p, m->ld, m->rows, m->cols, out, ld, plane};
     }
-    int* f = flags ? flags + n * kSplitBlocks : nullptr;
-    n += k;
+    int* clear = cleared ? nullptr : words;
+    cleared = true;
     if (c.dry) return VMOE_OK;
-    return c.run([&] { return launch_split3(s, k, f, c.s); }, "fp32 planes");
+    return c.run([&] { return launch_split3(s, k, clear, c.s); }, "fp32 planes");
   }
 };
 
@@ -247,7 +249,7 @@ constexpr int kF32RunBlocks = 8;
 
 // C = sum over the pairs of A B, or with two groups (gated: two Bs) one product for each, then
 // the epilogue.  p.a / p.b and the pairs' lists are filled in here.
-int run_f32(Call& c, Product p, const F32Planes& planes, std::initializer_list<const F32Mat*> as,
+int run_f32(Call& c, Product p, F32Planes& planes, std::initializer_list<const F32Mat*> as,
             std::initializer_list<const F32Mat*> bs) {
   TRY(check_tiles(c, p));
   const int na = static_cast<int>(as.size()), nb = static_cast<int>(bs.size());
@@ -270,33 +272,25 @@ int run_f32(Call& c, Product p, const F32Planes& planes, std::initializer_list<c
   DenseGemm g = plan_product(c, p, true);
   g.run_kb = kF32RunBlocks;
   if (c.dry) return VMOE_OK;
+  if (planes.used == kRedoWords)
+    return ops_fail(c.o, VMOE_ERR_UNSUPPORTED_SHAPE, "%s: too many products in a call", p.what);
+  g.redo = planes.word();
   TRY(launch_product(c, p, g));
-  const int64_t area = p.M * g.ldp;
-  for (int q = 0; q < (na > nb ? na : nb); ++q) {
-    const F32Mat& a = *as.begin()[na == 2 ? q : 0];
-    const F32Mat& b = *bs.begin()[nb == 2 ? q : 0];
-    SimtGemm r{};
-    r.a = a.p;
-    r.b = b.p;
-    r.am = p.a_mn ? 1 : a.ld;
-    r.ak = p.a_mn ? a.ld : 1;
-    r.bn = p.b_mn ? 1 : b.ld;
-    r.bk = p.b_mn ? b.ld : 1;
-    r.M = p.M;
-    r.N = p.N;
-    r.K = p.K;
-    r.splits = g.splits;
-    r.k_per_split = (p.K + g.splits - 1) / g.splits;
-    r.partial = g.partial + (p.groups == 2 ? q * area : 0);
-    r.ldp = g.ldp;
-    r.split_stride = p.groups * area;
-    r.gated_cols = p.epi == kEpiGated ? 1 + q : 0;
-    r.accumulate = two_pairs && q > 0;
-    r.flags = planes.flags;
-    r.n_flags = planes.n * kSplitBlocks;
-    TRY(c.run([&] { return launch_dense_simt(r, c.s); }, p.what));
+  TRY(c.run([&] { return launch_dense_finish(kF32, p.epi, g, c.s); }, p.what));
+  RedoGemm r{};
+  r.g = g;
+  const F32Mat &a = *as.begin()[0], &b = *bs.begin()[0];
+  for (int q = 0; q < 2; ++q) {
+    r.a[q] = as.begin()[na == 2 ? q : 0]->p;
+    r.b[q] = bs.begin()[nb == 2 ? q : 0]->p;
   }
-  return c.run([&] { return launch_dense_finish(kF32, p.epi, g, c.s); }, p.what);
+  r.pairs = two_pairs ? 2 : 1;
+  r.am = p.a_mn ? 1 : a.ld;  // both of a kind have one pitch
+  r.ak = p.a_mn ? a.ld : 1;
+  r.bn = p.b_mn ? 1 : b.ld;
+  r.bk = p.b_mn ? b.ld : 1;
+  r.K = p.K;
+  return c.run([&] { return launch_dense_redo(p.epi, r, c.o->num_sms, c.s); }, p.what);
 }
 
 constexpr int kDzBlocksPerSm = 6;

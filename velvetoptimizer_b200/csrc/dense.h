@@ -63,6 +63,7 @@ struct DenseGemm {
   int band = 0;          // n tiles per band of the tile order
   float* partial = nullptr;  // given: [splits][groups][M][ldp], and no epilogue
   int64_t ldp = 0;
+  int* redo = nullptr;  // fp32: set where a sum is not finite (dense_f32.cu)
   DenseEpi epi;
   int* status = nullptr;
 };
@@ -88,26 +89,19 @@ struct Split3 {
   void* out;
   int64_t ldo, plane;
 };
-constexpr int kSplitBlocks = 592;  // blocks per matrix, each with a flag
-cudaError_t launch_split3(const Split3* m, int n, int* flags, cudaStream_t s);
+constexpr int kSplitBlocks = 592;  // blocks per matrix
+constexpr int kRedoWords = 8;      // a call's products at most; `clear`: theirs to be zeroed, or null
+cudaError_t launch_split3(const Split3* m, int n, int* clear, cudaStream_t s);
 
-// fp32 products on the CUDA cores (dense_f32.cu), overwriting a product's partials, where any
-// of the n_flags flags is set: element (m, k) of A at a[m * am + k * ak], (n, k) of B at
-// b[n * bn + k * bk].
-struct SimtGemm {
-  const float *a, *b;
-  int64_t am, ak, bn, bk;
-  int64_t M, N, K;
-  int splits;
-  int64_t k_per_split;
-  float* partial;  // split s at partial + s * split_stride
-  int64_t ldp, split_stride;
-  int gated_cols;  // 0 plain; 1 / 2: gate / up columns of the 128-feature interleave
-  int accumulate;  // add to what is stored
-  const int* flags;
-  int n_flags;
+// The fp32 product `g` once more on the CUDA cores (dense_f32.cu), where its finish has found sums
+// that are not finite: element (m, k) of A at a[m * am + k * ak], (n, k) of B at b[n * bn + k * bk].
+struct RedoGemm {
+  DenseGemm g;
+  const float *a[2], *b[2];  // two pairs, one A for each group, or (gated) gate and up
+  int pairs;
+  int64_t am, ak, bn, bk, K;
 };
-cudaError_t launch_dense_simt(const SimtGemm& g, cudaStream_t s);
+cudaError_t launch_dense_redo(int epi, const RedoGemm& r, int num_sms, cudaStream_t s);
 
 // Few rows (at most kSmallTokens): weights streamed once through registers (dense_small.cu).
 constexpr int kSmallTokens = 16;

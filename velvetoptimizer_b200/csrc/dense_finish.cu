@@ -9,94 +9,33 @@
 #include "common.cuh"
 #include "dense.h"
 #include "dense_act.cuh"
+#include "dense_finish.cuh"
 
 namespace vmoe {
 namespace {
 
-constexpr int V = 8;  // columns per thread of the finish kernel
-
 template <typename T, int EPI>
 __global__ void __launch_bounds__(256)
 dense_finish_kernel(const DenseGemm g) {
-  constexpr bool kFast = sizeof(T) == 2;
   pdl_wait_and_trigger();
-  const DenseEpi& ep = g.epi;
-  const int64_t per_row = (g.N + V - 1) / V;
+  const int64_t per_row = (g.N + kChunk - 1) / kChunk;
   const int64_t total = g.M * per_row;
   const int grp = blockIdx.y;
-  const int64_t split_stride = static_cast<int64_t>(g.groups) * g.M * g.ldp;
+  bool redo = false;
   for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
-    const int64_t row = i / per_row, col = (i - row * per_row) * V;
-    const int64_t valid = g.N - col;
-    const int64_t pcol = EPI == kEpiGated ? (col / 128) * 256 + (col & 127) : col;
-    const float* p = g.partial + (static_cast<int64_t>(grp) * g.M + row) * g.ldp + pcol;
-    float v[V] = {}, u[V] = {};
-    for (int s = 0; s < g.splits; ++s, p += split_stride) {
-      float t[V];
-      load_row<V, float>(p, t, V, true);
-#pragma unroll
-      for (int j = 0; j < V; ++j) v[j] += t[j];
-      if constexpr (EPI == kEpiGated) {
-        load_row<V, float>(p + 128, t, V, true);
-#pragma unroll
-        for (int j = 0; j < V; ++j) u[j] += t[j];
+    const int64_t row = i / per_row, col = (i - row * per_row) * kChunk;
+    float v[kChunk], u[kChunk];
+    chunk_sums<EPI>(g, grp, row, col, v, u);
+    if constexpr (sizeof(T) == 4) {  // left to dense_redo_kernel
+      if (g.redo && !chunk_finite<EPI>(v, u, g.N - col)) {
+        redo = true;
+        continue;
       }
     }
-    if constexpr (EPI == kEpiGluBwd) {
-      float gg[V];
-      load_row<V>(static_cast<const float*>(ep.z) + row * ep.ldz + col, gg, valid, ep.vec & kVecZ);
-      load_row<V>(static_cast<const float*>(ep.z2) + row * ep.ldz + col, u, valid, ep.vec & kVecZ);
-      act_switch(ep.act, [&](auto A) {
-        float d[V];
-        act_grads<kFast, decltype(A)::value>(gg, d, ep.gamma);
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float a = gg[j];
-          gg[j] = v[j] * u[j] * d[j];
-          u[j] = v[j] * a;
-        }
-      });
-      store_row<V>(static_cast<T*>(ep.out) + row * ep.ldo + col, gg, valid, ep.vec & kVecOut);
-      store_row<V>(static_cast<T*>(ep.out2) + row * ep.ldo + col, u, valid, ep.vec & kVecOut);
-      continue;
-    }
-    if (ep.bias) {
-      float b[V];
-      load_row<V>(static_cast<const T*>(ep.bias) + col, b, valid, false);
-#pragma unroll
-      for (int j = 0; j < V; ++j) v[j] += b[j];
-    }
-    if constexpr (EPI == kEpiGated) {
-      if (ep.bias2) {
-        float b[V];
-        load_row<V>(static_cast<const T*>(ep.bias2) + col, b, valid, false);
-#pragma unroll
-        for (int j = 0; j < V; ++j) u[j] += b[j];
-      }
-      if (ep.z) {
-        store_row<V>(static_cast<float*>(ep.z) + row * ep.ldz + col, v, valid, ep.vec & kVecZ);
-        store_row<V>(static_cast<float*>(ep.z2) + row * ep.ldz + col, u, valid, ep.vec & kVecZ);
-      }
-      act_switch(ep.act, [&](auto A) {
-        act_values<kFast, decltype(A)::value>(v, ep.gamma);
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[j] *= u[j];
-      });
-    } else {
-      if (ep.z) store_row<V>(static_cast<T*>(ep.z) + row * ep.ldz + col, v, valid, ep.vec & kVecZ);
-      act_switch(ep.act, [&](auto A) { act_values<kFast, decltype(A)::value>(v, ep.gamma); });
-      if (ep.res) {
-        float r[V];
-        load_row<V>(static_cast<const T*>(ep.res) + row * ep.ldr + col, r, valid, ep.vec & kVecRes);
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[j] += r[j];
-      }
-    }
-    void* out = grp ? ep.out2 : ep.out;
-    if (ep.out_f32)
-      store_row<V>(static_cast<float*>(out) + row * ep.ldo + col, v, valid, ep.vec & kVecOut);
-    else
-      store_row<V>(static_cast<T*>(out) + row * ep.ldo + col, v, valid, ep.vec & kVecOut);
+    finish_chunk<T, EPI>(g, grp, row, col, v, u);
+  }
+  if constexpr (sizeof(T) == 4) {
+    if (redo) *g.redo = 1;
   }
 }
 
@@ -238,7 +177,7 @@ bool vec_ok(const void* p, int64_t ld) {
 }  // namespace
 
 cudaError_t launch_dense_finish(int dtype, int epi, const DenseGemm& g, cudaStream_t s) {
-  const dim3 grid(blocks_for(g.M * ((g.N + V - 1) / V)), static_cast<unsigned>(g.groups));
+  const dim3 grid(blocks_for(g.M * ((g.N + kChunk - 1) / kChunk)), static_cast<unsigned>(g.groups));
   cudaError_t e;
   if (dtype == kF32) {
     if (epi == kEpiGated) e = launch_kernel(dense_finish_kernel<float, kEpiGated>, grid, dim3(256), 0, s, g);
