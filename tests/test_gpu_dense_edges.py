@@ -394,3 +394,69 @@ def test_f32_gated_products_that_overflow(T):
         if name in ("y", "dx"):
             ok = b[rows] < 1e30
             assert ((a[rows] - b[rows])[ok].abs() <= 1e-5 * b[rows][ok]).all(), name
+
+
+CAPTURE = """
+import gc, torch, velvetoptimizer_b200 as vb
+torch.manual_seed(0)
+def leaf(*s): return torch.randn(*s, device="cuda").to(torch.bfloat16).requires_grad_()
+x, w, b = leaf(40, 64), leaf(72, 64), leaf(72)
+ws = [leaf(72, 64), leaf(72, 64), leaf(64, 72)]
+deep = leaf(4, 10, 64)  # reaches linear through a view
+cases = ((lambda: vb.linear(x, w, b, activation="silu"), [x, w, b]),
+         (lambda: vb.gated_ffn(x, *ws), [x, *ws]),
+         (lambda: vb.linear(deep, w), [deep, w]))
+def backward(fn, ps, how):
+    y = fn()
+    if how == "grad":
+        return torch.autograd.grad(y.float().square().sum(), ps)
+    y.float().square().sum().backward()
+for fn, ps in cases:
+    want = backward(fn, ps, "grad")
+    for how in ("grad", "backward"):
+        for p in ps: p.grad = torch.zeros_like(p)
+        alive = fn()
+        graph = torch.cuda.CUDAGraph()
+        try:
+            with torch.cuda.graph(graph):
+                backward(fn, ps, how)
+            raise SystemExit("the capture was not refused")
+        except RuntimeError as e:
+            assert "alive" in str(e), e
+        del alive, graph
+        gc.collect()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = backward(fn, ps, how)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = got or [p.grad for p in ps]
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        del graph, got
+    for p in ps: p.grad = None
+    # an eager backward with an eager graph alive is as ever, and so is a captured forward
+    alive = fn()
+    assert all(torch.equal(a, b) for a, b in zip(backward(fn, ps, "grad"), want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = fn()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, alive)
+    del alive, y, graph
+    gc.collect()
+print("captured")
+"""
+
+
+def test_captured_backward_beside_a_living_eager_graph_is_refused():
+    """It would end the process (the leaves' gradients are accumulated on the default stream); it
+    raises before that, the process goes on, and without the eager graph the capture works."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", CAPTURE], cwd=root, capture_output=True, text=True,
+                       timeout=180)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stdout + r.stderr

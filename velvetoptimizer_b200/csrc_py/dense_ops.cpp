@@ -6,9 +6,12 @@
 #include <torch/extension.h>
 
 #include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAStream.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <torch/csrc/autograd/engine.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
@@ -21,6 +24,7 @@
 
 #include <algorithm>
 #include <array>
+#include <unordered_set>
 
 #include "vesper_moe.h"
 
@@ -314,6 +318,38 @@ variable_list once(variable_list grads) {
   return grads;
 }
 
+// A gradient is accumulated on the stream that its leaf's accumulator was made on, and an eager
+// graph that is still alive keeps the accumulators of its leaves.  Where those belong to the
+// default stream, a captured backward would make that stream wait for the capture: not allowed,
+// and the end of the process.  So the backward of a capture looks at the accumulators it leads to
+// first, and raises.
+void check_capture(const torch::autograd::Node* self) {
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+  const auto* exec = torch::autograd::get_current_graph_task_exec_info();
+  std::unordered_set<const torch::autograd::Node*> seen{self};
+  std::vector<const torch::autograd::Node*> todo{self};
+  while (!todo.empty()) {
+    const auto* node = todo.back();
+    todo.pop_back();
+    for (const auto& edge : node->next_edges()) {
+      auto* next = edge.function.get();
+      if (!next || !seen.insert(next).second) continue;
+      if (exec && !exec->empty()) {
+        const auto it = exec->find(next);
+        if (it == exec->end() || !it->second.should_execute()) continue;
+      }
+      if (dynamic_cast<torch::autograd::AccumulateGrad*>(next)) {
+        const auto s = next->stream();
+        TORCH_CHECK(!s || s->id() != 0,
+                    "the backward of linear or gated_ffn is being captured while an earlier graph of "
+                    "the same leaves, made on the default stream, is alive: delete the outputs or "
+                    "losses that hold it before the capture, or make it on a side stream");
+      }
+      todo.push_back(next);
+    }
+  }
+}
+
 Tensor to_param(const Tensor& g, at::ScalarType type) {
   return g.scalar_type() == type ? g : g.to(type);
 }
@@ -346,6 +382,7 @@ struct LinearBackward : public torch::autograd::Node {
   variable_list apply(variable_list&& dys) override {
     variable_list out(4);
     if (!dys[0].defined()) return out;
+    check_capture(this);
     const bool nx = task_should_compute_output(0), nw = task_should_compute_output(1),
                nb = task_should_compute_output(2), nr = task_should_compute_output(3);
     if (nx || nw || nb) {
@@ -377,6 +414,7 @@ struct GatedFfnBackward : public torch::autograd::Node {
   variable_list apply(variable_list&& dys) override {
     variable_list out(8);
     if (!dys[0].defined()) return out;
+    check_capture(this);
     std::vector<bool> want(7);
     bool any = false;
     for (size_t i = 0; i < 7; ++i) any |= (want[i] = task_should_compute_output(i));
