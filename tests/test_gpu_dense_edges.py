@@ -460,3 +460,30 @@ def test_captured_backward_beside_a_living_eager_graph_is_refused():
     r = subprocess.run([sys.executable, "-c", CAPTURE], cwd=root, capture_output=True, text=True,
                        timeout=180)
     assert r.returncode == 0 and "captured" in r.stdout, r.stdout + r.stderr
+
+
+@pytest.mark.parametrize("change", [lambda m: m.cpu(), lambda m: m.double(), lambda m: m.half(),
+                                    lambda m: m.cpu().double()])
+def test_feed_forward_takes_parameters_of_any_kind(change):
+    """In grad mode and under no_grad alike: parameters of another device or floating type than
+    the kernels read; their gradients come back in their own place and type."""
+    from tests.test_gpu_dense import module_inputs
+    m, x, dy = module_inputs(BF16, F32)
+    with torch.no_grad():
+        for p in m.parameters():
+            p.copy_(p.half())  # exact in every type
+    want = torch.autograd.grad(m(x, residual=x), list(m.parameters()), dy)
+    plain = m(x)
+    m = change(m)
+    with torch.no_grad():
+        packed = m(x)
+    # two roundings each (h and out), and the packed path's tanh.approx (2^-11)
+    assert float((packed.float() - plain.detach().float()).norm() / plain.detach().float().norm()) <= 4 * 2.0 ** -8
+    # the fold's last bit may differ with its device and type, and with it a folded weight's
+    # rounding to bf16: one step of 2^-8 at most in y and in the gradients
+    near = lambda a, b: float((a.double().cpu() - b.double().cpu()).norm() / b.double().norm())  # noqa: E731
+    assert near(m(x).detach(), plain.detach()) <= 2.0 ** -8
+    got = torch.autograd.grad(m(x, residual=x), list(m.parameters()), dy)
+    for p, g, w in zip(m.parameters(), got, want):
+        assert g.dtype == p.dtype and g.device == p.device
+        assert near(g, w) <= 2.0 ** -8 + 2.0 ** -11

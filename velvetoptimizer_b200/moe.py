@@ -453,10 +453,12 @@ class FeedForward(_PackedHandleMixin, nn.Module):
         wants_grad = torch.is_grad_enabled() and (
             x.requires_grad or any(p.requires_grad for p in self._param_list()))
         if residual is not None or (wants_grad and x.dtype == torch.bfloat16):
-            gate_w, gate_b = self.gate_proj.folded()
-            up_w, up_b = self.up_proj.folded()
-            return gated_ffn(x, gate_w, up_w, self.down_proj.weight, gate_b, up_b,
-                             self.down_proj.bias, residual=residual, activation="era",
+            # as the packed path takes them: parameters of any floating type, on any device
+            there = lambda p: p.to(x.device, p.dtype if p.dtype in _DTYPES else torch.float32)  # noqa: E731
+            gate_w, gate_b = map(there, self.gate_proj.folded())
+            up_w, up_b = map(there, self.up_proj.folded())
+            return gated_ffn(x, gate_w, up_w, there(self.down_proj.weight), gate_b, up_b,
+                             there(self.down_proj.bias), residual=residual, activation="era",
                              gamma=self.config.era_gamma)
         if wants_grad and not getattr(self, "_warned_fp32_grad", False):
             warnings.warn("velvetoptimizer_b200.FeedForward: the backward runs on bfloat16 inputs "
