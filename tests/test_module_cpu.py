@@ -179,3 +179,26 @@ def test_native_pairs_match_the_parameters():
     assert moe._native_pairs(plist) != raw
     with pytest.raises(TypeError):
         moe._native_pairs([1, 2])
+
+
+def test_host_modules_are_built_with_cxx(tmp_path, monkeypatch):
+    """$CXX is honoured, and the module takes the shared libstdc++ whatever $CXX would link."""
+    import os
+    import subprocess
+    import sys
+
+    from velvetoptimizer_b200 import build
+    real = os.environ.get("CXX") or "g++"
+    cxx = tmp_path / "cxx"
+    cxx.write_text(f'#!/bin/sh\necho called >> {tmp_path}/log\nexec {real} "$@"\n')
+    cxx.chmod(0o755)
+    monkeypatch.setenv("CXX", str(cxx))
+    monkeypatch.setattr(build, "LIB_DIR", str(tmp_path))
+    out = build.build_host_module("param_key")
+    assert (tmp_path / "log").read_text() == "called\n" and os.path.dirname(out) == str(tmp_path)
+    code = (f"import torch, importlib.util as u; s = u.spec_from_file_location('_param_key', {out!r}); "
+            "m = u.module_from_spec(s); s.loader.exec_module(m); print(len(m.pairs([torch.zeros(2)])))")
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True)
+    assert r.stdout.split() == ["16"], r.stderr
+    with open(out, "rb") as f:
+        assert b"libstdc++.so.6" in f.read()

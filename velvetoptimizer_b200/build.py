@@ -83,15 +83,16 @@ def build_host_module(name: str, force: bool = False, verbose: bool = False) -> 
     tdir = os.path.dirname(torch.__file__)
     abi = int(getattr(torch._C, "_GLIBCXX_USE_CXX11_ABI", True))
     cuda = os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include")
-    # the host compiler nvcc takes, before $CXX: a toolchain that links libstdc++ statically
-    # would give the module streams and locales of its own, apart from torch's
-    cmd = [shutil.which("g++") or os.environ["CXX"], "-O2", "-std=c++17", "-fPIC", "-shared",
+    cmd = [os.environ.get("CXX") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared",
            "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
            "-I", sysconfig.get_paths()["include"], "-I", INCLUDE, "-I", cuda,
            "-I", os.path.join(tdir, "include"),
            "-I", os.path.join(tdir, "include", "torch", "csrc", "api", "include"),
            src, "-o", out + ".tmp", "-L", os.path.join(tdir, "lib"),
-           "-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_python"]
+           "-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_python",
+           # the libstdc++ that torch has loaded, also where $CXX would link one statically: the
+           # module's streams, locales and exceptions are then torch's
+           "-l:libstdc++.so.6"]
     if name == "dense_ops":  # calls the C ABI library beside it
         cmd += ["-lc10_cuda", "-ltorch_cuda", LIB, "-Wl,-rpath,$ORIGIN"]
     cmd += [f"-Wl,-rpath,{os.path.join(tdir, 'lib')}"]
