@@ -340,9 +340,10 @@ VMOE_API int vmoe_ffn_forward(vmoe_handle* h, const void* x, int64_t tokens, voi
  * layout: nothing is packed or kept between calls, so a training loop that changes its
  * weights every step calls them as they are.  They run on a vmoe_ops context: one per device
  * and calling thread (calls on one context must not overlap; two contexts may run at once,
- * each call with its own workspace).  bf16 needs an sm_100 GPU; every product accumulates in
- * fp32.  Each function returns a status code, enqueues its work on `stream` and allocates
- * nothing; vmoe_ops_last_error has the text of the last failure. */
+ * each call with its own workspace).  They need an sm_100 GPU (fp32 products of more than
+ * 16 rows run on its tensor cores too); every product accumulates in fp32.  Each function
+ * returns a status code, enqueues its work on `stream` and allocates nothing;
+ * vmoe_ops_last_error has the text of the last failure. */
 typedef struct vmoe_ops vmoe_ops;
 VMOE_API int vmoe_ops_create(int device, vmoe_ops** out);
 VMOE_API int vmoe_ops_destroy(vmoe_ops* ops);

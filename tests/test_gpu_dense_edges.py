@@ -487,3 +487,18 @@ def test_feed_forward_takes_parameters_of_any_kind(change):
     for p, g, w in zip(m.parameters(), got, want):
         assert g.dtype == p.dtype and g.device == p.device
         assert near(g, w) <= 2.0 ** -8 + 2.0 ** -11
+
+
+def test_another_architecture_is_refused_in_both_types():
+    _lib, o = ops()
+    ctypes.cast(o.ptr, ctypes.POINTER(OpsHead)).contents.sm100 = False
+    n = ctypes.c_size_t()
+    for dtype in (_lib.VMOE_F32, _lib.VMOE_BF16):
+        for backward in (0, 1):
+            d = _lib.VmoeLinear(40, 64, 64, 64, 64, 64, dtype, 2, 0.1, dtype)
+            e = _lib.VmoeGatedFfn(40, 64, 64, 64, 64, dtype, 2, 0.1, dtype)
+            with pytest.raises(_lib.VmoeError, match="sm_100") as err:
+                o.check(o.lib.vmoe_linear_workspace_size(o.ptr, d, backward, n), "size")
+            assert err.value.code == _lib.VMOE_ERR_UNSUPPORTED_SHAPE
+            with pytest.raises(_lib.VmoeError, match="sm_100"):
+                o.check(o.lib.vmoe_gated_ffn_workspace_size(o.ptr, e, backward, n, None), "size")

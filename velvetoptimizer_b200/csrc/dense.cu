@@ -349,8 +349,8 @@ int check_common(vmoe_ops* o, int64_t T, int32_t dtype, int32_t act, int32_t gra
     return ops_fail(o, VMOE_ERR_INVALID_ARG, "unknown activation %d", act);
   if (act == VMOE_ACT_ERA && !(gamma - gamma == 0.f))
     return ops_fail(o, VMOE_ERR_INVALID_ARG, "gamma must be finite");
-  if (dtype == VMOE_BF16 && !o->sm100)
-    return ops_fail(o, VMOE_ERR_UNSUPPORTED_SHAPE, "the bf16 path needs an sm_100 GPU");
+  if (!o->sm100)  // fp32 products run on the tensor cores too
+    return ops_fail(o, VMOE_ERR_UNSUPPORTED_SHAPE, "the dense operators need an sm_100 GPU");
   return VMOE_OK;
 }
 

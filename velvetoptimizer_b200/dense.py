@@ -5,8 +5,9 @@ the reference's dense feed-forward block (python/vesper/model.py:249-270) with i
 Both read the weights where they are, in ``nn.Linear``'s layout: nothing is packed or kept
 between calls, so weights that change every step need no repacking.  They run on torch's
 current stream of x's device through the C ABI (``vmoe_linear_*``, ``vmoe_gated_ffn_*``).
-bfloat16 runs on the tensor cores, float32 on the CUDA cores; everything accumulates in fp32.
-There is no CPU path.
+bfloat16 runs on the tensor cores; float32 does too, as six bfloat16 products, except for up to 16
+rows in a forward and for sums that are not finite, which take the CUDA cores.  Everything
+accumulates in fp32.  They need an sm_100 GPU; there is no CPU path.
 
 Parameters may have another floating type than x (fp32 masters of a bf16 step): they are cast
 to x's type for the call, and their gradients come back in their own type, from fp32 sums.
