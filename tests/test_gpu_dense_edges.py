@@ -502,3 +502,27 @@ def test_another_architecture_is_refused_in_both_types():
             assert err.value.code == _lib.VMOE_ERR_UNSUPPORTED_SHAPE
             with pytest.raises(_lib.VmoeError, match="sm_100"):
                 o.check(o.lib.vmoe_gated_ffn_workspace_size(o.ptr, e, backward, n, None), "size")
+
+
+@pytest.mark.parametrize("T", [4, 40, 200])
+def test_negated_views(T):
+    """Views that torch negates when they are read, in every place."""
+    import velvetoptimizer_b200 as vb
+    gen = torch.Generator().manual_seed(0)
+    for dtype in (F32, BF16):
+        x, w, b, r, dy = (rand(gen, *s, dtype=dtype).cuda()
+                          for s in ((T, 64), (72, 64), (72,), (T, 72), (T, 72)))
+        ws = [rand(gen, *s, dtype=dtype).cuda() for s in ((72, 64), (72, 64), (64, 72), (72,), (72,), (64,))]
+        for neg in (lambda t: torch._neg_view(-t), lambda t: t):
+            def run():
+                p = [neg(t).detach().requires_grad_() for t in (x, w, b, *ws)]
+                y = vb.linear(*p[:3], residual=neg(r), activation="silu")
+                z = vb.gated_ffn(p[0], *p[3:], residual=neg(x))
+                g = torch.autograd.grad((y, z), p, (neg(dy), neg(x)))
+                return [t.resolve_neg() for t in (y, z, *g)]
+            if neg(x).is_neg():
+                got = run()
+            else:
+                assert all(torch.equal(a, c) for a, c in zip(got, run()))
+        g = torch._neg_view(x.clone())
+        assert torch.equal(vb.grad_norm([g]), vb.grad_norm([x]))

@@ -72,9 +72,14 @@ bool supported(at::ScalarType t) { return t == at::kFloat || t == at::kBFloat16;
 
 bool misaligned(const Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) != 0; }
 
+// A view whose elements are negated only when they are read (an imaginary part of a conjugate)
+// as a tensor of its own
+Tensor plain(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+
 // The matrix as the kernels read it, and its row pitch: itself where its rows are contiguous
 // (and 16-byte aligned where the pitch is), else a contiguous copy.
-Tensor rows(const Tensor& t, int64_t& ld) {
+Tensor rows(const Tensor& view, int64_t& ld) {
+  const Tensor t = plain(view);
   const int64_t r = t.size(0), c = t.size(1), s0 = t.stride(0), s1 = t.stride(1);
   if ((s1 == 1 || c == 1) && (r <= 1 || s0 >= c)) {
     ld = r > 1 ? s0 : c;
@@ -97,7 +102,7 @@ Tensor grad_rows(const Tensor& t, int64_t& ld) {
 }
 
 Tensor packed(const Tensor& t) {
-  Tensor m = t.contiguous();
+  Tensor m = plain(t).contiguous();
   return misaligned(m) ? m.clone(at::MemoryFormat::Contiguous) : m;
 }
 
@@ -134,7 +139,7 @@ void* stream_of(const Tensor& x) {
 }
 
 OptTensor contiguous(const OptTensor& b) {
-  return b && b->defined() ? OptTensor(b->contiguous()) : std::nullopt;
+  return b && b->defined() ? OptTensor(plain(*b).contiguous()) : std::nullopt;
 }
 
 // ---- linear -----------------------------------------------------------------------------
