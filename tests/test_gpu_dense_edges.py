@@ -526,3 +526,20 @@ def test_negated_views(T):
                 assert all(torch.equal(a, c) for a, c in zip(got, run()))
         g = torch._neg_view(x.clone())
         assert torch.equal(vb.grad_norm([g]), vb.grad_norm([x]))
+
+
+@pytest.mark.parametrize("T", [8, 100, 400])
+def test_era_far_down(T):
+    """bf16 ERA below zero, where softplus is log2(1 + e^z): its logarithm is off by at most 2^-22
+    near 1, so y by gamma 2^-22 beside its rounding; it ends in 0, never below."""
+    import velvetoptimizer_b200 as vb
+    z = torch.linspace(-40, -5, T).to(BF16)
+    y = vb.linear(z[:, None].cuda(), torch.ones(8, 1, device="cuda", dtype=BF16), activation="era",
+                  gamma=GAMMA)
+    v = z.double()[:, None].expand(T, 8)
+    gelu = v * torch.sigmoid(1.5957691216057308 * (v + 0.044715 * v ** 3))
+    want = gelu + GAMMA * torch.log1p(torch.exp(v))
+    bound = 2.0 ** -8 * want.abs() + GAMMA * 2.0 ** -22 + 2.0 ** -18 * gelu.abs()
+    got = y.double().cpu()
+    assert ((got - want).abs() <= bound).all()
+    assert (got[z < -20] >= 0).all() and (got[z < -20] <= GAMMA * 2.0 ** -22).all()
