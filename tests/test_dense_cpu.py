@@ -121,17 +121,19 @@ def test_tangents_are_refused_before_the_device():
 
 
 def test_the_eager_path_gives_way_to_tracers():
-    """Tracers and dispatch modes get the registered ops; subclasses in any place do too."""
+    """Tracers and dispatch modes get the registered ops; tensors with a dispatch of their own, in
+    any place, do too."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
     from torch.fx.experimental.proxy_tensor import make_fx
     from torch.utils._python_dispatch import TorchDispatchMode
 
-    from velvetoptimizer_b200.dense import _eager
+    from velvetoptimizer_b200.lib._dense_ops import eager
     t = torch.ones(2)
-    assert _eager(t, torch.nn.Parameter(t), None)
+    assert eager(t, torch.nn.Parameter(t))
     seen = []
 
     def fn(x):
-        seen.append(_eager(t))
+        seen.append(eager(t, t))
         return x + 1
 
     make_fx(fn)(t)
@@ -145,12 +147,9 @@ def test_the_eager_path_gives_way_to_tracers():
 
     with Mode():
         fn(t)
-    assert seen == [False] * 5 and _eager(t)
-
-    class Sub(torch.Tensor):
-        pass
-
-    assert not _eager(t, t.as_subclass(Sub)) and not _eager(t.as_subclass(Sub), t)
+    assert seen == [False] * 5 and eager(t, t)
+    fake = FakeTensorMode().from_tensor(t)
+    assert not eager(t, fake) and not eager(fake, t)
     for trace in (lambda f: make_fx(f)(t), lambda f: make_fx(f, pre_dispatch=True)(t),
                   lambda f: torch.jit.trace(f, t, check_trace=False)):
         with pytest.raises(RuntimeError, match="cannot be traced"):
@@ -161,3 +160,20 @@ def test_device_status_wants_a_cuda_device():
     for bad in ("cpu", torch.device("cpu")):
         with pytest.raises(ValueError, match="CUDA"):
             vb.device_status(bad)
+
+
+def test_what_is_no_tensor_is_refused():
+    x, w = torch.zeros(2, 8), torch.zeros(4, 8)
+    for bad in ([1.0], 2.0, "x"):
+        with pytest.raises(TypeError):
+            vb.linear(bad, w)
+        with pytest.raises(TypeError):
+            vb.linear(x, w, bad)
+        with pytest.raises(TypeError):
+            vb.gated_ffn(x, w, bad, w.t())
+    with pytest.raises(TypeError):
+        vb.linear(None, w)
+    with pytest.raises(TypeError):
+        vb.linear(x, None)
+    with pytest.raises(TypeError):
+        vb.linear(x, w, activation="silu", gamma="a")

@@ -364,7 +364,7 @@ int check_dim(vmoe_ops* o, const char* name, int64_t v) {
 // A matrix of the call: below 2^40 elements, so that no size or offset derived from it (its
 // bytes, three planes, two groups of 16 splits) leaves 64 bits.
 int check_area(vmoe_ops* o, const char* name, int64_t rows, int64_t cols) {
-  if (rows > 0 && cols > (static_cast<int64_t>(1) << 40) / rows)
+  if (rows * cols > static_cast<int64_t>(1) << 40)  // both are below 2^31
     return ops_fail(o, VMOE_ERR_UNSUPPORTED_SHAPE, "%s of %lld x %lld is more than 2^40 elements",
                     name, static_cast<long long>(rows), static_cast<long long>(cols));
   return VMOE_OK;
@@ -383,14 +383,14 @@ int check_ptr(vmoe_ops* o, const char* name, const void* p, int64_t ld, int dtyp
   if (!p) return ops_fail(o, VMOE_ERR_INVALID_ARG, "%s is required", name);
   if (dtype == VMOE_BF16 && ld % 8 == 0 && !aligned16(p))
     return ops_fail(o, VMOE_ERR_INVALID_ARG, "%s must be 16-byte aligned", name);
-  if (reinterpret_cast<uintptr_t>(p) % dtype_bytes(dtype))
+  if (reinterpret_cast<uintptr_t>(p) & (dtype_bytes(dtype) - 1))
     return ops_fail(o, VMOE_ERR_INVALID_ARG, "%s is not aligned to its elements", name);
   return VMOE_OK;
 }
 
 // an operand that is read or written element by element, or none
 int check_elt(vmoe_ops* o, const char* name, const void* p, size_t elt) {
-  if (reinterpret_cast<uintptr_t>(p) % elt)
+  if (reinterpret_cast<uintptr_t>(p) & (elt - 1))
     return ops_fail(o, VMOE_ERR_INVALID_ARG, "%s is not aligned to its elements", name);
   return VMOE_OK;
 }

@@ -110,7 +110,12 @@ Tensor packed(const Tensor& t) {
 template <typename... T>
 void no_tangents(const char* name, const T&... tensors) {
   if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
-  auto dual = [](const OptTensor& t) { return t && t->defined() && t->_fw_grad(/*level=*/0).defined(); };
+  auto dual = [](const auto& t) {
+    if constexpr (std::is_same_v<std::decay_t<decltype(t)>, Tensor>)
+      return t.defined() && t._fw_grad(/*level=*/0).defined();
+    else
+      return t && t->defined() && t->_fw_grad(/*level=*/0).defined();
+  };
   TORCH_CHECK_NOT_IMPLEMENTED(!(dual(tensors) || ...), name,
                               " has no forward-mode derivative: an argument carries a tangent");
 }
@@ -810,6 +815,22 @@ std::optional<Tensor> grad_norm(const py::object& items, bool use_grad, double m
   return out;
 }
 
+// Whether a call on these tensors may go past the dispatcher: none has a __torch_dispatch__ of its
+// own, and no dispatch mode (make_fx, fake tensors, counters), pre-dispatch tracing or
+// torch.jit.trace would miss the call.
+template <typename... T>
+bool eager(const T&... tensors) {
+  auto own = [](const auto& t) {
+    if constexpr (std::is_same_v<std::decay_t<decltype(t)>, Tensor>)
+      return t.key_set().has(c10::DispatchKey::Python);
+    else
+      return t && t->defined() && t->key_set().has(c10::DispatchKey::Python);
+  };
+  return !(own(tensors) || ...) && !c10::impl::TorchDispatchModeTLS::any_modes_set() &&
+         !c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch) &&
+         !torch::jit::tracer::isTracing();
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_dense_ops, m) {
@@ -823,8 +844,19 @@ PYBIND11_MODULE(_dense_ops, m) {
     }
   });
   using Release = py::call_guard<py::gil_scoped_release>;
-  m.def("linear", &linear, Release());
-  m.def("gated_ffn", &gated_ffn, Release());
+  // None where the call is not the eager path's (see `eager`)
+  m.def("linear", [](const Tensor& x, const Tensor& w, const OptTensor& b, const OptTensor& r, int64_t act,
+                     double gamma) {
+    return eager(x, w, b, r) ? OptTensor(linear(x, w, b, r, act, gamma)) : std::nullopt;
+  }, Release());
+  m.def("gated_ffn", [](const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& wd,
+                        const OptTensor& bg, const OptTensor& bu, const OptTensor& bd, const OptTensor& r,
+                        int64_t act, double gamma) {
+    return eager(x, wg, wu, wd, bg, bu, bd, r)
+               ? OptTensor(gated_ffn(x, wg, wu, wd, bg, bu, bd, r, act, gamma))
+               : std::nullopt;
+  }, Release());
+  m.def("eager", [](const Tensor& x, const Tensor& w) { return eager(x, w); });
   // the tracers' ops return a tensor in every place
   m.def("linear_forward", [](const Tensor& x, const Tensor& w, const OptTensor& b, const OptTensor& r,
                              int64_t act, double gamma, bool keep) {
@@ -839,13 +871,6 @@ PYBIND11_MODULE(_dense_ops, m) {
     return std::make_tuple(y, keep ? saved : fresh({0}, x.options().dtype(at::kByte)));
   }, Release());
   m.def("gated_ffn_backward", &gated_ffn_backward, Release());
-  // Whether a call on plain tensors may come here past the dispatcher: no dispatch mode (make_fx,
-  // fake tensors, counters), no pre-dispatch tracing and no torch.jit.trace wants to see it.
-  m.def("eager", [] {
-    return !c10::impl::TorchDispatchModeTLS::any_modes_set() &&
-           !c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch) &&
-           !torch::jit::tracer::isTracing();
-  });
   m.def("grad_norm", &grad_norm);
   m.def("share_memory", [](const Tensor& a, const Tensor& b) {
     return share_memory(Footprint(a), Footprint(b));

@@ -60,16 +60,7 @@ def _native():
 _module = None
 
 
-_PLAIN = (torch.Tensor, torch.nn.Parameter, type(None))
-
-
-def _eager(*tensors: torch.Tensor | None) -> bool:
-    """Whether a call on these arguments may skip the registered ops: plain tensors all, and no
-    tracer or dispatch mode that would miss the call."""
-    for t in tensors:
-        if type(t) not in _PLAIN:
-            return False
-    return not torch.compiler.is_compiling() and _native().eager()
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
 
 
 # ------------------------------------------------------------------------------ the kernels
@@ -211,6 +202,8 @@ class _GatedFfnFn(torch.autograd.Function):
 # ------------------------------------------------------------------------------ the operators
 # The eager path checks the same in C++.
 def _check_x(name: str, x: torch.Tensor) -> None:
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"{name}: x must be a tensor, not {type(x).__name__}")
     if x.device.type != "cuda":
         raise RuntimeError(f"{name} runs on CUDA tensors only (there is no CPU path)")
     if x.dtype not in _DTYPES:
@@ -248,8 +241,10 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     if activation not in ACTIVATIONS:
         raise ValueError(f"linear: activation must be one of {', '.join(ACTIVATIONS)}, "
                          f"not {activation!r}")
-    if _eager(x, weight, bias, residual):
-        return _native().linear(x, weight, bias, residual, ACTIVATIONS[activation], gamma)
+    if type(x) in _PLAIN and not torch.compiler.is_compiling():
+        y = _native().linear(x, weight, bias, residual, ACTIVATIONS[activation], gamma)
+        if y is not None:  # None: a tracer, a dispatch mode or a subclass wants the registered op
+            return y
     _check_x("linear", x)
     if weight.dim() != 2 or weight.shape[1] != x.shape[-1] or 0 in weight.shape:
         raise ValueError(f"linear: weight must be [N, {x.shape[-1]}] with N and K at least 1, "
@@ -288,9 +283,11 @@ def gated_ffn(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: torch.Tenso
     if activation == "none" or activation not in ACTIVATIONS:
         raise ValueError(f"gated_ffn: activation must be one of {', '.join(ACTIVATIONS)} but none, "
                          f"not {activation!r}")
-    if _eager(x, gate_weight, up_weight, down_weight, gate_bias, up_bias, down_bias, residual):
-        return _native().gated_ffn(x, gate_weight, up_weight, down_weight, gate_bias, up_bias,
-                                   down_bias, residual, ACTIVATIONS[activation], gamma)
+    if type(x) in _PLAIN and not torch.compiler.is_compiling():
+        y = _native().gated_ffn(x, gate_weight, up_weight, down_weight, gate_bias, up_bias, down_bias,
+                                residual, ACTIVATIONS[activation], gamma)
+        if y is not None:  # None: a tracer, a dispatch mode or a subclass wants the registered op
+            return y
     _check_x("gated_ffn", x)
     H = x.shape[-1]
     if gate_weight.dim() != 2 or gate_weight.shape[1] != H or 0 in gate_weight.shape:
