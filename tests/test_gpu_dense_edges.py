@@ -543,3 +543,29 @@ def test_era_far_down(T):
     got = y.double().cpu()
     assert ((got - want).abs() <= bound).all()
     assert (got[z < -20] >= 0).all() and (got[z < -20] <= GAMMA * 2.0 ** -22).all()
+
+
+@pytest.mark.parametrize("T,K,N", [(40, 72, 40), (300, 2048, 40), (300, 300, 130), (64, 4096, 264)])
+@pytest.mark.parametrize("act", ["none", "silu"])
+def test_f32_all_not_a_number(T, K, N, act):
+    """Every sum of a product formed again, with k divided and not: what fp32 gives."""
+    import velvetoptimizer_b200 as vb
+    gen = torch.Generator().manual_seed(T)
+    x, w, dy = (rand(gen, *s, dtype=F32) for s in ((T, K), (N, K), (T, N)))
+    for bad, at in ((float("nan"), slice(None)), (float("inf"), slice(0, T, 2))):
+        v = x.clone()
+        v[at] = bad
+        w1 = w.abs() + 0.5
+        lx, lw = leaf(v), leaf(w1)
+        y = vb.linear(lx, lw, activation=act)
+        if act == "none":
+            dx, dw = torch.autograd.grad(y, (lx, lw), dy.abs().cuda())
+            same_as_fp32(dx, dy.abs(), w1)
+            same_as_fp32(dw, dy.abs().t(), v)
+            same_as_fp32(y, v, w1.t())
+        else:
+            want = torch.nn.functional.silu(v @ w1.t())
+            got = y.detach().cpu()
+            assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isinf(), want.isinf())
+        # the same bits again
+        assert torch.equal(vb.linear(lx, lw, activation=act).nan_to_num(7.0), y.nan_to_num(7.0))

@@ -271,6 +271,8 @@ int run_f32(Call& c, Product p, F32Planes& planes, std::initializer_list<const F
   p.follower_b = p.epi == kEpiGated ? 3 : 0;
   DenseGemm g = plan_product(c, p, true);
   g.run_kb = kF32RunBlocks;
+  g.redo_tiles = redo_tiles(p.epi, p.M, p.N, p.groups);
+  g.arrived = c.ws.take<int>(static_cast<size_t>(g.redo_tiles) * sizeof(int));
   if (c.dry) return VMOE_OK;
   if (planes.used == kRedoWords)
     return ops_fail(c.o, VMOE_ERR_UNSUPPORTED_SHAPE, "%s: too many products in a call", p.what);

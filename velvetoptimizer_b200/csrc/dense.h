@@ -63,7 +63,10 @@ struct DenseGemm {
   int band = 0;          // n tiles per band of the tile order
   float* partial = nullptr;  // given: [splits][groups][M][ldp], and no epilogue
   int64_t ldp = 0;
-  int* redo = nullptr;  // fp32: set where a sum is not finite (dense_f32.cu)
+  // fp32 (dense_f32.cu): set where a sum is not finite, and a counter for each of its tiles
+  int* redo = nullptr;
+  int* arrived = nullptr;
+  int64_t redo_tiles = 0;
   DenseEpi epi;
   int* status = nullptr;
 };
@@ -101,6 +104,7 @@ struct RedoGemm {
   int pairs;
   int64_t am, ak, bn, bk, K;
 };
+int64_t redo_tiles(int epi, int64_t M, int64_t N, int groups);
 cudaError_t launch_dense_redo(int epi, const RedoGemm& r, int num_sms, cudaStream_t s);
 
 // Few rows (at most kSmallTokens): weights streamed once through registers (dense_small.cu).

@@ -26,9 +26,12 @@ dense_finish_kernel(const DenseGemm g) {
     const int64_t row = i / per_row, col = (i - row * per_row) * kChunk;
     float v[kChunk], u[kChunk];
     chunk_sums<EPI>(g, grp, row, col, v, u);
-    if constexpr (sizeof(T) == 4) {  // left to dense_redo_kernel
+    if constexpr (sizeof(T) == 4) {
       if (g.redo && !chunk_finite<EPI>(v, u, g.N - col)) {
+        // left to dense_redo_kernel, and marked in every split's partials
         redo = true;
+        float* p = partial_at<EPI>(g, grp, row, col);
+        for (int s = 0; s < g.splits; ++s) p[s * split_stride(g)] = __int_as_float(0x7fffffff);
         continue;
       }
     }
@@ -36,6 +39,9 @@ dense_finish_kernel(const DenseGemm g) {
   }
   if constexpr (sizeof(T) == 4) {
     if (redo) *g.redo = 1;
+    if (g.arrived && grp == 0)
+      for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < g.redo_tiles; i += gridDim.x * 256ll)
+        g.arrived[i] = 0;
   }
 }
 

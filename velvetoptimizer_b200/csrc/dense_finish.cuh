@@ -10,22 +10,44 @@ namespace vmoe {
 
 constexpr int kChunk = 8;
 
-// v, and for a gated product u (the up columns)
+// a product's partials: from one split to the next, and column col of a row (gated: the gate's)
+__device__ __forceinline__ int64_t split_stride(const DenseGemm& g) {
+  return static_cast<int64_t>(g.groups) * g.M * g.ldp;
+}
 template <int EPI>
+__device__ __forceinline__ float* partial_at(const DenseGemm& g, int grp, int64_t row, int64_t col) {
+  const int64_t pcol = EPI == kEpiGated ? (col / 128) * 256 + (col & 127) : col;
+  return g.partial + (static_cast<int64_t>(grp) * g.M + row) * g.ldp + pcol;
+}
+
+// 8 partials; from L2 where another block of this kernel may have written them
+template <bool L2>
+__device__ __forceinline__ void load_chunk(const float* p, float (&t)[kChunk]) {
+#pragma unroll
+  for (int i = 0; i < kChunk; i += 4) {
+    const float4 q = L2 ? __ldcg(reinterpret_cast<const float4*>(p + i))
+                        : *reinterpret_cast<const float4*>(p + i);
+    t[i] = q.x;
+    t[i + 1] = q.y;
+    t[i + 2] = q.z;
+    t[i + 3] = q.w;
+  }
+}
+
+// v, and for a gated product u (the up columns)
+template <int EPI, bool L2 = false>
 __device__ __forceinline__ void chunk_sums(const DenseGemm& g, int grp, int64_t row, int64_t col,
                                            float (&v)[kChunk], float (&u)[kChunk]) {
-  const int64_t split_stride = static_cast<int64_t>(g.groups) * g.M * g.ldp;
-  const int64_t pcol = EPI == kEpiGated ? (col / 128) * 256 + (col & 127) : col;
-  const float* p = g.partial + (static_cast<int64_t>(grp) * g.M + row) * g.ldp + pcol;
+  const float* p = partial_at<EPI>(g, grp, row, col);
 #pragma unroll
   for (int j = 0; j < kChunk; ++j) v[j] = u[j] = 0.f;
-  for (int s = 0; s < g.splits; ++s, p += split_stride) {
+  for (int s = 0; s < g.splits; ++s, p += split_stride(g)) {
     float t[kChunk];
-    load_row<kChunk, float>(p, t, kChunk, true);
+    load_chunk<L2>(p, t);
 #pragma unroll
     for (int j = 0; j < kChunk; ++j) v[j] += t[j];
     if constexpr (EPI == kEpiGated) {
-      load_row<kChunk, float>(p + 128, t, kChunk, true);
+      load_chunk<L2>(p + 128, t);
 #pragma unroll
       for (int j = 0; j < kChunk; ++j) u[j] += t[j];
     }
