@@ -87,6 +87,16 @@ __device__ __forceinline__ void store16_from_f(T* p, const float* in) {
   *reinterpret_cast<uint4*>(p) = v;
 }
 
+// c += a (16 x 16) b (16 x 8), fragments of one warp
+__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                         uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
 // ERA(x) = GELU_tanh(x) + gamma * softplus(x) with torch's softplus threshold of 20
 // (python/vesper/model.py:69-76).  Accurate form for the fp32 path.
 __device__ __forceinline__ float era_precise(float g, float gamma) {

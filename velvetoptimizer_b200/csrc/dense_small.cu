@@ -21,15 +21,6 @@ namespace {
 
 constexpr int UNROLL = 4;
 
-__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
-                                         uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-      "{%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
 // 8 elements of a row from k on, 0 past K or without a row
 template <bool VEC>
 __device__ __forceinline__ uint4 load8(const __nv_bfloat16* row, int64_t k, int64_t K) {
@@ -259,6 +250,9 @@ cudaError_t launch_dense_small(int dtype, int epi, const SmallGemm& g, cudaStrea
   // register form's loads too few.  One row, cold weights, register / stream form: 8192 x 2048
   // 10.9 / 9.9 us, gate|up of 2048 x 8192 14.8 / 13.3 us, but 2048 x 8192 8.9 / 9.6 us and
   // 2048 x 2048 4.1 / 4.8 us; 16 rows: 2048 x 8192 13.0 / 11.3 us, 2048 x 2048 6.4 / 5.4 us.
+  // Between 2048 and 4096 k the last slice is short and the rule is wide of the mark for a single
+  // product: 2560 x 2048 5.5 / 5.9 us with one row, 2560 x 8192 15.9 / 19.7 us with 16; a block of
+  // 2304 x 8192, whose second launch asks for its weights early, 33.3 / 27.9 and 39.2 / 41.5 us.
   if (g.vec_in && (g.K > 2048 || (g.N + rows - 1) / rows >= 6 * g.num_sms || (g.T > 8 && g.K > 1024)))
     return launch_dense_stream(epi, g, s);
   const unsigned blocks = static_cast<unsigned>((g.N + rows - 1) / rows);
