@@ -4,8 +4,10 @@
 // lo = bf16(x - hi - mid); both differences are exact, what is left is below 2^-26 |x|), so
 //   x y = lo hi + hi lo + mid mid + mid hi + hi mid + hi hi + O(2^-25) |x y|,
 // six bf16 products, exact in fp32, accumulated from the smallest up by the pair kernel as six
-// operand pairs of one product (512 x 768 x 1024: 12 to 16 us a product, its finish 5 more).  Six times the work of a bf16 product at sixteen times and more
-// the rate of the fp32 pipes; the split kernel below writes the planes (10 bytes per element).
+// operand pairs of one product (512 x 768 x 1024: 12 to 13 us a product; its finish and the redo
+// launch, which come up while it runs, add 5).  Six times the work of a bf16 product at sixteen
+// times and more the rate of the fp32 pipes; the split kernel below writes the planes (10 bytes per
+// element).
 //
 // Where such a sum leaves fp32's range the parts give NaN (infinity times a zero part, or plus and
 // minus infinity from parts of either sign) though fp32 arithmetic may give infinity: operands

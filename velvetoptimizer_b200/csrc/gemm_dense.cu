@@ -27,9 +27,10 @@
 // Every wait is bounded and reports a status code; no TMA multicast.
 //
 // Bound by the tensor cores, the activation's gradient also by its epilogue's bytes.  Block of
-// 32,768 x 2048 x 8192, bf16, fraction of a measured 1627.5 TFLOP/s: down 740 us (91 %), dx 1558
-// (87 %), gate's and up's weight gradients 1636 (83 %), gate|up keeping fp32 g and u 1700 (79 %),
-// down's weight gradient, split, 862 + 34 (75 % with its finish), dh with the gradient 1309 (52 %).
+// 32,768 x 2048 x 8192, bf16, fraction of a measured 1627.5 TFLOP/s (boxes differ by 5 %): down
+// 776 us (87 %), dx 1611 (84 %), gate's and up's weight gradients 1658 (81 %), gate|up keeping fp32
+// g and u 1764 (77 %), down's weight gradient, split, 873 + 35 (74 % with its finish), dh with the
+// gradient 1352 (50 %).
 #include <atomic>
 #include <type_traits>
 

@@ -39,7 +39,8 @@ def grad_norm(tensors, norm_type: float = 2.0) -> torch.Tensor:
     CUDA tensors on one device) as a float32 scalar on their device.
 
     ``norm_type`` is 2, 1 or ``inf``.  A tensor given twice counts once.  Sums are held in fp64
-    in a fixed order, so two calls give the same bits.  Without tensors the norm is 0.
+    in a fixed order, so two calls give the same bits.  Without tensors the norm is 0.  The norm
+    carries no gradient.
     """
     return _run(_tensors(tensors), False, -1.0, _norm_code(norm_type))
 
