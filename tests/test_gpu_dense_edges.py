@@ -569,3 +569,99 @@ def test_f32_all_not_a_number(T, K, N, act):
             assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isinf(), want.isinf())
         # the same bits again
         assert torch.equal(vb.linear(lx, lw, activation=act).nan_to_num(7.0), y.nan_to_num(7.0))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("T", [5, 90, 300])
+def test_relu_cuts_off_whatever_the_gradient_is(T, dtype):
+    """Where relu is 0 no gradient passes, an infinite or NaN one neither; where its input is NaN the
+    gradient passes, as the value does."""
+    import velvetoptimizer_b200 as vb
+    gen = torch.Generator().manual_seed(T)
+    K, N = 24, 40
+    x, w, dy = (rand(gen, *s, dtype=dtype) for s in ((T, K), (N, K), (T, N)))
+    x[3] = float("nan")
+    z = x.double() @ w.double().t()
+    for i, bad in enumerate((float("inf"), float("nan"), -float("inf"))):
+        off = (z[i] < -1).nonzero()[0]
+        dy[i, off] = bad
+    lx, lw = leaf(x), leaf(w)
+    y = vb.linear(lx, lw, activation="relu")
+    dx, dw = torch.autograd.grad(y, (lx, lw), dy.cuda())
+    keep = ~(z <= 0)
+    dz = torch.where(keep, dy.double(), 0.0)
+    want = dz @ w.double()
+    assert y[3].isnan().all() and torch.isfinite(dx).all() and dw.isnan().all()
+    lim = 4 * ref.U[dtype] if dtype == BF16 else 1e-5
+    assert float((d64(dx) - want).norm() / want.norm()) <= lim
+    # the block: dg alone is cut off (du is dh times relu's own 0)
+    wu, wd = rand(gen, N, K, dtype=dtype), torch.zeros(K, N, dtype=dtype)
+    wd[0] = 1
+    g, dout = torch.zeros(T, K, dtype=dtype), torch.zeros(T, K, dtype=dtype)
+    dout[1, 0] = float("inf")
+    g[:, 1] = 1
+    wg = torch.zeros(N, K, dtype=dtype)
+    wg[:, 1] = -1.0
+    bg = torch.zeros(N, dtype=dtype)
+    p = [leaf(t) for t in (g, wg, wu, wd, bg)]
+    y = vb.gated_ffn(*p, activation="relu")
+    dbg, = torch.autograd.grad(y, p[4], dout.cuda())
+    assert not dbg.any()
+
+
+def test_saved_tensor_hooks_and_checkpoints():
+    """What the forward keeps goes through the hooks: on the CPU and back, or formed again."""
+    from torch.utils.checkpoint import checkpoint
+
+    import velvetoptimizer_b200 as vb
+    gen = torch.Generator().manual_seed(0)
+    for dtype in (BF16, F32):
+        p = [rand(gen, 60, 72, dtype=dtype), *(rand(gen, *s, std=0.1, dtype=dtype)
+                                               for s in ((104, 72), (104, 72), (72, 104), (40, 72)))]
+        p = [t.cuda().requires_grad_() for t in p]
+        dy = rand(gen, 60, 40, dtype=dtype).cuda()
+
+        def fn(x, wg, wu, wd, wp):
+            return vb.linear(vb.gated_ffn(x, wg, wu, wd, residual=x), wp, activation="silu")
+
+        want = torch.autograd.grad(fn(*p), p, dy)
+        with torch.autograd.graph.save_on_cpu():
+            y = fn(*p)
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, p, dy), want))
+        y = checkpoint(fn, *p, use_reentrant=False)
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, p, dy), want))
+
+
+def test_f32_captured_with_and_without_infinities():
+    """A captured fp32 call replayed on finite and other inputs in turn: nothing of one replay
+    is left for the next."""
+    import velvetoptimizer_b200 as vb
+    gen = torch.Generator().manual_seed(0)
+    x = rand(gen, 150, 300, dtype=F32).cuda()
+    w = rand(gen, 130, 300, dtype=F32).cuda().requires_grad_()
+    dy = rand(gen, 150, 130, dtype=F32).cuda()
+    good = x.clone()
+    bad = x.clone()
+    bad[7, 11], bad[100] = float("inf"), float("nan")
+
+    def step():
+        lx = x.detach().requires_grad_()
+        y = vb.linear(lx, w, activation="silu")
+        return [y, *torch.autograd.grad(y, (lx, w), dy)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for values in (bad, good, bad, bad, good):
+        x.copy_(values)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.detach().clone() for t in out]
+        for a, b in zip(got, step()):
+            assert torch.equal(a.isnan(), b.isnan()) and torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0))
+    assert torch.isfinite(got[0]).all()

@@ -43,7 +43,7 @@ template <int ACT>
 __device__ __forceinline__ void act_grad1(float z, float gamma, float& a, float& d) {
   if constexpr (ACT == kActRelu) {
     a = z < 0.f ? 0.f : z;
-    d = z > 0.f ? 1.f : 0.f;
+    d = z <= 0.f ? 0.f : 1.f;  // NaN hands the gradient on, as the value stays NaN
   } else if constexpr (ACT == kActSilu) {
     const float s = sigmoid1(z);
     a = z * s;
@@ -146,7 +146,7 @@ template <int ACT>
 __device__ __forceinline__ void act_grad2(float2 z, float gamma, float2& a, float2& d) {
   if constexpr (ACT == kActRelu) {
     a = act_value2<kActRelu>(z, gamma);
-    d = make_float2(z.x > 0.f ? 1.f : 0.f, z.y > 0.f ? 1.f : 0.f);
+    d = make_float2(z.x <= 0.f ? 0.f : 1.f, z.y <= 0.f ? 0.f : 1.f);
   } else if constexpr (ACT == kActSilu) {
     const float2 s = rcp_2(add2(ex2_2(mul2(z, both(-kLog2e))), both(1.f)));
     a = mul2(z, s);
@@ -167,6 +167,19 @@ __device__ __forceinline__ void act_grad2(float2 z, float gamma, float2& a, floa
     a = z;
     d = both(1.f);
   }
+}
+
+// v act'(z), where d is act'(z): what relu cuts off is 0 though v be infinite or NaN
+template <int ACT>
+__device__ __forceinline__ float times_slope(float v, float d) {
+  if constexpr (ACT == kActRelu) return d == 0.f ? 0.f : v;
+  return v * d;
+}
+template <int ACT>
+__device__ __forceinline__ float2 times_slope2(float2 v, float2 d) {
+  if constexpr (ACT == kActRelu)
+    return make_float2(times_slope<ACT>(v.x, d.x), times_slope<ACT>(v.y, d.y));
+  return mul2(v, d);
 }
 
 // v[i] = act(v[i]); N even

@@ -69,7 +69,7 @@ dense_dz_kernel(const DzArgs a, bool vec_dy, bool vec_z, bool vec_dz) {
         float d[W];
         act_grads<kFast, decltype(A)::value>(g, d, a.gamma);
 #pragma unroll
-        for (int j = 0; j < W; ++j) v[j] *= d[j];
+        for (int j = 0; j < W; ++j) v[j] = times_slope<decltype(A)::value>(v[j], d[j]);
       });
     };
     auto finish = [&](float (&v)[W], int64_t r) {

@@ -84,7 +84,7 @@ __device__ __forceinline__ void finish_chunk(const DenseGemm& g, int grp, int64_
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         const float a = gg[j];
-        gg[j] = v[j] * u[j] * d[j];
+        gg[j] = times_slope<decltype(A)::value>(v[j] * u[j], d[j]);
         u[j] = v[j] * a;
       }
     });

@@ -657,8 +657,9 @@ gemm_dense_kernel(const __grid_constant__ DenseMaps maps, const __grid_constant_
                 float2 a0, d0, a1, d1;
                 act_grad2<decltype(A)::value>(make_float2(gv.x, gv.y), ep.gamma, a0, d0);
                 act_grad2<decltype(A)::value>(make_float2(gv.z, gv.w), ep.gamma, a1, d1);
-                const float2 g0 = mul2(mul2(p0, make_float2(uv.x, uv.y)), d0), u0 = mul2(p0, a0);
-                const float2 g1 = mul2(mul2(p1, make_float2(uv.z, uv.w)), d1), u1 = mul2(p1, a1);
+                const float2 g0 = times_slope2<decltype(A)::value>(mul2(p0, make_float2(uv.x, uv.y)), d0);
+                const float2 g1 = times_slope2<decltype(A)::value>(mul2(p1, make_float2(uv.z, uv.w)), d1);
+                const float2 u0 = mul2(p0, a0), u1 = mul2(p1, a1);
                 uint32_t* tg = reinterpret_cast<uint32_t*>(dg) + 8 * half + 2 * k;
                 uint32_t* tu = reinterpret_cast<uint32_t*>(du) + 8 * half + 2 * k;
                 tg[0] = pack_bf16x2(g0.x, g0.y);
