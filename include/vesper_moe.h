@@ -388,10 +388,10 @@ VMOE_API int vmoe_linear_forward(vmoe_ops* ops, const vmoe_linear* d, const void
                                  const void* weight, const void* bias, const void* residual,
                                  void* y, void* z, void* workspace, size_t workspace_bytes,
                                  void* stream);
-/* dz = dy act'(z) (relu: 0 where z <= 0, whatever dy is);  dx = dz W;  dW = dz^T x;  db = column sums of dz (fp32 sums, fixed order:
- * two runs give the same bits).  Each output may be null; they are overwritten.  The
- * residual's gradient is dy itself.  dy [T, N] has row pitch lddy: N, or for bf16 any larger
- * multiple of 8 (fp32: any), and x's alignment. */
+/* dz = dy act'(z) (relu: 0 where z <= 0, whatever dy is);  dx = dz W;  dW = dz^T x;
+ * db = column sums of dz (fp32 sums, fixed order: two runs give the same bits).  Each output may
+ * be null; they are overwritten.  The residual's gradient is dy itself.  dy [T, N] has row pitch
+ * lddy: N, or for bf16 any larger multiple of 8 (fp32: any), and x's alignment. */
 VMOE_API int vmoe_linear_backward(vmoe_ops* ops, const vmoe_linear* d, const void* x,
                                   const void* weight, const void* z, const void* dy, int64_t lddy,
                                   void* dx, void* dweight, void* dbias, void* workspace,

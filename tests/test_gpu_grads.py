@@ -325,3 +325,15 @@ def test_overlapping_gradients_that_are_not_dense_are_refused():
         q.grad = t
     vb.clip_grad_norm_(ps, 1.0)
     assert torch.allclose(wide, torch.full_like(wide, 1 / math.sqrt(2400)))
+
+
+def test_expanded_tensors_count_once():
+    """The same expansion twice is one tensor; another one of the same memory overlaps it."""
+    import velvetoptimizer_b200 as vb
+    row = torch.randn(1, 60, device="cuda")
+    e = row.expand(40, 60)
+    want = norm64([e], 2.0)
+    assert float(vb.grad_norm([e, e, row.expand(40, 60)])) == pytest.approx(want, rel=2.0 ** -22)
+    for other in (row.expand(10, 60), row):
+        with pytest.raises(ValueError, match="overlap"):
+            vb.grad_norm([e, other])

@@ -650,9 +650,11 @@ struct GradTable {
 // outermost first; the last dimension is the run of consecutive bytes.
 struct Footprint {
   uintptr_t at = 0, end = 0;
+  int64_t numel = 0;
   std::vector<std::pair<int64_t, int64_t>> dims;  // size, stride
 
-  explicit Footprint(const Tensor& t) : at(reinterpret_cast<uintptr_t>(t.data_ptr())) {
+  explicit Footprint(const Tensor& t)
+      : at(reinterpret_cast<uintptr_t>(t.data_ptr())), numel(t.numel()) {
     const int64_t elt = static_cast<int64_t>(t.element_size());
     std::vector<std::pair<int64_t, int64_t>> d{{elt, 1}};
     for (int64_t k = 0; k < t.dim(); ++k)
@@ -667,7 +669,7 @@ struct Footprint {
         dims.push_back(q);
     }
   }
-  bool operator==(const Footprint& o) const { return at == o.at && dims == o.dims; }
+  bool operator==(const Footprint& o) const { return at == o.at && numel == o.numel && dims == o.dims; }
 };
 
 // Whether two footprints share a byte: is there a sum of a's multiples minus b's that equals the
